@@ -180,3 +180,132 @@ def attn_bwd_window(qkv, d_out, cu_seqlens, n_q: int, n_kv: int, head_dim: int, 
         y = ref.attention_varlen(x, cu_seqlens, n_q, n_kv, head_dim, scale, window=window)
         (dx,) = torch.autograd.grad(y, x, d_out.float())
     return dx.to(qkv.dtype)
+
+
+# ---------------------------------------------------------------------------------- speculative decoding
+def _ancestors(parents: list, t: int) -> list:
+    """The node at position ``t`` and its ancestors; nothing for padding."""
+    if parents[t] < -1:
+        return []
+    seen = [t]
+    while 0 <= parents[t] < t:
+        t = parents[t]
+        seen.append(t)
+    return sorted(seen)
+
+
+def _spans(cu_nodes, total: int, max_nodes: int) -> list:
+    """(first row, nodes) of every sequence, held inside the batch."""
+    cu = cu_nodes.tolist()
+    first = [min(max(c, 0), total) for c in cu[:-1]]
+    return [(lo, min(max(hi - lo, 0), max_nodes, total - lo)) for lo, hi in zip(first, cu[1:])]
+
+
+def tree_attn(qkv, k_cache, v_cache, block_table, ctx, cu_nodes, parents, n_q: int, n_kv: int, head_dim: int, scale: float, max_nodes: int, out=None):
+    """Attention of drafted token trees over the paged cache, sequence by sequence."""
+    from . import fused
+
+    fused._check_tree_attn(qkv, k_cache, v_cache, block_table, ctx, cu_nodes, parents, n_q, n_kv, head_dim, scale, max_nodes, out, qkv.dtype)
+    N, group, page = qkv.shape[0], n_q // n_kv, fused.KV_PAGE
+    if out is None:
+        out = torch.empty(N, n_q * head_dim, dtype=qkv.dtype, device=qkv.device)
+    par = parents.tolist()
+    for b, (lo, n) in enumerate(_spans(cu_nodes, N, max_nodes)):
+        if n == 0:
+            continue
+        x = qkv[lo:lo + n].float().view(n, n_q + 2 * n_kv, head_dim)
+        c = min(max(int(ctx[b]), 0), block_table.shape[1] * page)
+        at = torch.arange(c, device=qkv.device)
+        blk = block_table[b].long()[at // page]
+        there = ((blk >= 0) & (blk < k_cache.shape[0])).view(-1, 1, 1)
+        blk = torch.where(there.view(-1), blk, 0)
+        old_k = k_cache[blk, :, at % page].float().masked_fill(~there, 0.0) if c else x[:0, :n_kv]
+        old_v = v_cache[blk, :, at % page].float().masked_fill(~there, 0.0) if c else x[:0, :n_kv]
+        k = torch.cat([old_k, x[:, n_q:n_q + n_kv]]).repeat_interleave(group, 1)
+        v = torch.cat([old_v, x[:, n_q + n_kv:]]).repeat_interleave(group, 1)
+        live = torch.ones(n, c + n, dtype=torch.bool)
+        live[:, c:] = False
+        for t in range(n):
+            live[t, [c + a for a in _ancestors(par[lo:lo + n], t)]] = True
+        s = torch.einsum("nhd,jhd->hnj", x[:, :n_q], k) * scale
+        s = s.masked_fill(~live.to(s.device), float("-inf"))
+        o = torch.einsum("hnj,jhd->nhd", torch.softmax(s, -1), v).reshape(n, -1)
+        pad = torch.tensor([p < -1 for p in par[lo:lo + n]], device=qkv.device)
+        out[lo:lo + n] = o.masked_fill(pad[:, None], 0.0).to(qkv.dtype)
+    return out
+
+
+def verify_tree(logits, tokens, parents, cu_nodes, temperature, u_accept, u_sample, max_nodes: int, draft_probs=None):
+    """Verification of drafted trees, node by node in 64 bits; returns (count, tokens, path, logprobs)."""
+    from . import fused
+
+    fused._check_verify_tree(logits, tokens, parents, cu_nodes, temperature, u_accept, u_sample, max_nodes, draft_probs, logits.dtype)
+    (N, V), B, dev = logits.shape, temperature.shape[0], logits.device
+    count = torch.zeros(B, dtype=torch.int32)
+    emitted = torch.full((B, max_nodes), -1, dtype=torch.int64)
+    path = torch.full((B, max_nodes), -1, dtype=torch.int32)
+    logprobs = torch.zeros(B, max_nodes, dtype=torch.float32)
+    par, tok, coin = parents.tolist(), tokens.tolist(), u_accept.double().tolist()
+    for b, (lo, n) in enumerate(_spans(cu_nodes, N, max_nodes)):
+        if n == 0:
+            continue
+        t = float(temperature[b])
+
+        def arrive(node):
+            z = logits[node].float() / (t if t > 0 else 1.0)
+            lp = torch.log_softmax(z.double(), -1)
+            if t > 0:
+                return lp, lp.exp()
+            p = torch.zeros_like(lp)
+            p[int(torch.argmax((logits[node] == logits[node].max()).int()))] = 1.0
+            return lp, p
+
+        cur, k = lo, 0
+        lp, r = arrive(cur)
+        path[b, 0] = cur
+        for j in range(1, n):
+            if par[lo + j] != cur - lo:
+                continue
+            x = tok[lo + j]
+            known = 0 <= x < V
+            q = draft_probs[cur].double() if draft_probs is not None else None
+            qx = 1.0 if q is None else float(q[x]) if known else 0.0
+            if known and coin[lo + j] * qx < float(r[x]):
+                emitted[b, k], logprobs[b, k] = x, float(lp[x])
+                k, cur = k + 1, lo + j
+                path[b, k] = cur
+                lp, r = arrive(cur)
+                continue
+            left = r.clone()
+            if q is not None:
+                left = (r - q).clamp(min=0.0)
+            elif known:
+                left[x] = 0.0
+            if float(left.sum()) > 0:
+                r = left / left.sum()
+        c = r.cumsum(0)
+        over = torch.nonzero(c > float(u_sample[b].double()) * c[-1])
+        live = torch.nonzero(r > 0)
+        x = int(over[0]) if len(over) else int(live[-1]) if len(live) else 0
+        emitted[b, k], logprobs[b, k], count[b] = x, float(lp[x]), k + 1
+    return count.to(dev), emitted.to(dev), path.to(dev), logprobs.to(dev)
+
+
+def kv_commit_(qkv_layers, k_cache, v_cache, block_table, ctx, path, n_q: int, n_kv: int, head_dim: int) -> None:
+    """Keys and values of the accepted nodes into the paged cache of every layer."""
+    from . import fused
+
+    fused._check_kv_commit(qkv_layers, k_cache, v_cache, block_table, ctx, path, n_q, n_kv, head_dim, k_cache.dtype)
+    page, (N, L) = fused.KV_PAGE, (qkv_layers[0].shape[0], len(qkv_layers))
+    for b, nodes in enumerate(path.tolist()):
+        for j, node in enumerate(nodes):
+            at = int(ctx[b]) + j
+            if not 0 <= node < N or at < 0 or at // page >= block_table.shape[1]:
+                continue
+            blk = int(block_table[b, at // page])
+            if not 0 <= blk < k_cache.shape[1]:
+                continue
+            for i in range(L):
+                x = qkv_layers[i][node].view(n_q + 2 * n_kv, head_dim)
+                k_cache[i, blk, :, at % page] = x[n_q:n_q + n_kv]
+                v_cache[i, blk, :, at % page] = x[n_q + n_kv:]

@@ -7,7 +7,9 @@ call fails in Python instead of on the device.
 
 from __future__ import annotations
 
+import ctypes
 import functools
+import math
 
 import torch
 
@@ -381,3 +383,187 @@ def attn_bwd_window(qkv, d_out, cu_seqlens, n_q: int, n_kv: int, head_dim: int, 
         y = _window_attention(x, cu_seqlens, n_q, n_kv, head_dim, scale, window, max_len)
         (dx,) = torch.autograd.grad(y, x, d_out.reshape(y.shape))
     return dx
+
+
+# ---------------------------------------------------------------------------------- speculative decoding
+KV_PAGE = 64         # tokens of one page of the paged KV cache
+MAX_TREE_NODES = 64  # nodes of one sequence's draft tree (its newest token included)
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with the current stream of ``device`` as the last argument, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream_ptr())
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_ptr())
+
+
+def _check_index(t: torch.Tensor, dtype, shape: tuple, device, name: str) -> None:
+    if t.dtype != dtype or t.device != device:
+        raise TypeError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor of shape {shape}, got {tuple(t.shape)}")
+
+
+def _check_rows(t: torch.Tensor, dtype, width: int, device, name: str) -> None:
+    if t.dtype != dtype or t.device != device:
+        raise TypeError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
+    if t.dim() != 2 or t.shape[1] != width or t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: expected [N, {width}], 16-byte aligned, contiguous rows with a stride that is a multiple of 8, got {tuple(t.shape)}")
+
+
+def _check_cache(k_cache, v_cache, block_table, ctx, n_kv: int, head_dim: int, dtype, device, lead: tuple = ()) -> None:
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.dtype != dtype or t.device != device:
+            raise TypeError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
+        if t.dim() != 4 + len(lead) or tuple(t.shape[:len(lead)]) != lead or tuple(t.shape[-3:]) != (n_kv, KV_PAGE, head_dim) or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{name}: expected a contiguous [{''.join(f'{n}, ' for n in lead)}blocks, {n_kv}, {KV_PAGE}, {head_dim}] cache, got {tuple(t.shape)}")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have the same shape")
+    if ctx.dim() != 1:
+        raise ValueError(f"ctx: expected [B], got {tuple(ctx.shape)}")
+    _check_index(ctx, torch.int32, (ctx.shape[0],), device, "ctx")
+    if block_table.dtype != torch.int32 or block_table.device != device:
+        raise TypeError(f"block_table: expected int32 on {device}, got {block_table.dtype} on {block_table.device}")
+    if block_table.dim() != 2 or block_table.shape[0] != ctx.shape[0] or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table: expected [{ctx.shape[0]}, pages] with contiguous rows, got {tuple(block_table.shape)}")
+
+
+def _check_tree_attn(qkv, k_cache, v_cache, block_table, ctx, cu_nodes, parents, n_q: int, n_kv: int, head_dim: int, scale: float, max_nodes: int,
+                     out, dtype) -> None:
+    dev = qkv.device
+    if head_dim != 128 or n_kv < 1 or n_q % n_kv or not 1 <= n_q // n_kv <= 128:
+        raise ValueError(f"tree attention: head_dim 128 and up to 128 query heads per KV head, got {n_q} / {n_kv} heads of {head_dim}")
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"tree attention needs a positive finite scale, got {scale}")
+    if not 1 <= max_nodes <= MAX_TREE_NODES:
+        raise ValueError(f"draft trees have 1 to {MAX_TREE_NODES} nodes a sequence, got max_nodes = {max_nodes}")
+    _check_rows(qkv, dtype, (n_q + 2 * n_kv) * head_dim, dev, "qkv")
+    _check_cache(k_cache, v_cache, block_table, ctx, n_kv, head_dim, dtype, dev)
+    _check_index(cu_nodes, torch.int32, (ctx.shape[0] + 1,), dev, "cu_nodes")
+    _check_index(parents, torch.int32, (qkv.shape[0],), dev, "parents")
+    if out is not None:
+        _check_index(out, dtype, (qkv.shape[0], n_q * head_dim), dev, "out")
+
+
+def _check_verify_tree(logits, tokens, parents, cu_nodes, temperature, u_accept, u_sample, max_nodes: int, draft_probs, dtype) -> None:
+    dev = logits.device
+    if logits.dtype != dtype:
+        raise TypeError(f"logits: expected {dtype}, got {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] < 1 or logits.stride(1) != 1:
+        raise ValueError(f"logits: expected [N, V] with contiguous rows, got {tuple(logits.shape)}")
+    if not 1 <= max_nodes <= MAX_TREE_NODES:
+        raise ValueError(f"draft trees have 1 to {MAX_TREE_NODES} nodes a sequence, got max_nodes = {max_nodes}")
+    if temperature.dim() != 1:
+        raise ValueError(f"temperature: expected [B], got {tuple(temperature.shape)}")
+    N, B = logits.shape[0], temperature.shape[0]
+    _check_index(tokens, torch.int64, (N,), dev, "tokens")
+    _check_index(parents, torch.int32, (N,), dev, "parents")
+    _check_index(cu_nodes, torch.int32, (B + 1,), dev, "cu_nodes")
+    _check_index(temperature, torch.float32, (B,), dev, "temperature")
+    _check_index(u_accept, torch.float32, (N,), dev, "u_accept")
+    _check_index(u_sample, torch.float32, (B,), dev, "u_sample")
+    if draft_probs is not None:
+        if draft_probs.dtype != torch.float32 or draft_probs.device != dev:
+            raise TypeError(f"draft_probs: expected torch.float32 on {dev}, got {draft_probs.dtype} on {draft_probs.device}")
+        if draft_probs.shape != logits.shape or draft_probs.stride(1) != 1:
+            raise ValueError(f"draft_probs: expected {tuple(logits.shape)} with contiguous rows, got {tuple(draft_probs.shape)}")
+
+
+def _check_kv_commit(qkv_layers, k_cache, v_cache, block_table, ctx, path, n_q: int, n_kv: int, head_dim: int, dtype) -> None:
+    L = len(qkv_layers)
+    if L < 1 or k_cache.dim() < 1 or L != k_cache.shape[0]:
+        raise ValueError(f"kv_commit_: {L} layers of qkv for a cache of shape {tuple(k_cache.shape)}")
+    if head_dim != 128 or n_kv < 1 or n_q < 0:
+        raise ValueError(f"kv_commit_: head_dim 128, got {n_q} / {n_kv} heads of {head_dim}")
+    first = qkv_layers[0]
+    dev, shape, ld = first.device, first.shape, first.stride(0)
+    _check_rows(first, dtype, (n_q + 2 * n_kv) * head_dim, dev, "qkv of layer 0")
+    for i, t in enumerate(qkv_layers):
+        if t.dtype != dtype or t.device != dev or t.shape != shape or t.stride(0) != ld or t.stride(1) != 1 or t.data_ptr() % 16:
+            raise ValueError(f"kv_commit_: the qkv rows of layer {i} are not laid out as those of layer 0")
+    _check_cache(k_cache, v_cache, block_table, ctx, n_kv, head_dim, dtype, dev, (L,))
+    if path.dim() != 2:
+        raise ValueError(f"path: expected [B, P], got {tuple(path.shape)}")
+    _check_index(path, torch.int32, (ctx.shape[0], path.shape[1]), dev, "path")
+
+
+def _need_cuda(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda:
+        raise TypeError(f"{name}: expected a CUDA tensor, got one on {t.device}")
+
+
+def tree_attn(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, ctx: torch.Tensor,
+              cu_nodes: torch.Tensor, parents: torch.Tensor, n_q: int, n_kv: int, head_dim: int, scale: float, max_nodes: int,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted token trees over the paged KV cache; returns bf16 [N, n_q * head_dim].
+
+    ``qkv`` bf16 [N, (n_q + 2 n_kv) * head_dim] (rows may be strided by a multiple of 8 elements) holds the post-RoPE rows of
+    the nodes of all sequences, sequence ``b`` owning rows ``cu_nodes[b] .. cu_nodes[b + 1]`` (int32 [B + 1]), at most
+    ``max_nodes`` <= 64 of them.  A node attends to the first ``ctx[b]`` (int32 [B]) cached tokens of its sequence, found
+    through ``block_table`` (int32 [B, pages]) in the caches [blocks, n_kv, 64, head_dim], to its ancestors and to itself.
+    ``parents`` (int32 [N]) gives a node's parent as a position inside its own sequence, smaller than the node's own; -1 is a
+    root, -2 padding (its row of the result is zero).  The nodes' keys and values are read from ``qkv``: the cache does not
+    hold them and is not written.  Cache rows at or past ``ctx`` may hold anything; a page that is not in the cache reads as zeros.  One node per sequence is an ordinary
+    decode step.  With ``out`` the rows at and past ``cu_nodes[B]`` are left as they are.  head_dim 128, bf16 only."""
+    _need_cuda(qkv, "qkv")
+    _check_tree_attn(qkv, k_cache, v_cache, block_table, ctx, cu_nodes, parents, n_q, n_kv, head_dim, scale, max_nodes, out, torch.bfloat16)
+    dev, N, B = qkv.device, qkv.shape[0], ctx.shape[0]
+    if out is None:
+        out = torch.empty(N, n_q * head_dim, dtype=torch.bfloat16, device=dev)
+    _call_on(dev, "b200_tree_attn", ptr(qkv), qkv.stride(0), ptr(k_cache), ptr(v_cache), k_cache.shape[0], ptr(block_table),
+             block_table.stride(0), block_table.shape[1], ptr(ctx), ptr(cu_nodes), ptr(parents), B, N, max_nodes, n_q, n_kv, head_dim, scale,
+             ptr(out))
+    return out
+
+
+def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_nodes: torch.Tensor, temperature: torch.Tensor,
+                u_accept: torch.Tensor, u_sample: torch.Tensor, max_nodes: int, draft_probs: torch.Tensor | None = None):
+    """Verify drafted token trees against the target's probabilities; every emitted token is distributed as the target's own
+    sample.  Returns ``(count, tokens, path, logprobs)``:
+
+    * ``count`` int32 [B]: tokens emitted for each sequence, the accepted drafts and one more (0 for a sequence without nodes);
+    * ``tokens`` int64 [B, max_nodes]: the emitted tokens, -1 behind them;
+    * ``path`` int32 [B, max_nodes]: the batch rows of the sequence's first node and of the accepted ones, ``count`` in all and
+      -1 behind them: the rows whose keys and values belong into the cache (``kv_commit_``);
+    * ``logprobs`` fp32 [B, max_nodes]: log-probability of each emitted token under the target's distribution at ``temperature``
+      (at temperature 0 under the plain softmax), 0 behind them.
+
+    ``logits`` bf16 [N, V] (rows may be strided): what the target predicts AFTER each node.  ``tokens`` int64 [N], ``parents`` /
+    ``cu_nodes`` as for ``tree_attn``.  ``temperature`` fp32 [B], 0 = greedy.  From a sequence's first node on, the children of
+    the current node are tried in the order of their positions with ``r = p``: child ``x`` is accepted if
+    ``u_accept[x] * q(x) < r(x)``, else ``r`` becomes the normalised ``max(r - q, 0)``; when none is left, the last token is the
+    first whose cumulative share of ``r`` exceeds ``u_sample``.  ``u_accept`` fp32 [N] and ``u_sample`` fp32 [B] are uniform
+    numbers in [0, 1).  ``draft_probs`` fp32 [N, V] holds the distribution that the children of each node were drawn from
+    (independently of each other); without it a draft counts as certain, ``q(x) = 1``, and a rejected token leaves ``r``."""
+    _need_cuda(logits, "logits")
+    _check_verify_tree(logits, tokens, parents, cu_nodes, temperature, u_accept, u_sample, max_nodes, draft_probs, torch.bfloat16)
+    dev, (N, V), B = logits.device, logits.shape, temperature.shape[0]
+    count = torch.empty(B, dtype=torch.int32, device=dev)
+    out_tokens = torch.empty(B, max_nodes, dtype=torch.int64, device=dev)
+    path = torch.empty(B, max_nodes, dtype=torch.int32, device=dev)
+    logprobs = torch.empty(B, max_nodes, dtype=torch.float32, device=dev)
+    _call_on(dev, "b200_verify_tree", ptr(logits), logits.stride(0), V, ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0),
+             ptr(tokens), ptr(parents), ptr(cu_nodes), B, N, max_nodes, ptr(temperature), ptr(u_accept), ptr(u_sample), ptr(count),
+             ptr(out_tokens), ptr(path), ptr(logprobs))
+    return count, out_tokens, path, logprobs
+
+
+def kv_commit_(qkv_layers, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, ctx: torch.Tensor, path: torch.Tensor,
+               n_q: int, n_kv: int, head_dim: int) -> None:
+    """Write the keys and values of the accepted nodes into the paged cache, all layers in one launch.
+
+    ``qkv_layers``: for each layer the fused qkv rows [N, (n_q + 2 n_kv) * head_dim] that ``tree_attn`` read (bf16, one row
+    stride for all of them); the caches are [layers, blocks, n_kv, 64, head_dim].  Node ``path[b, j]`` (int32 [B, P], from
+    ``verify_tree``; negative = nothing) goes to position ``ctx[b] + j`` of sequence ``b``, the next free ones.  Positions
+    outside the block table and pages outside the cache are not written."""
+    L = len(qkv_layers)
+    if L:
+        _need_cuda(qkv_layers[0], "qkv")
+    _check_kv_commit(qkv_layers, k_cache, v_cache, block_table, ctx, path, n_q, n_kv, head_dim, torch.bfloat16)
+    first = qkv_layers[0]
+    pointers = (ctypes.c_void_p * L)(*[t.data_ptr() for t in qkv_layers])
+    _call_on(first.device, "b200_kv_commit", ctypes.addressof(pointers), L, first.stride(0), first.shape[0], ptr(k_cache), ptr(v_cache),
+             k_cache.stride(0), k_cache.shape[1], ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(ctx), ptr(path),
+             ctx.shape[0], path.shape[1], n_q, n_kv, head_dim)

@@ -57,6 +57,9 @@ _SIGNATURES = {
     "b200_paged_decode_variant": [I],
     "b200_rope_kv_decode": [P, P, P, P, P, I, I, I, I, P],
     "b200_sample": [P, L, I, I, P, P, P, P, P, P, P],
+    "b200_tree_attn": [P, L, P, P, I, P, L, I, P, P, P, I, I, I, I, I, I, F, P, P],
+    "b200_verify_tree": [P, L, I, P, L, P, P, P, I, I, I, P, P, P, P, P, P, P, P],
+    "b200_kv_commit": [P, I, L, I, P, P, L, I, P, L, I, P, P, I, I, I, I, I, P],
     "b200_attn_fwd": [P, P, P, P, P, I, I, I, I, I, I, F, P],
     "b200_attn_bwd": [P, P, P, P, P, P, P, P, I, I, I, I, I, I, F, P],
 }

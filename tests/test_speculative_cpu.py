@@ -1,0 +1,164 @@
+"""Speculative-decoding operators on the CPU: the PyTorch restatements against 64-bit oracles, and the refusals, which the kernel
+wrappers share with them."""
+
+import pytest
+import torch
+
+from open_instruct_b200.ops import emulated, fused
+from _speculative import DIM, PAGE, attn_oracle, logprob_bound, make_attn, make_verify, verify_oracle
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (7, 1), (2, 2)])
+@pytest.mark.parametrize("shape", ["chain", "tree", "star"])
+def test_tree_attention(heads, kv_heads, shape):
+    a = make_attn(heads, kv_heads, [0, 1, 63, 64, 65, 200, 10], [1, 3, 0, 5, 9, 2, 4], shape, dtype=torch.float32, row_extra=8, table_extra=1)
+    out = emulated.tree_attn(**a)
+    ref, mag = attn_oracle(a)
+    assert ((out.double() - ref).abs() <= 2.0 ** -13 * mag + 1e-30).all()   # fp32 throughout: the bound's fp32 share
+
+
+def test_tree_attention_padding_and_bad_pages():
+    a = make_attn(4, 2, [70, 130], [6, 5], dtype=torch.float32, extra_rows=3)
+    a["parents"][[4, 5, 10]] = -2
+    a["parents"][9] = 0
+    a["block_table"][0, 1] = -3
+    a["block_table"][1, 0] = a["k_cache"].shape[0]
+    out = torch.full((14, 4 * DIM), 7.0)
+    assert emulated.tree_attn(**a, out=out) is out
+    ref, mag = attn_oracle(a)
+    assert ((out[:11].double() - ref[:11]).abs() <= 2.0 ** -13 * mag[:11] + 1e-30).all()
+    assert (out[[4, 5, 10]] == 0).all() and (out[11:] == 7.0).all()
+
+
+@pytest.mark.parametrize("drafted", [False, True])
+@pytest.mark.parametrize("shape", ["chain", "tree", "star"])
+@pytest.mark.parametrize("vocab", [1, 2, 97, 1000])
+def test_verification(vocab, shape, drafted):
+    a = make_verify([3, 1, 0, 7, 5, 12, 2, 4] * 3, vocab, shape, drafted, temps=(1.0, 0.0, 0.6, 1.7, 1.0), seed=vocab, row_extra=3, extra_rows=2)
+    got, want = emulated.verify_tree(**a), verify_oracle(a)
+    for x, y in zip(got[:3], want[:3]):
+        assert torch.equal(x, y.to(x.dtype))
+    assert (got[3].double() - want[3]).abs().max() <= logprob_bound(vocab)
+
+
+@pytest.mark.parametrize("drafted", [False, True])
+def test_emitted_tokens_follow_the_target(drafted):
+    """The first emitted token over many independent draws has the target's distribution, whatever is drafted: each bin's count is
+    within six standard deviations."""
+    g = torch.Generator().manual_seed(5)
+    V, trials, kids = 6, 4000, 3
+    z = torch.tensor([1.0, 0.0, -1.0, 2.0, 0.5, -3.0]).bfloat16()
+    q = torch.softmax(torch.tensor([0.0, 1.0, 0.5, 0.0, 2.0, -1.0]), -1)
+    counts = [kids + 1] * trials
+    a = make_verify(counts, V, "star", seed=1)
+    a["logits"] = z.expand(len(a["tokens"]), V).contiguous()
+    a["tokens"] = torch.multinomial(q, len(a["tokens"]), replacement=True, generator=g)
+    a["draft_probs"] = q.expand(len(a["tokens"]), V).contiguous() if drafted else None
+    _, tokens, _, _ = emulated.verify_tree(**a)
+    p = torch.softmax(z.double(), -1)
+    seen = torch.bincount(tokens[:, 0], minlength=V).double()
+    assert ((seen - trials * p).abs() <= 6 * (trials * p * (1 - p)).sqrt()).all(), (seen / trials, p)
+
+
+def _commit_inputs(layers, kv_heads=2, heads=4, dtype=torch.float32, device="cpu"):
+    a = make_attn(heads, kv_heads, [0, 60, 64, 127, 200], [3, 8, 1, 5, 2], dtype=dtype, garbage=False, table_extra=1, device=device, row_extra=16)
+    g = torch.Generator().manual_seed(3)
+    total = a["k_cache"].shape[0] + 8
+    table = torch.randperm(total, generator=g)[: 5 * a["block_table"].shape[1]]
+    total = max(total, 5 * a["block_table"].shape[1])
+    table = torch.randperm(total, generator=g)[: 5 * a["block_table"].shape[1]].view(5, -1).int().to(device)
+    width = (heads + 2 * kv_heads) * DIM
+    qkv = [torch.randn(19, width + 16, generator=g).to(device, dtype)[:, :width] for _ in range(layers)]
+    path = torch.full((5, 4), -1, dtype=torch.int32)
+    path[0, :3] = torch.tensor([0, 1, 2])
+    path[1] = torch.tensor([3, 5, 6, 10])
+    path[2, 0] = 11
+    path[3, :2] = torch.tensor([12, 16])
+    shape = (layers, total, kv_heads, PAGE, DIM)
+    k, v = (torch.randn(shape, generator=g).to(device, dtype) for _ in range(2))
+    return dict(qkv_layers=qkv, k_cache=k, v_cache=v, block_table=table, ctx=a["ctx"], path=path.to(device), n_q=heads, n_kv=kv_heads, head_dim=DIM)
+
+
+def _commit_oracle(a):
+    k, v = a["k_cache"].clone(), a["v_cache"].clone()
+    hq, hk = a["n_q"], a["n_kv"]
+    for b, nodes in enumerate(a["path"].tolist()):
+        for j, node in enumerate(nodes):
+            pos = int(a["ctx"][b]) + j
+            if not 0 <= node < a["qkv_layers"][0].shape[0] or pos // PAGE >= a["block_table"].shape[1]:
+                continue
+            blk = int(a["block_table"][b, pos // PAGE])
+            if not 0 <= blk < k.shape[1]:
+                continue
+            for i, x in enumerate(a["qkv_layers"]):
+                row = x[node].view(hq + 2 * hk, DIM)
+                k[i, blk, :, pos % PAGE], v[i, blk, :, pos % PAGE] = row[hq:hq + hk], row[hq + hk:]
+    return k, v
+
+
+@pytest.mark.parametrize("bad", [False, True])
+def test_commit(bad):
+    a = _commit_inputs(3)
+    if bad:   # a page outside the cache on either side, a node outside the batch, a context past the table
+        a["block_table"][1, 0], a["block_table"][0, 0], a["path"][3, 1], a["ctx"][4] = -1, a["k_cache"].shape[1], 19, 64 * a["block_table"].shape[1]
+        a["path"][4, 0] = 17
+    want = _commit_oracle(a)
+    emulated.kv_commit_(**a)
+    assert torch.equal(a["k_cache"], want[0]) and torch.equal(a["v_cache"], want[1])
+
+
+def _change(a, **kw):
+    return {**a, **kw}
+
+
+def test_refusals_of_tree_attention():
+    a = make_attn(4, 2, [70, 3], [3, 2], dtype=torch.float32)
+    with pytest.raises(TypeError, match="CUDA"):
+        fused.tree_attn(**a)
+    odd = torch.zeros(5, 8 * DIM + 4)[:, : 8 * DIM]
+    bad = [
+        dict(head_dim=64), dict(n_kv=3), dict(n_kv=0), dict(n_q=2 * 129), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
+        dict(scale=float("nan")), dict(max_nodes=0), dict(max_nodes=65), dict(qkv=a["qkv"][:, :-DIM]), dict(qkv=odd), dict(qkv=a["qkv"][:, None]),
+        dict(k_cache=a["k_cache"].double()), dict(v_cache=a["v_cache"][:-1]), dict(k_cache=a["k_cache"].transpose(1, 2)),
+        dict(block_table=a["block_table"].long()), dict(block_table=a["block_table"][:1]), dict(block_table=a["block_table"].t()),
+        dict(ctx=a["ctx"].long()), dict(ctx=a["ctx"][:1]), dict(cu_nodes=a["cu_nodes"][:-1]), dict(cu_nodes=a["cu_nodes"].long()),
+        dict(parents=a["parents"][:-1]), dict(parents=a["parents"].long()), dict(out=torch.zeros(5, 4 * DIM, dtype=torch.float64)),
+        dict(out=torch.zeros(4, 4 * DIM)), dict(out=torch.zeros(5, 8 * DIM)[:, ::2]),
+    ]
+    for kw in bad:
+        with pytest.raises((TypeError, ValueError)):
+            emulated.tree_attn(**_change(a, **kw))
+
+
+def test_refusals_of_verification():
+    a = make_verify([3, 2], 10, drafted=True)
+    with pytest.raises(TypeError, match="CUDA"):
+        fused.verify_tree(**a)
+    with pytest.raises(TypeError):
+        fused._check_verify_tree(**_change(a, logits=a["logits"].float()), dtype=torch.bfloat16)
+    bad = [
+        dict(max_nodes=0), dict(max_nodes=65), dict(logits=a["logits"][0]), dict(logits=a["logits"][:, :0]), dict(logits=torch.zeros(5, 20)[:, ::2]),
+        dict(tokens=a["tokens"].int()), dict(tokens=a["tokens"][1:]), dict(parents=a["parents"].long()), dict(cu_nodes=a["cu_nodes"][1:]),
+        dict(temperature=a["temperature"].double()), dict(temperature=a["temperature"][:, None]), dict(u_accept=a["u_accept"][:4]),
+        dict(u_accept=a["u_accept"].double()), dict(u_sample=a["u_sample"][:1]), dict(draft_probs=a["draft_probs"].bfloat16()),
+        dict(draft_probs=a["draft_probs"][:, :9]), dict(draft_probs=a["draft_probs"].t().contiguous().t()),
+    ]
+    for kw in bad:
+        with pytest.raises((TypeError, ValueError)):
+            emulated.verify_tree(**_change(a, **kw))
+
+
+def test_refusals_of_commit():
+    a = _commit_inputs(2)
+    with pytest.raises(TypeError, match="CUDA"):
+        fused.kv_commit_(**a)
+    x = a["qkv_layers"]
+    bad = [
+        dict(qkv_layers=[]), dict(qkv_layers=x[:1]), dict(qkv_layers=[x[0], x[1][:-1]]), dict(qkv_layers=[x[0], x[1].contiguous()]),
+        dict(qkv_layers=[x[0], x[1].double()]), dict(head_dim=64), dict(n_kv=0), dict(n_q=5), dict(k_cache=a["k_cache"][:, :-1]),
+        dict(v_cache=a["v_cache"].double()), dict(path=a["path"].long()), dict(path=a["path"][:-1]), dict(path=a["path"][0]),
+        dict(ctx=a["ctx"].long()), dict(block_table=a["block_table"][:2]),
+    ]
+    for kw in bad:
+        with pytest.raises((TypeError, ValueError)):
+            emulated.kv_commit_(**_change(a, **kw))
