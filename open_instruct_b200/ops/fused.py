@@ -419,6 +419,8 @@ def _check_cache(k_cache, v_cache, block_table, ctx, n_kv: int, head_dim: int, d
             raise TypeError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
         if t.dim() != 4 + len(lead) or tuple(t.shape[:len(lead)]) != lead or tuple(t.shape[-3:]) != (n_kv, KV_PAGE, head_dim) or not t.is_contiguous() or t.data_ptr() % 16:
             raise ValueError(f"{name}: expected a contiguous [{''.join(f'{n}, ' for n in lead)}blocks, {n_kv}, {KV_PAGE}, {head_dim}] cache, got {tuple(t.shape)}")
+        if t.shape[len(lead)] < 1:
+            raise ValueError(f"{name}: a cache has one page at least")
     if k_cache.shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have the same shape")
     if ctx.dim() != 1:
@@ -494,6 +496,11 @@ def _need_cuda(t: torch.Tensor, name: str) -> None:
         raise TypeError(f"{name}: expected a CUDA tensor, got one on {t.device}")
 
 
+@functools.lru_cache(maxsize=None)
+def _tree_attn_scratch(max_nodes: int, n_q: int, n_kv: int) -> int:
+    return lib.load_ops().b200_tree_attn_scratch(max_nodes, n_q, n_kv)
+
+
 def tree_attn(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, ctx: torch.Tensor,
               cu_nodes: torch.Tensor, parents: torch.Tensor, n_q: int, n_kv: int, head_dim: int, scale: float, max_nodes: int,
               out: torch.Tensor | None = None) -> torch.Tensor:
@@ -512,9 +519,10 @@ def tree_attn(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     dev, N, B = qkv.device, qkv.shape[0], ctx.shape[0]
     if out is None:
         out = torch.empty(N, n_q * head_dim, dtype=torch.bfloat16, device=dev)
+    scratch = torch.empty(_tree_attn_scratch(max_nodes, n_q, n_kv), dtype=torch.uint8, device=dev)
     _call_on(dev, "b200_tree_attn", ptr(qkv), qkv.stride(0), ptr(k_cache), ptr(v_cache), k_cache.shape[0], ptr(block_table),
              block_table.stride(0), block_table.shape[1], ptr(ctx), ptr(cu_nodes), ptr(parents), B, N, max_nodes, n_q, n_kv, head_dim, scale,
-             ptr(out))
+             ptr(out), ptr(scratch), ptr(status_word(dev)))
     return out
 
 
