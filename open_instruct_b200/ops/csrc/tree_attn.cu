@@ -19,7 +19,7 @@
 // serves every step.
 //
 // One CTA: warp 0 streams pages with TMA through a ring of five 32 KB buffers, warp 1 issues S = Q K^T and O += P V, two groups
-// of four warps own the softmax (warps 4 to 7 and 8 to 11).  A unit of two row tiles gives each group one of them (the keys are loaded once for both); a
+// of four warps own the softmax (warps 4 to 7 and 8 to 11), warp 2 plans the segments ahead.  A unit of two row tiles gives each group one of them (the keys are loaded once for both); a
 // unit of one row tile gives the groups alternate key tiles, merged at the end, so that one group's exponentials always run
 // beside the other group's products.  P replaces S in tensor memory (bf16), O stays there for the whole unit and is rescaled
 // only when the row maximum has grown by more than 2^8.
@@ -30,30 +30,16 @@ namespace b200 {
 constexpr int TA_DH = 128;
 constexpr int TA_PAGE = 64;
 constexpr int TA_MAX_NODES = 64;
-constexpr int TA_THREADS = 384;          // four warps for TMA and products (two of them idle), two groups of four for the softmax
+constexpr int TA_THREADS = 384;          // four warps for TMA, products and planning (one idle), two groups of four for the softmax
 // Registers: 12 warps at launch have 168 a thread.  The softmax holds a row of 128 scores and spills at that; the first group
-// gives back what the other two take (72 + 2 * 216 = 3 * 168, checked against the launch).
-constexpr int TA_REGS = 168, TA_REGS_ISSUE = 72, TA_REGS_SOFTMAX = 216;
+// gives back what the other two take (56 + 2 * 224 = 3 * 168, checked against the launch).
+constexpr int TA_REGS = 168, TA_REGS_ISSUE = 56, TA_REGS_SOFTMAX = 224;
 static_assert(TA_REGS_ISSUE + 2 * TA_REGS_SOFTMAX <= 3 * TA_REGS, "the groups' shares exceed what the block is launched with");
 constexpr int TA_SUB = 128 * 64 * 2;     // bytes of one [128 x 64] swizzled sub-tile
 constexpr int TA_TILE = 2 * TA_SUB;      // a [128 keys or rows x 128] bf16 tile
 constexpr int TA_RING = 5;
 constexpr int TA_MIN_TILES = 2;          // key tiles a CTA takes at least: below that joining the parts costs more than it saves
 constexpr float TA_LOG2E = 1.4426950408889634f;
-
-// Ancestors (the node itself included) of the node at position t as a bit set; 0 for padding.  Parents come before their
-// children, anything else ends the walk, so it takes at most t steps whatever the table holds.
-__device__ __forceinline__ unsigned long long tree_ancestors(const int* __restrict__ parents, int t) {
-  int up = parents[t];
-  if (up < -1) return 0ull;
-  unsigned long long seen = 1ull << t;
-  while (up >= 0 && up < t) {
-    t = up;
-    seen |= 1ull << t;
-    up = parents[t];
-  }
-  return seen;
-}
 
 struct TreeArgs {
   const int* table;
@@ -73,44 +59,28 @@ struct TreeArgs {
   int* status;
 };
 
-// The CTA's share of the key tiles, unit by unit.  Every role of the CTA walks the same sequence on its own.
-struct TreeWalk {
-  int b, n0, T, C, nt, nru, unit, t0, t1;
-  long long left;
-
-  __device__ __forceinline__ void load(const TreeArgs& a) {
+// A sequence as the kernel sees it.  Tiles of 128 cached keys, then one tile with the tree's own keys; an odd last page shares
+// that tile with the tree (page in rows 0 .. 63, tree in rows 64 .. 127; without such a page the tree is in rows 0 .. 63).
+struct TreeSeq {
+  int n0, T, C, nt, nru;
+  __device__ __forceinline__ void load(const TreeArgs& a, int b) {
     n0 = min(max(a.cu[b], 0), a.N);
     T = min(min(max(a.cu[b + 1] - n0, 0), a.max_nodes), a.N - n0);
     C = min(max(a.ctx[b], 0), a.max_blocks * TA_PAGE);
-    nt = (C + 127) / 128 + 1;
+    nt = (C + TA_PAGE - 1) / TA_PAGE / 2 + 1;
     nru = (T + 2 * a.npt - 1) / (2 * a.npt);
   }
   __device__ __forceinline__ long long tiles(const TreeArgs& a) const { return static_cast<long long>(a.Hkv) * nru * nt; }
-  __device__ __forceinline__ void begin(const TreeArgs& a, int seq, long long offset, long long count) {
-    b = seq;
-    left = count;
-    load(a);
-    unit = static_cast<int>(offset / nt);
-    t0 = static_cast<int>(offset % nt);
-    t1 = static_cast<int>(min(static_cast<long long>(nt), t0 + left));
-  }
-  __device__ __forceinline__ bool more() const { return left > 0; }
-  __device__ __forceinline__ void next(const TreeArgs& a) {
-    left -= t1 - t0;
-    t0 = 0;
-    if (left <= 0) return;
-    if (++unit == a.Hkv * nru) {
-      unit = 0;
-      do {
-        ++b;
-        load(a);
-      } while (T == 0);
-    }
-    t1 = static_cast<int>(min(static_cast<long long>(nt), left));
-  }
-  __device__ __forceinline__ int kvh() const { return unit / nru; }
-  __device__ __forceinline__ int first_node(const TreeArgs& a) const { return unit % nru * 2 * a.npt; }
-  __device__ __forceinline__ int row_tiles(const TreeArgs& a) const { return T - first_node(a) > a.npt ? 2 : 1; }
+};
+
+// The part of one unit that a CTA works on, as the planning warp hands it to the others.
+struct TreeSegment {
+  int n0, T, C, nt;      // first row of the sequence in the batch, its nodes, its cached keys, tiles of the unit
+  int t0, t1;            // tiles of this segment (none: the CTA is done)
+  int kvh, first, nrt;   // KV head, first node of the unit, row tiles
+  int y0, y1;            // cache rows of the first tile's pages (-1: none)
+  int b;
+  unsigned long long sees[TA_MAX_NODES];
 };
 
 // Order of a segment's loads in the ring: K0 K1 V0 K2 V1 ... V(n-1), the order in which they are used.
@@ -120,14 +90,16 @@ __device__ __forceinline__ int ring_v(int i, int n) { return i == n - 1 ? 2 * n 
 struct TreeSmem {
   uint8_t q[2][TA_TILE];
   uint8_t ring[TA_RING][TA_TILE];
-  float2 ml[2][128];
-  uint64_t q_full[2], q_empty[2], r_full[TA_RING], r_empty[TA_RING], s_full[2], p_full[2], o_full[2], ml_full[2], epi_done;
+  float2 ml[128];        // (maximum, sum) of the group that does not write a one-row-tile unit's result
+  TreeSegment seg[2];
+  uint64_t q_full[2], q_empty[2], r_full[TA_RING], r_empty[TA_RING], s_full[2], p_full[2], o_full[2], o_free[2], seg_full[2], seg_empty[2], ml_full;
   long long scan[TA_THREADS / 32];
   long long at_off;
   int at_seq;
   uint32_t tmem_ptr;
   int abort_flag;
 };
+static_assert(sizeof(TreeSmem) <= 232448, "shared memory of a CTA");
 
 __device__ __forceinline__ uint64_t ta_desc_k(uint32_t tile, int k) { return umma_desc_sw128(tile + (k >> 2) * TA_SUB + (k & 3) * 32, 16, 1024); }
 __device__ __forceinline__ uint64_t ta_desc_mn(uint32_t tile, int k) { return umma_desc_sw128(tile + k * 2048, TA_SUB, 1024); }
@@ -142,6 +114,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// the low n bits, n in 0 .. 64
+__device__ __forceinline__ unsigned long long low_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
 __global__ void __launch_bounds__(TA_THREADS, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_node, const __grid_constant__ CUtensorMap tm_k,
@@ -150,6 +124,26 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   TreeSmem& sm = *reinterpret_cast<TreeSmem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &sm.abort_flag;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.q_full[i], 1);
+      mbar_init(&sm.q_empty[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i], 4);
+      mbar_init(&sm.o_full[i], 1);
+      mbar_init(&sm.o_free[i], 4);
+      mbar_init(&sm.seg_full[i], 1);
+      mbar_init(&sm.seg_empty[i], 10);  // the TMA and the product threads, eight softmax warps
+    }
+    for (int i = 0; i < TA_RING; ++i) {
+      mbar_init(&sm.r_full[i], 1);
+      mbar_init(&sm.r_empty[i], 1);
+    }
+    mbar_init(&sm.ml_full, 4);
+    sm.abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
   griddep_launch_dependents();
   griddep_wait();
 
@@ -174,9 +168,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   };
   auto tiles_of = [&](int b) {
     if (b >= a.B) return 0ll;
-    TreeWalk s;
-    s.b = b;
-    s.load(a);
+    TreeSeq s;
+    s.load(a, b);
     return s.tiles(a);
   };
   long long total = 0, chunk, mine = 0, incl = 0;
@@ -211,25 +204,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       base += chunk;
     }
   }
-
-  if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.q_full[i], 1);
-      mbar_init(&sm.q_empty[i], 1);
-      mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i], 4);
-      mbar_init(&sm.o_full[i], 1);
-      mbar_init(&sm.ml_full[i], 4);
-    }
-    for (int i = 0; i < TA_RING; ++i) {
-      mbar_init(&sm.r_full[i], 1);
-      mbar_init(&sm.r_empty[i], 1);
-    }
-    mbar_init(&sm.epi_done, 8);
-    sm.abort_flag = 0;
-    fence_barrier_init();
-    fence_proxy_async();
-  }
   if (warp == 1) {
     tmem_alloc(&sm.tmem_ptr, 512);
     tmem_relinquish();
@@ -237,225 +211,325 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sm.tmem_ptr;  // S (then P) of group w at column 128 w, O of group w at 256 + 128 w
-
-  TreeWalk w;
-  w.begin(a, sm.at_seq, sm.at_off, end - begin);
+  const uint32_t tmem = sm.tmem_ptr;  // S (then P) of group g at column 128 g, O of group g at 256 + 128 g
 
   if (warp < 4) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_REGS_ISSUE));
-   if (warp == 0) {
-    if (elect_one()) {
-      prefetch_tensormap(&tm_k);
-      prefetch_tensormap(&tm_v);
-      uint32_t rc = 0, qc = 0;  // loads issued into the ring, row tiles issued
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_REGS_ISSUE));
+    if (warp == 2) {
+      // ---- planning: the CTA's segments one or two ahead of the others, so that their loads wait for no index
+      TreeSeq q;
+      int b = sm.at_seq;
+      q.load(a, b);
+      long long left = end - begin;
+      int unit = static_cast<int>(sm.at_off / q.nt), t0 = static_cast<int>(sm.at_off % q.nt), have = -1;
+      unsigned long long s0 = 0, s1 = 0;  // what nodes `lane` and `lane + 32` see
       bool ok = true;
-      auto ring_slot = [&](uint32_t bytes) -> int {
-        const int s = rc % TA_RING;
-        if (!mbar_wait(&sm.r_empty[s], ((rc / TA_RING) & 1) ^ 1, abort_flag)) {
-          atomicCAS(a.status, 0, ST_TIMEOUT_EMPTY);
-          return -1;
-        }
-        mbar_expect_tx(&sm.r_full[s], bytes);
-        ++rc;
-        return s;
-      };
-      for (; w.more() && ok; w.next(a)) {
-        const int kvh = w.kvh(), first = w.first_node(a), nrt = w.row_tiles(a), nq = w.nt - 1;
-        for (int rt = 0; rt < nrt && ok; ++rt, ++qc) {
-          const int s = qc & 1;
-          if (!mbar_wait(&sm.q_empty[s], ((qc >> 1) & 1) ^ 1, abort_flag)) {
-            atomicCAS(a.status, 0, ST_TIMEOUT_EMPTY);
-            ok = false;
-            break;
+      for (uint32_t n = 0; ok; ++n) {
+        TreeSegment& g = sm.seg[n & 1];
+        if (n >= 2) ok = ta_warp_wait(&sm.seg_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        const int t1 = left > 0 ? static_cast<int>(min(static_cast<long long>(q.nt), t0 + left)) : t0;
+        if (left > 0) {
+          const int kvh = unit / q.nru, first = unit % q.nru * 2 * a.npt;
+          if (have != b) {
+            have = b;
+            int p0 = lane < q.T ? a.parents[q.n0 + lane] : -2, p1 = lane + 32 < q.T ? a.parents[q.n0 + lane + 32] : -2;
+            // Ancestors as bit sets.  Parents come before their children, anything else ends the walk: at most 64 steps.
+            s0 = p0 < -1 ? 0ull : 1ull << lane;
+            s1 = p1 < -1 ? 0ull : 1ull << (lane + 32);
+            int u0 = p0 < lane ? p0 : -1, u1 = p1 < lane + 32 ? p1 : -1;
+            while (__any_sync(0xffffffffu, u0 >= 0 || u1 >= 0)) {
+              const int a0 = __shfl_sync(0xffffffffu, p0, u0 & 31), a1 = __shfl_sync(0xffffffffu, p0, u1 & 31),
+                        c1 = __shfl_sync(0xffffffffu, p1, u1 & 31);
+              if (u0 >= 0) {
+                s0 |= 1ull << u0;
+                u0 = a0 < u0 ? a0 : -1;
+              }
+              if (u1 >= 0) {
+                s1 |= 1ull << u1;
+                const int up = u1 < 32 ? a1 : c1;
+                u1 = up < u1 ? up : -1;
+              }
+            }
           }
-          mbar_expect_tx(&sm.q_full[s], a.G * a.npt * 256);
-          tma_load_3d(sm.q[s], &tm_q, &sm.q_full[s], 0, kvh * a.G, w.n0 + first + rt * a.npt);
-          tma_load_3d(sm.q[s] + TA_SUB, &tm_q, &sm.q_full[s], 64, kvh * a.G, w.n0 + first + rt * a.npt);
-        }
-        const int* row = a.table + w.b * a.table_ld;
-        int yk0 = 0, yk1 = 0, yv0 = 0, yv1 = 0;  // page rows of the tile whose K / V is next
-        auto pages = [&](int t, int& y0, int& y1) {
-          y0 = y1 = -1;
-          if (t < nq) {
-            auto at = [&](int p) {
-              const int blk = row[p];
-              return (min(static_cast<unsigned>(blk), static_cast<unsigned>(a.num_blocks)) * a.Hkv + kvh) * TA_PAGE;  // outside: past the end, reads as zeros
-            };
-            y0 = at(2 * t);
-            if ((2 * t + 1) * TA_PAGE < w.C) y1 = at(2 * t + 1);
+          g.sees[lane] = s0;
+          g.sees[lane + 32] = s1;
+          if (lane < 2) {
+            const int p = 2 * t0 + lane;
+            int y = -1;
+            if (p * TA_PAGE < q.C)
+              y = (min(static_cast<unsigned>(a.table[b * a.table_ld + p]), static_cast<unsigned>(a.num_blocks)) * a.Hkv + kvh) * TA_PAGE;
+            (lane ? g.y1 : g.y0) = y;
           }
+          if (lane == 0) {
+            g.n0 = q.n0;
+            g.T = q.T;
+            g.C = q.C;
+            g.nt = q.nt;
+            g.kvh = kvh;
+            g.first = first;
+            g.nrt = q.T - first > a.npt ? 2 : 1;
+            g.b = b;
+            if (left <= t1 - t0) {  // the CTA's last: a unit that begins here and goes on elsewhere is joined from its parts
+              int4 join = make_int4(0, 0, 0, 0);
+              if (t0 == 0 && t1 < q.nt) {
+                const long long last = end - t1 + q.nt - 1;  // the unit's last tile in the order of all tiles
+                int c = static_cast<int>(last * ctas / total);
+                while (total * (c + 1) / ctas <= last) ++c;
+                while (total * c / ctas > last) --c;
+                join = make_int4(c - cta + 1, q.n0 + first, min(2 * a.npt, q.T - first), kvh);
+              }
+              a.joins[cta] = join;
+            }
+          }
+        }
+        if (lane == 0) {
+          g.t0 = t0;
+          g.t1 = t1;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.seg_full[n & 1]);
+        if (t1 == t0) break;
+        left -= t1 - t0;
+        t0 = 0;
+        if (left > 0 && ++unit == a.Hkv * q.nru) {
+          unit = 0;
+          do q.load(a, ++b);
+          while (q.T == 0);
+        }
+      }
+      if (!ok && lane == 0) atomicCAS(a.status, 0, ST_TIMEOUT_EMPTY);
+    } else if (warp == 0) {
+      if (elect_one()) {
+        prefetch_tensormap(&tm_k);
+        prefetch_tensormap(&tm_v);
+        uint32_t rc = 0, qc = 0;  // loads issued into the ring, row tiles issued
+        bool ok = true;
+        auto ring_slot = [&](uint32_t bytes) -> int {
+          const int s = rc % TA_RING;
+          if (!mbar_wait(&sm.r_empty[s], ((rc / TA_RING) & 1) ^ 1, abort_flag)) return -1;
+          mbar_expect_tx(&sm.r_full[s], bytes);
+          ++rc;
+          return s;
         };
-        auto load_tile = [&](const CUtensorMap* cache, int head, int t, int y0, int y1) -> bool {
-          const bool tree = t == nq;
-          const int s = ring_slot(tree || y1 < 0 ? TA_TILE / 2 : TA_TILE);
-          if (s < 0) return false;
-          uint8_t* dst = sm.ring[s];
-          if (tree) {
-            tma_load_3d(dst, &tm_node, &sm.r_full[s], 0, head, w.n0);
-            tma_load_3d(dst + TA_SUB, &tm_node, &sm.r_full[s], 64, head, w.n0);
+        for (uint32_t n = 0; ok; ++n) {
+          const TreeSegment& g = sm.seg[n & 1];
+          ok = mbar_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
+          if (!ok || g.t0 == g.t1) break;
+          const int t0 = g.t0, t1 = g.t1, tree = g.nt - 1, kvh = g.kvh, nrt = g.nrt, C = g.C, n0 = g.n0;
+          int yk0 = g.y0, yk1 = g.y1;  // page rows of the next tile of K
+          const int q0 = n0 + g.first;
+          const int* row = a.table + g.b * a.table_ld;
+          mbar_arrive(&sm.seg_empty[n & 1]);
+          for (int rt = 0; rt < nrt && ok; ++rt, ++qc) {
+            const int s = qc & 1;
+            ok = mbar_wait(&sm.q_empty[s], ((qc >> 1) & 1) ^ 1, abort_flag);
+            if (!ok) break;
+            mbar_expect_tx(&sm.q_full[s], a.G * a.npt * 256);
+            tma_load_3d(sm.q[s], &tm_q, &sm.q_full[s], 0, kvh * a.G, q0 + rt * a.npt);
+            tma_load_3d(sm.q[s] + TA_SUB, &tm_q, &sm.q_full[s], 64, kvh * a.G, q0 + rt * a.npt);
+          }
+          auto page = [&](int p) {  // a page outside the cache: rows past its end, which read as zeros
+            if (p * TA_PAGE >= C) return -1;
+            return static_cast<int>((min(static_cast<unsigned>(row[p]), static_cast<unsigned>(a.num_blocks)) * a.Hkv + kvh) * TA_PAGE);
+          };
+          auto load_tile = [&](const CUtensorMap* cache, int head, int t, int y0, int y1) -> bool {
+            const int s = ring_slot((t == tree && y0 < 0) || (t != tree && y1 < 0) ? TA_TILE / 2 : TA_TILE);
+            if (s < 0) return false;
+            uint8_t* dst = sm.ring[s];
+            if (y0 >= 0) {
+              tma_load_2d(dst, cache, &sm.r_full[s], 0, y0);
+              tma_load_2d(dst + TA_SUB, cache, &sm.r_full[s], 64, y0);
+            }
+            uint8_t* second = y0 >= 0 ? dst + TA_SUB / 2 : dst;
+            if (t == tree) {
+              tma_load_3d(second, &tm_node, &sm.r_full[s], 0, head, n0);
+              tma_load_3d(second + TA_SUB, &tm_node, &sm.r_full[s], 64, head, n0);
+            } else if (y1 >= 0) {
+              tma_load_2d(second, cache, &sm.r_full[s], 0, y1);
+              tma_load_2d(second + TA_SUB, cache, &sm.r_full[s], 64, y1);
+            }
             return true;
+          };
+          int yn0 = -1, yn1 = -1;      // of the tile after that
+          if (t0 + 1 < t1) yn0 = page(2 * t0 + 2), yn1 = page(2 * t0 + 3);
+          if (ok) ok = load_tile(&tm_k, a.Hq + kvh, t0, yk0, yk1);
+          for (int t = t0; t < t1 && ok; ++t) {
+            const int yv0 = yk0, yv1 = yk1;
+            yk0 = yn0;
+            yk1 = yn1;
+            if (t + 1 < t1) {
+              if (t + 2 < t1) yn0 = page(2 * t + 4), yn1 = page(2 * t + 5);
+              ok = load_tile(&tm_k, a.Hq + kvh, t + 1, yk0, yk1);
+            }
+            if (ok) ok = load_tile(&tm_v, a.Hq + a.Hkv + kvh, t, yv0, yv1);
           }
-          tma_load_2d(dst, cache, &sm.r_full[s], 0, y0);
-          tma_load_2d(dst + TA_SUB, cache, &sm.r_full[s], 64, y0);
-          if (y1 >= 0) {
-            tma_load_2d(dst + TA_SUB / 2, cache, &sm.r_full[s], 0, y1);
-            tma_load_2d(dst + TA_SUB + TA_SUB / 2, cache, &sm.r_full[s], 64, y1);
-          }
+        }
+        if (!ok) atomicCAS(a.status, 0, ST_TIMEOUT_EMPTY);
+      }
+    } else if (warp == 1) {
+      if (elect_one()) {
+        constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, false, false), idesc_s64 = umma_idesc_bf16(128, 64, false, false);
+        constexpr uint32_t idesc_o = umma_idesc_bf16(128, 128, false, true);
+        struct Job {
+          int grp, vslot;
+          uint32_t vpar;
+          bool half, wait_v, free_v, first, last;
+        };
+        uint32_t jc = 0, rbase = 0, qc = 0, pc = 0;  // pc: bit g is the parity of group g's next P
+        bool ok = true;
+        auto give_up = [&](int code) {
+          atomicCAS(a.status, 0, code);
+          return false;
+        };
+        auto issue_pv = [&](const Job& j, uint32_t seg) -> bool {
+          if (!mbar_wait(&sm.p_full[j.grp], (pc >> j.grp) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
+          pc ^= 1u << j.grp;
+          if (j.wait_v && !mbar_wait(&sm.r_full[j.vslot], j.vpar, abort_flag)) return give_up(ST_TIMEOUT_FULL);
+          // a group's first product of a unit overwrites its O: the last unit's must have been read
+          if (j.first && seg > 0 && !mbar_wait(&sm.o_free[j.grp], (seg - 1) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
+          tc_fence_after();
+          const uint32_t v = smem_u32(sm.ring[j.vslot]), p = tmem + j.grp * 128, o = tmem + 256 + j.grp * 128;
+          const int steps = j.half ? 4 : 8;
+          for (int k = 0; k < steps; ++k) umma_ts(o, p + k * 8, ta_desc_mn(v, k), idesc_o, !(j.first && k == 0));
+          if (j.free_v) umma_commit(&sm.r_empty[j.vslot]);
+          if (j.last) umma_commit(&sm.o_full[j.grp]);
           return true;
         };
-        if (ok) {
-          pages(w.t0, yk0, yk1);
-          ok = load_tile(&tm_k, a.Hq + kvh, w.t0, yk0, yk1);
-        }
-        for (int t = w.t0; t < w.t1 && ok; ++t) {
-          yv0 = yk0;
-          yv1 = yk1;
-          if (t + 1 < w.t1) {
-            pages(t + 1, yk0, yk1);
-            ok = load_tile(&tm_k, a.Hq + kvh, t + 1, yk0, yk1);
-          }
-          if (ok) ok = load_tile(&tm_v, a.Hq + a.Hkv + kvh, t, yv0, yv1);
-        }
-      }
-    }
-  } else if (warp == 1) {
-    if (elect_one()) {
-      constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, false, false), idesc_s64 = umma_idesc_bf16(128, 64, false, false);
-      constexpr uint32_t idesc_o = umma_idesc_bf16(128, 128, false, true);
-      struct Job {
-        int grp, vslot;
-        uint32_t vpar;
-        bool tree, wait_v, free_v, first, last, new_seg;
-      };
-      uint32_t jc = 0, rbase = 0, qc = 0, pc = 0, seg = 0;  // pc: bit g is the parity of group g's next P
-      bool ok = true;
-      auto give_up = [&](int code) {
-        atomicCAS(a.status, 0, code);
-        return false;
-      };
-      auto issue_pv = [&](const Job& j, uint32_t seg_of) -> bool {
-        if (!mbar_wait(&sm.p_full[j.grp], (pc >> j.grp) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
-        pc ^= 1u << j.grp;
-        if (j.wait_v && !mbar_wait(&sm.r_full[j.vslot], j.vpar, abort_flag)) return give_up(ST_TIMEOUT_FULL);
-        // the first product of a unit overwrites O: both groups must have read the last unit's
-        if (j.new_seg && seg_of > 0 && !mbar_wait(&sm.epi_done, (seg_of - 1) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
-        tc_fence_after();
-        const uint32_t v = smem_u32(sm.ring[j.vslot]), p = tmem + j.grp * 128, o = tmem + 256 + j.grp * 128;
-        const int steps = j.tree ? 4 : 8;
-        for (int k = 0; k < steps; ++k) umma_ts(o, p + k * 8, ta_desc_mn(v, k), idesc_o, !(j.first && k == 0));
-        if (j.free_v) umma_commit(&sm.r_empty[j.vslot]);
-        if (j.last) umma_commit(&sm.o_full[j.grp]);
-        return true;
-      };
-      Job prev;
-      bool have = false;
-      uint32_t prev_seg = 0;
-      for (; w.more() && ok; w.next(a), ++seg) {
-        const int n = w.t1 - w.t0, nrt = w.row_tiles(a), jobs = n * nrt;
-        for (int x = 0; x < jobs && ok; ++x, ++jc) {
-          const int i = nrt == 2 ? x >> 1 : x, rt = nrt == 2 ? x & 1 : 0;
-          const bool tree = w.t0 + i == w.nt - 1;
-          Job j;
-          j.grp = jc & 1;
-          const uint32_t kn = rbase + ring_k(i), vn = rbase + ring_v(i, n);
-          const int ks = kn % TA_RING, qs = (qc + rt) & 1;
-          j.vslot = vn % TA_RING;
-          j.vpar = (vn / TA_RING) & 1;
-          j.tree = tree;
-          j.wait_v = rt == 0;
-          j.free_v = rt == nrt - 1;
-          j.first = x < 2;
-          j.last = x >= jobs - 2;
-          j.new_seg = x == 0;
-          if (i == 0 && !mbar_wait(&sm.q_full[qs], ((qc + rt) >> 1) & 1, abort_flag)) {
+        Job prev;
+        bool have = false;
+        uint32_t prev_seg = 0;
+        for (uint32_t n = 0; ok; ++n) {
+          const TreeSegment& g = sm.seg[n & 1];
+          if (!mbar_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag)) {
             ok = give_up(ST_TIMEOUT_FULL);
             break;
           }
-          if (rt == 0 && !mbar_wait(&sm.r_full[ks], (kn / TA_RING) & 1, abort_flag)) {
-            ok = give_up(ST_TIMEOUT_FULL);
-            break;
-          }
-          tc_fence_after();
-          const uint32_t q = smem_u32(sm.q[qs]), kt = smem_u32(sm.ring[ks]);
+          if (g.t0 == g.t1) break;
+          const int count = g.t1 - g.t0, nrt = g.nrt, jobs = count * nrt;
+          const int half_at = g.C <= (g.nt - 1) * 128 ? g.nt - 1 - g.t0 : -1;  // the tree's tile without a page: 64 keys
+          mbar_arrive(&sm.seg_empty[n & 1]);
+          for (int x = 0; x < jobs && ok; ++x, ++jc) {
+            const int i = nrt == 2 ? x >> 1 : x, rt = nrt == 2 ? x & 1 : 0;
+            Job j;
+            j.grp = jc & 1;
+            const uint32_t kn = rbase + ring_k(i), vn = rbase + ring_v(i, count);
+            const int ks = kn % TA_RING, qs = (qc + rt) & 1;
+            j.vslot = vn % TA_RING;
+            j.vpar = (vn / TA_RING) & 1;
+            j.half = i == half_at;
+            j.wait_v = rt == 0;
+            j.free_v = rt == nrt - 1;
+            j.first = x < 2;
+            j.last = x >= jobs - 2;
+            if ((i == 0 && !mbar_wait(&sm.q_full[qs], ((qc + rt) >> 1) & 1, abort_flag)) ||
+                (rt == 0 && !mbar_wait(&sm.r_full[ks], (kn / TA_RING) & 1, abort_flag))) {
+              ok = give_up(ST_TIMEOUT_FULL);
+              break;
+            }
+            tc_fence_after();
+            const uint32_t q = smem_u32(sm.q[qs]), kt = smem_u32(sm.ring[ks]);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) umma_ss(tmem + j.grp * 128, ta_desc_k(q, k), ta_desc_k(kt, k), tree ? idesc_s64 : idesc_s, k != 0);
-          if (rt == nrt - 1) umma_commit(&sm.r_empty[ks]);
-          if (i == n - 1) umma_commit(&sm.q_empty[qs]);
-          umma_commit(&sm.s_full[j.grp]);
-          if (have) ok = issue_pv(prev, prev_seg);
-          prev = j;
-          prev_seg = seg;
-          have = true;
+            for (int k = 0; k < 8; ++k) umma_ss(tmem + j.grp * 128, ta_desc_k(q, k), ta_desc_k(kt, k), j.half ? idesc_s64 : idesc_s, k != 0);
+            if (rt == nrt - 1) umma_commit(&sm.r_empty[ks]);
+            if (i == count - 1) umma_commit(&sm.q_empty[qs]);
+            umma_commit(&sm.s_full[j.grp]);
+            if (have) ok = issue_pv(prev, prev_seg);
+            prev = j;
+            prev_seg = n;
+            have = true;
+          }
+          rbase += 2 * count;
+          qc += nrt;
         }
-        rbase += 2 * n;
-        qc += nrt;
+        if (ok && have) issue_pv(prev, prev_seg);
       }
-      if (ok && have) issue_pv(prev, prev_seg);
     }
-   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TA_REGS_SOFTMAX));
     const int grp = (warp - 4) >> 2, lg = warp & 3, r = lg * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(lg * 32) << 16;
     const uint32_t t_s = tmem + grp * 128 + lane_off, t_o = tmem + 256 + lane_off;
     const float c = a.scale * TA_LOG2E;
-    uint32_t jc = 0, rbase = 0, sc = 0, oc0 = 0, oc1 = 0, mc_seg = 0, seg = 0;
+    uint32_t jc = 0, rbase = 0;
+    uint32_t par_s = 0, par_o = 0, par_ml = 0;  // parities of the next S, of the next O of either group (bits 0 and 1), of the next exchange
+    bool late = false;                            // this group's last O was somebody else's to wait for
     const int rn = r / a.G, rg = r - rn * a.G;  // node of the row tile and head of the group
     bool ok = true;
-    for (; w.more() && ok; w.next(a), ++seg) {
-      const int n = w.t1 - w.t0, nrt = w.row_tiles(a), kvh = w.kvh(), first = w.first_node(a), jobs = n * nrt;
+    for (uint32_t n = 0; ok; ++n) {
+      const TreeSegment& g = sm.seg[n & 1];
+      ok = ta_warp_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
+      if (!ok || g.t0 == g.t1) break;
+      const int t0 = g.t0, count = g.t1 - t0, nt = g.nt, nrt = g.nrt, T = g.T, C = g.C, jobs = count * nrt;
       const int x0 = (grp ^ jc) & 1;           // my first job of this segment; then every second one
-      const int rt = nrt == 2 ? x0 : 0;
-      const int node = first + rt * a.npt + rn;
-      const bool valid = rn < a.npt && node < w.T;
+      const int rt = nrt == 2 ? x0 : 0, node = g.first + rt * a.npt + rn;
+      const bool valid = rn < a.npt && node < T;
+      const unsigned long long sees = valid ? g.sees[node] : 0ull;
+      const long long out_at = ((static_cast<long long>(g.n0) + node) * a.Hq + g.kvh * a.G + rg) * TA_DH;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.seg_empty[n & 1]);
       const bool busy = __any_sync(0xffffffffu, valid);
-      unsigned long long sees = 0;
-      if (valid) sees = tree_ancestors(a.parents + w.n0, node);
       float m = -INFINITY, l = 0.f;
-      for (int x = x0; x < jobs && ok; x += 2) {
-        const int i = nrt == 2 ? x >> 1 : x, t = w.t0 + i;
-        const bool tree = t == w.nt - 1;
-        const int nkeys = tree ? w.T : min(128, w.C - t * 128);
-        ok = ta_warp_wait(&sm.s_full[grp], sc & 1, abort_flag);
-        ++sc;
+      for (int x = x0; x < jobs; x += 2) {
+        const int i = nrt == 2 ? x >> 1 : x, t = t0 + i;
+        ok = ta_warp_wait(&sm.s_full[grp], par_s, abort_flag);
+        par_s ^= 1;
+        if (ok && late) {  // complete since this S was issued behind it: keeps the parity in step
+          ok = ta_warp_wait(&sm.o_full[grp], (par_o >> grp & 1) ^ 1, abort_flag);
+          late = false;
+        }
         if (!ok) break;
         tc_fence_after();
-        if (nkeys < (tree ? 64 : 128) && (nrt == 1 || rt == 0)) {
-          // rows of V behind the last key hold whatever was there: 0 * NaN must not reach the output
-          const uint32_t vn = rbase + ring_v(i, n);
-          ok = ta_warp_wait(&sm.r_full[vn % TA_RING], (vn / TA_RING) & 1, abort_flag);
-          if (!ok) break;
-          if (r >= nkeys && r < (tree ? 64 : 128)) {
-            uint4* row = reinterpret_cast<uint4*>(sm.ring[vn % TA_RING] + r * 128);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) row[q] = row[q + TA_SUB / 16] = make_uint4(0u, 0u, 0u, 0u);
+        // keys of this tile as two words of columns, and the rows of V that hold none (0 * NaN must not reach the output)
+        const int keys = min(128, C - t * 128);
+        unsigned long long lo = ~0ull, hi = ~0ull;
+        bool half = false;
+        if (t == nt - 1 || keys < 128) {
+          int z0 = keys, z1 = 128, z2 = 128, z3 = 128;  // rows [z0, z1) and [z2, z3) of V are empty
+          if (t == nt - 1) {
+            half = keys <= 0;
+            lo = half ? sees : low_bits(keys);
+            hi = half ? 0ull : sees;
+            z0 = max(keys, 0);
+            z1 = half ? 0 : 64;
+            z2 = z1 + T;
+            z3 = z1 + 64;
+          } else {
+            lo = low_bits(keys);
+            hi = low_bits(max(keys - 64, 0));
           }
-          fence_proxy_async();
+          if (rt == 0 && (z0 < z1 || z2 < z3)) {
+            const uint32_t vn = rbase + ring_v(i, count);
+            ok = ta_warp_wait(&sm.r_full[vn % TA_RING], (vn / TA_RING) & 1, abort_flag);
+            if (!ok) break;
+            if ((r >= z0 && r < z1) || (r >= z2 && r < z3)) {
+              uint4* row = reinterpret_cast<uint4*>(sm.ring[vn % TA_RING] + r * 128);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const int at = (q + lane) & 7;  // neighbouring rows start in different banks
+                row[at] = row[at + TA_SUB / 16] = make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+            fence_proxy_async();
+          }
         }
         if (busy) {
-          const int cols = tree ? 2 : 4;
           uint32_t sv[4][32];
-#pragma unroll
-          for (int cc = 0; cc < 4; ++cc)
-            if (cc < cols) tmem_ld32(t_s + cc * 32, sv[cc]);
+          tmem_ld32(t_s, sv[0]);
+          tmem_ld32(t_s + 32, sv[1]);
+          if (!half) {
+            tmem_ld32(t_s + 64, sv[2]);
+            tmem_ld32(t_s + 96, sv[3]);
+          }
           tmem_ld_wait();
-          if (tree) {
-#pragma unroll
-            for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((sees >> (cc * 32 + e)) & 1ull)) sv[cc][e] = 0xff800000u;
-#pragma unroll
-            for (int cc = 2; cc < 4; ++cc)
-#pragma unroll
-              for (int e = 0; e < 32; ++e) sv[cc][e] = 0xff800000u;
-          } else if (nkeys < 128) {
+          if ((lo & hi) != ~0ull) {
+            const uint32_t words[4] = {static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
+                                       static_cast<uint32_t>(hi >> 32)};
 #pragma unroll
             for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (cc * 32 + e >= nkeys) sv[cc][e] = 0xff800000u;
+                if (!((words[cc] >> e) & 1u)) sv[cc][e] = 0xff800000u;
           }
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -474,7 +548,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           float rs4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int cc = 0; cc < 4; ++cc) {
-            if (cc < cols) {
+            if (cc < 2 || !half) {
               uint32_t pk[16];
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
@@ -507,112 +581,100 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       }
       if (!ok) break;
 
-      // ---- end of the segment: join the two groups (one row tile), write the result or a part of it
-      const bool whole = w.t0 == 0 && w.t1 == w.nt;
-      const long long part = (static_cast<long long>(cta) * 2 + (w.t0 == 0 ? 1 : 0)) * a.part_rows;
-      const long long token = w.n0 + node;
-      __nv_bfloat16* dst = a.out + (token * a.Hq + kvh * a.G + rg) * TA_DH;
+      // ---- end of the segment: the result or a part of it.  Two row tiles: each group writes its own.  One: the group of the last
+      // job joins both, the other hands over its maxima and sums and goes on with the next unit.
       if (!sees) {
         m = -INFINITY;
         l = 0.f;
       }
-      float a0 = 1.f, a1 = 0.f;
-      int c0 = 0, c1 = 4;  // my columns, in steps of 32
-      bool had0 = true, had1 = true;
+      m *= c;  // base-2 scale from here on
+      const int last = (jc + jobs - 1) & 1;
+      const bool both = nrt == 1 && jobs > 1;
+      jc += jobs;
+      rbase += 2 * count;
+      float a0 = 1.f, a1 = 0.f;  // weights of my own O and of the other group's
       if (nrt == 2) {
-        ok = ta_warp_wait(&sm.o_full[grp], (grp ? oc1 : oc0) & 1, abort_flag);
-        ++oc0;
-        ++oc1;
+        ok = ta_warp_wait(&sm.o_full[grp], par_o >> grp & 1, abort_flag);
+        par_o ^= 3;
         if (!ok) break;
+      } else if (grp != last) {
+        if (both) {
+          if (n > 0) ok = ta_warp_wait(&sm.o_free[0], (n - 1) & 1, abort_flag);  // the last pair has been read
+          if (!ok) break;
+          sm.ml[r] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.ml_full);
+          late = true;
+        }
+        par_o ^= both ? 3 : 1 << last;
+        par_ml ^= both;
+        continue;
       } else {
-        const int jobs0 = (jobs + 1 - (jc & 1)) / 2, jobs1 = jobs - jobs0;  // job 0 belongs to group jc & 1
-        had0 = jobs0 > 0;
-        had1 = jobs1 > 0;
-        if (seg > 0) ok = ta_warp_wait(&sm.epi_done, (seg - 1) & 1, abort_flag);  // the other group has read the last pair
-        if (!ok) break;
-        sm.ml[grp][r] = make_float2(m * c, l);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.ml_full[grp]);
-        ok = ta_warp_wait(&sm.ml_full[grp ^ 1], mc_seg & 1, abort_flag);
-        ++mc_seg;
-        if (!ok) break;
-        const float2 other = sm.ml[grp ^ 1][r];
-        const float2 m0 = grp == 0 ? make_float2(m * c, l) : other, m1 = grp == 0 ? other : make_float2(m * c, l);
-        const float top = fmaxf(m0.x, m1.x);
-        a0 = m0.y != 0.f ? ex2_approx(m0.x - top) : 0.f;
-        a1 = m1.y != 0.f ? ex2_approx(m1.x - top) : 0.f;
-        l = a0 * m0.y + a1 * m1.y;
-        m = top;  // from here on in the base-2 scale
-        c0 = grp * 2;
-        c1 = c0 + 2;
-        if (had0) {
-          ok = ta_warp_wait(&sm.o_full[0], oc0 & 1, abort_flag);
-          ++oc0;
+        if (both) {
+          ok = ta_warp_wait(&sm.ml_full, par_ml, abort_flag);
+          if (ok) ok = ta_warp_wait(&sm.o_full[grp ^ 1], par_o >> (grp ^ 1) & 1, abort_flag);
+          if (!ok) break;
+          const float2 other = sm.ml[r];
+          const float top = fmaxf(m, other.x);
+          a0 = l != 0.f ? ex2_approx(m - top) : 0.f;
+          a1 = other.y != 0.f ? ex2_approx(other.x - top) : 0.f;
+          l = a0 * l + a1 * other.y;
+          m = top;
         }
-        if (ok && had1) {
-          ok = ta_warp_wait(&sm.o_full[1], oc1 & 1, abort_flag);
-          ++oc1;
-        }
+        ok = ta_warp_wait(&sm.o_full[grp], par_o >> grp & 1, abort_flag);
+        par_o ^= both ? 3 : 1 << grp;
+        par_ml ^= both;
         if (!ok) break;
       }
       tc_fence_after();
+      const bool whole = t0 == 0 && count == nt;
+      const long long part = (static_cast<long long>(cta) * 2 + (t0 == 0 ? 1 : 0)) * a.part_rows + rt * 128 + r;
       const float inv = l != 0.f ? 1.f / l : 0.f;  // an empty row gives zeros, a NaN stays one
-      if (busy) {
-        for (int cc = c0; cc < c1; ++cc) {
-          uint32_t o[32], o1[32];
-          if (nrt == 2) {
-            tmem_ld32(t_o + grp * 128 + cc * 32, o);
-            tmem_ld_wait();
-          } else {
-            if (had0) tmem_ld32(t_o + cc * 32, o);
-            if (had1) tmem_ld32(t_o + 128 + cc * 32, o1);
-            tmem_ld_wait();
+      auto load_o = [&](int cc, float (&f)[32]) {
+        uint32_t v[32];
+        tmem_ld32(t_o + grp * 128 + cc * 32, v);
+        tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float x0v = a0 != 0.f ? a0 * __uint_as_float(o[e]) : 0.f, x1v = a1 != 0.f ? a1 * __uint_as_float(o1[e]) : 0.f;
-              o[e] = __float_as_uint(x0v + x1v);
-            }
-          }
-          if (!valid) continue;
+        for (int e = 0; e < 32; ++e) f[e] = a0 != 0.f ? a0 * __uint_as_float(v[e]) : 0.f;
+        if (both) {
+          tmem_ld32(t_o + (grp ^ 1) * 128 + cc * 32, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] += a1 != 0.f ? a1 * __uint_as_float(v[e]) : 0.f;
+        }
+      };
+      uint32_t pk[64];
+      if (busy) {
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          float f[32];
+          load_o(cc, f);
           if (whole) {
 #pragma unroll
-            for (int g8 = 0; g8 < 4; ++g8) {
-              uint4 v4;
-              uint32_t* p4 = &v4.x;
+            for (int e = 0; e < 16; ++e) pk[cc * 16 + e] = sees ? pack_bf16x2(f[2 * e] * inv, f[2 * e + 1] * inv) : 0u;
+          } else if (valid) {
+            float4* dst = reinterpret_cast<float4*>(a.part_o + part * TA_DH + cc * 32);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float lo = __uint_as_float(o[g8 * 8 + 2 * e]) * inv, hi = __uint_as_float(o[g8 * 8 + 2 * e + 1]) * inv;
-                p4[e] = sees ? pack_bf16x2(lo, hi) : 0u;
-              }
-              reinterpret_cast<uint4*>(dst + cc * 32)[g8] = v4;
-            }
-          } else {
-            float4* to = reinterpret_cast<float4*>(a.part_o + (part + rt * 128 + r) * TA_DH + cc * 32);
-#pragma unroll
-            for (int g4 = 0; g4 < 8; ++g4)
-              to[g4] = make_float4(__uint_as_float(o[4 * g4]), __uint_as_float(o[4 * g4 + 1]), __uint_as_float(o[4 * g4 + 2]),
-                                   __uint_as_float(o[4 * g4 + 3]));
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
           }
         }
-        if (!whole && valid && (nrt == 2 || grp == 0)) a.part_ml[part + rt * 128 + r] = make_float2(nrt == 2 ? m * c : m, l);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.epi_done);
-      jc += jobs;
-      rbase += 2 * n;
-      // a unit that begins here and goes on elsewhere: leave word for the kernel that joins the parts
-      if (warp == 4 && lane == 0 && w.left == w.t1 - w.t0) {
-        int4 join = make_int4(0, 0, 0, 0);
-        if (w.t0 == 0 && !whole) {
-          const long long last_tile = end - w.t1 + w.nt - 1;  // of the unit, in the order of all tiles
-          int lastc = static_cast<int>(last_tile * ctas / total);
-          while (total * (lastc + 1) / ctas <= last_tile) ++lastc;
-          while (total * lastc / ctas > last_tile) --lastc;
-          join = make_int4(lastc - cta + 1, w.n0 + first, min(2 * a.npt, w.T - first), kvh);
-        }
-        a.joins[cta] = join;
+      if (lane == 0) {  // O may be overwritten; the stores of a whole unit's result need not hold that up
+        mbar_arrive(&sm.o_free[grp]);
+        if (nrt == 1) mbar_arrive(&sm.o_free[grp ^ 1]);
       }
+      if (valid) {
+        if (whole) {
+          uint4* dst = reinterpret_cast<uint4*>(a.out + out_at);
+#pragma unroll
+          for (int q = 0; q < 16; ++q) dst[q] = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+        } else {
+          a.part_ml[part] = make_float2(m, l);
+        }
+      }
+      __syncwarp();
     }
     if (!ok && lane == 0) atomicCAS(a.status, 0, ST_TIMEOUT_TMEM_FULL);
   }
