@@ -70,7 +70,18 @@ struct TreeSeq {
     nt = (C + TA_PAGE - 1) / TA_PAGE / 2 + 1;
     nru = (T + 2 * a.npt - 1) / (2 * a.npt);
   }
-  __device__ __forceinline__ long long tiles(const TreeArgs& a) const { return static_cast<long long>(a.Hkv) * nru * nt; }
+  __device__ __forceinline__ int tiles(const TreeArgs& a) const { return a.Hkv * nru * nt; }
+};
+
+// Even shares of `total` tiles: the first `more` CTAs take one more than the others.
+struct TreeShares {
+  int each, more;
+  __device__ __forceinline__ TreeShares(int total, int ctas) : each(total / ctas), more(total % ctas) {}
+  __device__ __forceinline__ int begin(int cta) const { return each * cta + min(cta, more); }
+  __device__ __forceinline__ int owner(int tile) const {
+    const int low = more * (each + 1);
+    return tile < low ? tile / (each + 1) : more + (tile - low) / each;
+  }
 };
 
 // The part of one unit that a CTA works on, as the planning warp hands it to the others.
@@ -93,9 +104,9 @@ struct TreeSmem {
   float2 ml[128];        // (maximum, sum) of the group that does not write a one-row-tile unit's result
   TreeSegment seg[2];
   uint64_t q_full[2], q_empty[2], r_full[TA_RING], r_empty[TA_RING], s_full[2], p_full[2], o_full[2], o_free[2], seg_full[2], seg_empty[2], ml_full;
-  long long scan[TA_THREADS / 32];
-  long long at_off;
-  int at_seq;
+  int scan[TA_THREADS / 32];
+  TreeSeq at;            // the sequence in which the CTA's share begins
+  int at_seq, at_off;
   uint32_t tmem_ptr;
   int abort_flag;
 };
@@ -114,6 +125,33 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// ---- two fp32 values in a register pair: one instruction for both
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  return d;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
+  return d;
+}
 // the low n bits, n in 0 .. 64
 __device__ __forceinline__ unsigned long long low_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
@@ -124,6 +162,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   TreeSmem& sm = *reinterpret_cast<TreeSmem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &sm.abort_flag;
+  if (tid == 32) {
+    prefetch_tensormap(&tm_q);
+    prefetch_tensormap(&tm_node);
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+  }
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.q_full[i], 1);
@@ -148,16 +192,16 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   griddep_wait();
 
   // ---- this CTA's share: total number of key tiles, then the sequence in which the share begins
-  auto block_scan = [&](long long v, long long& total) {  // inclusive prefix over the block's threads
+  auto block_scan = [&](int v, int& total) {  // inclusive prefix over the block's threads
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, v, o);
+      const int up = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += up;
     }
     __syncthreads();
     if (lane == 31) sm.scan[warp] = v;
     __syncthreads();
-    long long before = 0;
+    int before = 0;
     total = 0;
 #pragma unroll
     for (int w = 0; w < TA_THREADS / 32; ++w) {
@@ -166,22 +210,21 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
     return v + before;
   };
+  TreeSeq seq;
   auto tiles_of = [&](int b) {
-    if (b >= a.B) return 0ll;
-    TreeSeq s;
-    s.load(a, b);
-    return s.tiles(a);
+    if (b >= a.B) return 0;
+    seq.load(a, b);
+    return seq.tiles(a);
   };
-  long long total = 0, chunk, mine = 0, incl = 0;
+  int total = 0, chunk, mine = 0, incl = 0;
   for (int b0 = 0; b0 < a.B; b0 += TA_THREADS) {
     mine = tiles_of(b0 + tid);
     incl = block_scan(mine, chunk);
     total += chunk;
   }
-  const long long want = total / TA_MIN_TILES;
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(want, 1ll)));
-  const int cta = blockIdx.x;
-  const long long begin = total * cta / ctas, end = total * (cta + 1) / ctas;
+  const int ctas = min(static_cast<int>(gridDim.x), max(total / TA_MIN_TILES, 1)), cta = blockIdx.x;
+  const TreeShares share(total, ctas);
+  const int begin = share.begin(cta), end = share.begin(cta + 1);
   if (cta >= ctas || begin >= end || (smem_u32(smem_raw) & 1023u)) {
     if (tid == 0) {
       a.joins[cta] = make_int4(0, 0, 0, 0);
@@ -189,19 +232,16 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
     return;
   }
-  {
-    long long base = 0;
-    for (int b0 = 0; b0 < a.B; b0 += TA_THREADS) {
-      if (a.B > TA_THREADS) {  // more than one chunk: the values of this one again
-        mine = tiles_of(b0 + tid);
-        incl = block_scan(mine, chunk);
-      }
-      const long long lo = base + incl - mine;
-      if (mine > 0 && begin >= lo && begin < lo + mine) {
-        sm.at_seq = b0 + tid;
-        sm.at_off = begin - lo;
-      }
-      base += chunk;
+  for (int b0 = 0, base = 0; b0 < a.B; b0 += TA_THREADS, base += chunk) {
+    if (a.B > TA_THREADS) {  // more than one chunk: the values of this one again
+      mine = tiles_of(b0 + tid);
+      incl = block_scan(mine, chunk);
+    }
+    const int lo = base + incl - mine;
+    if (begin >= lo && begin < lo + mine) {
+      sm.at = seq;
+      sm.at_seq = b0 + tid;
+      sm.at_off = begin - lo;
     }
   }
   if (warp == 1) {
@@ -217,50 +257,50 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_REGS_ISSUE));
     if (warp == 2) {
       // ---- planning: the CTA's segments one or two ahead of the others, so that their loads wait for no index
-      TreeSeq q;
-      int b = sm.at_seq;
-      q.load(a, b);
-      long long left = end - begin;
-      int unit = static_cast<int>(sm.at_off / q.nt), t0 = static_cast<int>(sm.at_off % q.nt), have = -1;
+      TreeSeq q = sm.at;
+      int b = sm.at_seq, left = end - begin, unit = sm.at_off / q.nt, t0 = sm.at_off % q.nt, have = -1;
       unsigned long long s0 = 0, s1 = 0;  // what nodes `lane` and `lane + 32` see
       bool ok = true;
       for (uint32_t n = 0; ok; ++n) {
         TreeSegment& g = sm.seg[n & 1];
         if (n >= 2) ok = ta_warp_wait(&sm.seg_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag);
         if (!ok) break;
-        const int t1 = left > 0 ? static_cast<int>(min(static_cast<long long>(q.nt), t0 + left)) : t0;
+        const int t1 = left > 0 ? min(q.nt, t0 + left) : t0;
         if (left > 0) {
           const int kvh = unit / q.nru, first = unit % q.nru * 2 * a.npt;
+          int blk = -1;
+          if (lane < 2 && (2 * t0 + lane) * TA_PAGE < q.C) blk = a.table[b * a.table_ld + 2 * t0 + lane];
           if (have != b) {
             have = b;
-            int p0 = lane < q.T ? a.parents[q.n0 + lane] : -2, p1 = lane + 32 < q.T ? a.parents[q.n0 + lane + 32] : -2;
-            // Ancestors as bit sets.  Parents come before their children, anything else ends the walk: at most 64 steps.
-            s0 = p0 < -1 ? 0ull : 1ull << lane;
-            s1 = p1 < -1 ? 0ull : 1ull << (lane + 32);
-            int u0 = p0 < lane ? p0 : -1, u1 = p1 < lane + 32 ? p1 : -1;
+            int u0 = lane < q.T ? a.parents[q.n0 + lane] : -2, u1 = lane + 32 < q.T ? a.parents[q.n0 + lane + 32] : -2;
+            // Ancestors as bit sets, the paths' lengths doubling in every round: what a node sees, and where that path goes on.
+            // Parents come before their children; anything else ends a path, so six rounds cover 64 nodes.
+            s0 = u0 < -1 ? 0ull : 1ull << lane;
+            s1 = u1 < -1 ? 0ull : 1ull << (lane + 32);
+            if (u0 >= lane) u0 = -1;
+            if (u1 >= lane + 32) u1 = -1;
             while (__any_sync(0xffffffffu, u0 >= 0 || u1 >= 0)) {
-              const int a0 = __shfl_sync(0xffffffffu, p0, u0 & 31), a1 = __shfl_sync(0xffffffffu, p0, u1 & 31),
-                        c1 = __shfl_sync(0xffffffffu, p1, u1 & 31);
+              // node u < 64 lives in lane u & 31, in its second word from 32 on; u0 is always in the first
+              const unsigned long long f0 = __shfl_sync(0xffffffffu, s0, u0 & 31), f1 = __shfl_sync(0xffffffffu, s0, u1 & 31),
+                                       g1 = __shfl_sync(0xffffffffu, s1, u1 & 31);
+              const int v0 = __shfl_sync(0xffffffffu, u0, u0 & 31), v1 = __shfl_sync(0xffffffffu, u0, u1 & 31),
+                        w1 = __shfl_sync(0xffffffffu, u1, u1 & 31);
               if (u0 >= 0) {
-                s0 |= 1ull << u0;
-                u0 = a0 < u0 ? a0 : -1;
+                s0 |= f0;
+                u0 = v0;
               }
               if (u1 >= 0) {
-                s1 |= 1ull << u1;
-                const int up = u1 < 32 ? a1 : c1;
-                u1 = up < u1 ? up : -1;
+                s1 |= u1 < 32 ? f1 : g1;
+                u1 = u1 < 32 ? v1 : w1;
               }
             }
           }
           g.sees[lane] = s0;
           g.sees[lane + 32] = s1;
-          if (lane < 2) {
-            const int p = 2 * t0 + lane;
-            int y = -1;
-            if (p * TA_PAGE < q.C)
-              y = (min(static_cast<unsigned>(a.table[b * a.table_ld + p]), static_cast<unsigned>(a.num_blocks)) * a.Hkv + kvh) * TA_PAGE;
-            (lane ? g.y1 : g.y0) = y;
-          }
+          if (lane < 2)
+            (lane ? g.y1 : g.y0) = (2 * t0 + lane) * TA_PAGE < q.C
+                                       ? static_cast<int>((min(static_cast<unsigned>(blk), static_cast<unsigned>(a.num_blocks)) * a.Hkv + kvh) * TA_PAGE)
+                                       : -1;
           if (lane == 0) {
             g.n0 = q.n0;
             g.T = q.T;
@@ -273,10 +313,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             if (left <= t1 - t0) {  // the CTA's last: a unit that begins here and goes on elsewhere is joined from its parts
               int4 join = make_int4(0, 0, 0, 0);
               if (t0 == 0 && t1 < q.nt) {
-                const long long last = end - t1 + q.nt - 1;  // the unit's last tile in the order of all tiles
-                int c = static_cast<int>(last * ctas / total);
-                while (total * (c + 1) / ctas <= last) ++c;
-                while (total * c / ctas > last) --c;
+                const int c = share.owner(end - t1 + q.nt - 1);  // who has the unit's last tile
                 join = make_int4(c - cta + 1, q.n0 + first, min(2 * a.npt, q.T - first), kvh);
               }
               a.joins[cta] = join;
@@ -301,8 +338,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       if (!ok && lane == 0) atomicCAS(a.status, 0, ST_TIMEOUT_EMPTY);
     } else if (warp == 0) {
       if (elect_one()) {
-        prefetch_tensormap(&tm_k);
-        prefetch_tensormap(&tm_v);
         uint32_t rc = 0, qc = 0;  // loads issued into the ring, row tiles issued
         bool ok = true;
         auto ring_slot = [&](uint32_t bytes) -> int {
@@ -522,21 +557,27 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             tmem_ld32(t_s + 96, sv[3]);
           }
           tmem_ld_wait();
-          if ((lo & hi) != ~0ull) {
+          const bool masked = (lo & hi) != ~0ull;
+          if (masked) {
             const uint32_t words[4] = {static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
                                        static_cast<uint32_t>(hi >> 32)};
 #pragma unroll
             for (int cc = 0; cc < 4; ++cc)
+              if (cc < 2 || !half) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((words[cc] >> e) & 1u)) sv[cc][e] = 0xff800000u;
+                for (int e = 0; e < 32; ++e)
+                  if (!((words[cc] >> e) & 1u)) sv[cc][e] = 0xff800000u;
+              }
           }
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int cc = 0; cc < 4; ++cc)
+            if (cc < 2 || !half) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(sv[cc][e]));
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+              for (int e = 0; e < 32; e += 2)
+                mx4[e / 2 & 3] = max3(mx4[e / 2 & 3], __uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1]));
+            }
+          const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
           float alpha = 1.f;
           const bool grow = (mx - m) * c > 8.f;
           if (grow) {
@@ -544,23 +585,30 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             m = mx;
             l *= alpha;
           }
-          const float mc = m * c;
-          float rs4[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t c2 = pair2(c, c), mc2 = pair2(-m * c, -m * c);
+          uint64_t sum[2] = {0ull, 0ull};  // two pairs of zeros
 #pragma unroll
           for (int cc = 0; cc < 4; ++cc) {
             if (cc < 2 || !half) {
               uint32_t pk[16];
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
-                const float p0 = ex2_approx(fmaf(__uint_as_float(sv[cc][e]), c, -mc));
-                const float p1 = ex2_approx(fmaf(__uint_as_float(sv[cc][e + 1]), c, -mc));
-                rs4[(e >> 1) & 3] += p0 + p1;
+                const uint64_t x = fma2(pair2(__uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1])), c2, mc2);
+                float p0, p1;
+                unpair2(x, p0, p1);
+                p0 = ex2_approx(p0);
+                p1 = ex2_approx(p1);
+                sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair2(p0, p1));
                 pk[e >> 1] = pack_bf16x2(p0, p1);
               }
               tmem_st16(t_s + cc * 16, pk);
             }
           }
-          l += (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
+          {
+            float s0, s1;
+            unpair2(add2(sum[0], sum[1]), s0, s1);
+            l += s0 + s1;
+          }
           // S of this job was issued after every earlier P V of this group, so O is at rest here
           if (x >= 2 && __any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -629,29 +677,35 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       tc_fence_after();
       const bool whole = t0 == 0 && count == nt;
       const long long part = (static_cast<long long>(cta) * 2 + (t0 == 0 ? 1 : 0)) * a.part_rows + rt * 128 + r;
-      const float inv = l != 0.f ? 1.f / l : 0.f;  // an empty row gives zeros, a NaN stays one
-      auto load_o = [&](int cc, float (&f)[32]) {
-        uint32_t v[32];
-        tmem_ld32(t_o + grp * 128 + cc * 32, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = a0 != 0.f ? a0 * __uint_as_float(v[e]) : 0.f;
-        if (both) {
-          tmem_ld32(t_o + (grp ^ 1) * 128 + cc * 32, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] += a1 != 0.f ? a1 * __uint_as_float(v[e]) : 0.f;
-        }
-      };
-      uint32_t pk[64];
+      if (whole) {  // a row that sees nothing gives zeros (below), a NaN stays one
+        a0 *= 1.f / l;
+        a1 *= 1.f / l;
+      }
+      const uint64_t w0 = pair2(a0, a0), w1 = pair2(a1, a1);
       if (busy) {
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
+          uint32_t v[32], u[32];
+          tmem_ld32(t_o + grp * 128 + cc * 32, v);
+          if (both) tmem_ld32(t_o + (grp ^ 1) * 128 + cc * 32, u);
+          tmem_ld_wait();
           float f[32];
-          load_o(cc, f);
-          if (whole) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) pk[cc * 16 + e] = sees ? pack_bf16x2(f[2 * e] * inv, f[2 * e + 1] * inv) : 0u;
+          for (int e = 0; e < 32; e += 2) {
+            uint64_t y = mul2(pair2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), w0);
+            if (both) y = fma2(pair2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), w1, y);
+            unpair2(y, f[e], f[e + 1]);
+          }
+          if (whole) {
+            if (valid) {
+              uint4* dst = reinterpret_cast<uint4*>(a.out + out_at + cc * 32);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint4 y = make_uint4(pack_bf16x2(f[8 * e], f[8 * e + 1]), pack_bf16x2(f[8 * e + 2], f[8 * e + 3]),
+                                           pack_bf16x2(f[8 * e + 4], f[8 * e + 5]), pack_bf16x2(f[8 * e + 6], f[8 * e + 7]));
+                dst[e] = sees ? y : make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
           } else if (valid) {
             float4* dst = reinterpret_cast<float4*>(a.part_o + part * TA_DH + cc * 32);
 #pragma unroll
@@ -661,19 +715,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {  // O may be overwritten; the stores of a whole unit's result need not hold that up
+      if (lane == 0) {
         mbar_arrive(&sm.o_free[grp]);
         if (nrt == 1) mbar_arrive(&sm.o_free[grp ^ 1]);
       }
-      if (valid) {
-        if (whole) {
-          uint4* dst = reinterpret_cast<uint4*>(a.out + out_at);
-#pragma unroll
-          for (int q = 0; q < 16; ++q) dst[q] = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
-        } else {
-          a.part_ml[part] = make_float2(m, l);
-        }
-      }
+      if (valid && !whole) a.part_ml[part] = make_float2(m, l);
       __syncwarp();
     }
     if (!ok && lane == 0) atomicCAS(a.status, 0, ST_TIMEOUT_TMEM_FULL);
@@ -780,7 +826,9 @@ extern "C" int b200_tree_attn(const void* qkv, long long ld, const void* k_cache
   if (B <= 0 || N <= 0) return 0;
   const int need = b200_tree_attn_scratch(max_nodes, Hq, Hkv);
   if (Dh != TA_DH || need < 0 || num_blocks < 1 || max_blocks > (1 << 24)) return -1;
-  if ((static_cast<long long>(num_blocks) + 1) * Hkv * TA_PAGE >= (1ll << 31)) return -3;  // rows of the cache are 32-bit TMA coordinates
+  // rows of the cache are 32-bit TMA coordinates, tiles are counted in 32 bits
+  if ((static_cast<long long>(num_blocks) + 1) * Hkv * TA_PAGE >= (1ll << 31)) return -3;
+  if (static_cast<double>(B) * Hkv * ((max_nodes + 2 * (128 / (Hq / Hkv)) - 1) / (2 * (128 / (Hq / Hkv)))) * (max_blocks / 2 + 2) >= 2147483648.0) return -3;
   TreeArgs a;
   a.G = Hq / Hkv;
   a.npt = 128 / a.G;
