@@ -18,11 +18,16 @@
 // a second kernel joins in the order of the keys.  The shares are computed from ctx and cu on the device, so one captured graph
 // serves every step.
 //
-// One CTA: warp 0 streams pages with TMA through a ring of five 32 KB buffers, warp 1 issues S = Q K^T and O += P V, two groups
+// One CTA: warp 0 streams pages with TMA through a ring of four 32 KB buffers, warp 1 issues S = Q K^T and O += P V, two groups
 // of four warps own the softmax (warps 4 to 7 and 8 to 11), warp 2 plans the segments ahead.  A unit of two row tiles gives each group one of them (the keys are loaded once for both); a
 // unit of one row tile gives the groups alternate key tiles, merged at the end, so that one group's exponentials always run
 // beside the other group's products.  P replaces S in tensor memory (bf16), O stays there for the whole unit and is rescaled
 // only when the row maximum has grown by more than 2^8.
+//
+// A narrow unit has at most 32 rows (single tokens and short drafts); one warp per group would then do all the exponentials.
+// Its queries are laid into all four quarters of the row tile, so that every warp of a group finds the same 32 rows in its part of
+// tensor memory and takes 32 of the 128 keys; they agree on the rows' maxima through shared memory, and P goes back through it
+// (rows 0 .. 31 of the operand count; what lies behind them lands in rows of O that nobody reads).
 #include "common.cuh"
 
 namespace b200 {
@@ -37,7 +42,8 @@ constexpr int TA_REGS = 168, TA_REGS_ISSUE = 56, TA_REGS_SOFTMAX = 224;
 static_assert(TA_REGS_ISSUE + 2 * TA_REGS_SOFTMAX <= 3 * TA_REGS, "the groups' shares exceed what the block is launched with");
 constexpr int TA_SUB = 128 * 64 * 2;     // bytes of one [128 x 64] swizzled sub-tile
 constexpr int TA_TILE = 2 * TA_SUB;      // a [128 keys or rows x 128] bf16 tile
-constexpr int TA_RING = 5;
+constexpr int TA_RING = 4;               // two tiles of keys and values in flight (a fifth buffer was measured to change nothing)
+constexpr int TA_PSUB = 32 * 64 * 2;     // a narrow unit's P: two [32 x 64] swizzled sub-tiles
 constexpr int TA_MIN_TILES = 2;          // key tiles a CTA takes at least: below that joining the parts costs more than it saves
 constexpr float TA_LOG2E = 1.4426950408889634f;
 
@@ -49,7 +55,7 @@ struct TreeArgs {
   const int* cu;
   const int* parents;
   int B, N, max_nodes, Hq, Hkv;
-  int G, npt;           // query heads per KV head, nodes per row tile
+  int G, npt, npt32;    // query heads per KV head, nodes per row tile and per 32 rows
   int part_rows;        // rows of a part in the workspace
   float scale;
   __nv_bfloat16* out;
@@ -88,7 +94,7 @@ struct TreeShares {
 struct TreeSegment {
   int n0, T, C, nt;      // first row of the sequence in the batch, its nodes, its cached keys, tiles of the unit
   int t0, t1;            // tiles of this segment (none: the CTA is done)
-  int kvh, first, nrt;   // KV head, first node of the unit, row tiles
+  int kvh, first, nrt;   // KV head, first node of the unit, row tiles (0: one of at most 32 rows, see below)
   int y0, y1;            // cache rows of the first tile's pages (-1: none)
   int b;
   unsigned long long sees[TA_MAX_NODES];
@@ -100,10 +106,12 @@ __device__ __forceinline__ int ring_v(int i, int n) { return i == n - 1 ? 2 * n 
 
 struct TreeSmem {
   uint8_t q[2][TA_TILE];
+  uint8_t p[2][2 * TA_PSUB];  // before the ring: the products read 128 rows from here on
   uint8_t ring[TA_RING][TA_TILE];
-  float2 ml[128];        // (maximum, sum) of the group that does not write a one-row-tile unit's result
+  float ml[256];         // maxima and sums on their way to the group that writes a unit's result
+  uint16_t mx[2][4][32]; // narrow units: the row maxima of the four warps of a group, cut to bf16
   TreeSegment seg[2];
-  uint64_t q_full[2], q_empty[2], r_full[TA_RING], r_empty[TA_RING], s_full[2], p_full[2], o_full[2], o_free[2], seg_full[2], seg_empty[2], ml_full;
+  uint64_t q_full[2], q_empty[2], r_full[TA_RING], r_empty[TA_RING], s_full[2], p_full[2], o_full[2], o_free[2], seg_full[2], seg_empty[2], ml_full[2], mx_full[2], lx_full[2];
   int scan[TA_THREADS / 32];
   TreeSeq at;            // the sequence in which the CTA's share begins
   int at_seq, at_off;
@@ -156,7 +164,7 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 __device__ __forceinline__ unsigned long long low_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
 __global__ void __launch_bounds__(TA_THREADS, 1)
-tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_node, const __grid_constant__ CUtensorMap tm_k,
+tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_q32, const __grid_constant__ CUtensorMap tm_node, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TreeArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   TreeSmem& sm = *reinterpret_cast<TreeSmem*>(smem_raw);
@@ -164,6 +172,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   volatile int* abort_flag = &sm.abort_flag;
   if (tid == 32) {
     prefetch_tensormap(&tm_q);
+    prefetch_tensormap(&tm_q32);
     prefetch_tensormap(&tm_node);
     prefetch_tensormap(&tm_k);
     prefetch_tensormap(&tm_v);
@@ -175,7 +184,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.p_full[i], 4);
       mbar_init(&sm.o_full[i], 1);
-      mbar_init(&sm.o_free[i], 4);
+      mbar_init(&sm.o_free[i], 8);
+      mbar_init(&sm.ml_full[i], 4);
+      mbar_init(&sm.lx_full[i], 3);
+      mbar_init(&sm.mx_full[i], 4);
       mbar_init(&sm.seg_full[i], 1);
       mbar_init(&sm.seg_empty[i], 10);  // the TMA and the product threads, eight softmax warps
     }
@@ -183,7 +195,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_init(&sm.r_full[i], 1);
       mbar_init(&sm.r_empty[i], 1);
     }
-    mbar_init(&sm.ml_full, 4);
     sm.abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -308,7 +319,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             g.nt = q.nt;
             g.kvh = kvh;
             g.first = first;
-            g.nrt = q.T - first > a.npt ? 2 : 1;
+            g.nrt = q.T <= a.npt32 ? 0 : q.T - first > a.npt ? 2 : 1;
             g.b = b;
             if (left <= t1 - t0) {  // the CTA's last: a unit that begins here and goes on elsewhere is joined from its parts
               int4 join = make_int4(0, 0, 0, 0);
@@ -351,7 +362,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           const TreeSegment& g = sm.seg[n & 1];
           ok = mbar_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
           if (!ok || g.t0 == g.t1) break;
-          const int t0 = g.t0, t1 = g.t1, tree = g.nt - 1, kvh = g.kvh, nrt = g.nrt, C = g.C, n0 = g.n0;
+          const int t0 = g.t0, t1 = g.t1, tree = g.nt - 1, kvh = g.kvh, C = g.C, n0 = g.n0;
+          const bool narrow = g.nrt == 0;
+          const int nrt = narrow ? 1 : g.nrt;
           int yk0 = g.y0, yk1 = g.y1;  // page rows of the next tile of K
           const int q0 = n0 + g.first;
           const int* row = a.table + g.b * a.table_ld;
@@ -360,6 +373,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const int s = qc & 1;
             ok = mbar_wait(&sm.q_empty[s], ((qc >> 1) & 1) ^ 1, abort_flag);
             if (!ok) break;
+            if (narrow) {  // the same rows in every quarter of the tile
+              mbar_expect_tx(&sm.q_full[s], a.G * a.npt32 * 1024);
+              for (int copy = 0; copy < 4; ++copy) {
+                tma_load_3d(sm.q[s] + copy * 4096, &tm_q32, &sm.q_full[s], 0, kvh * a.G, q0);
+                tma_load_3d(sm.q[s] + TA_SUB + copy * 4096, &tm_q32, &sm.q_full[s], 64, kvh * a.G, q0);
+              }
+              continue;
+            }
             mbar_expect_tx(&sm.q_full[s], a.G * a.npt * 256);
             tma_load_3d(sm.q[s], &tm_q, &sm.q_full[s], 0, kvh * a.G, q0 + rt * a.npt);
             tma_load_3d(sm.q[s] + TA_SUB, &tm_q, &sm.q_full[s], 64, kvh * a.G, q0 + rt * a.npt);
@@ -409,7 +430,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         struct Job {
           int grp, vslot;
           uint32_t vpar;
-          bool half, wait_v, free_v, first, last;
+          bool narrow, half, wait_v, free_v, first, last, alone;
         };
         uint32_t jc = 0, rbase = 0, qc = 0, pc = 0;  // pc: bit g is the parity of group g's next P
         bool ok = true;
@@ -422,11 +443,20 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           pc ^= 1u << j.grp;
           if (j.wait_v && !mbar_wait(&sm.r_full[j.vslot], j.vpar, abort_flag)) return give_up(ST_TIMEOUT_FULL);
           // a group's first product of a unit overwrites its O: the last unit's must have been read
-          if (j.first && seg > 0 && !mbar_wait(&sm.o_free[j.grp], (seg - 1) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
+          // (each barrier is waited for once a segment, so that a parity always means the phase before)
+          if (j.first && seg > 0 &&
+              !(mbar_wait(&sm.o_free[j.grp], (seg - 1) & 1, abort_flag) && (!j.alone || mbar_wait(&sm.o_free[j.grp ^ 1], (seg - 1) & 1, abort_flag))))
+            return give_up(ST_TIMEOUT_TMEM_EMPTY);
           tc_fence_after();
           const uint32_t v = smem_u32(sm.ring[j.vslot]), p = tmem + j.grp * 128, o = tmem + 256 + j.grp * 128;
           const int steps = j.half ? 4 : 8;
-          for (int k = 0; k < steps; ++k) umma_ts(o, p + k * 8, ta_desc_mn(v, k), idesc_o, !(j.first && k == 0));
+          if (j.narrow) {
+            const uint32_t ps = smem_u32(sm.p[j.grp]);
+            for (int k = 0; k < steps; ++k)
+              umma_ss(o, umma_desc_sw128(ps + (k >> 2) * TA_PSUB + (k & 3) * 32, 16, 1024), ta_desc_mn(v, k), idesc_o, !(j.first && k == 0));
+          } else {
+            for (int k = 0; k < steps; ++k) umma_ts(o, p + k * 8, ta_desc_mn(v, k), idesc_o, !(j.first && k == 0));
+          }
           if (j.free_v) umma_commit(&sm.r_empty[j.vslot]);
           if (j.last) umma_commit(&sm.o_full[j.grp]);
           return true;
@@ -441,7 +471,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             break;
           }
           if (g.t0 == g.t1) break;
-          const int count = g.t1 - g.t0, nrt = g.nrt, jobs = count * nrt;
+          const bool narrow = g.nrt == 0;
+          const int count = g.t1 - g.t0, nrt = narrow ? 1 : g.nrt, jobs = count * nrt;
           const int half_at = g.C <= (g.nt - 1) * 128 ? g.nt - 1 - g.t0 : -1;  // the tree's tile without a page: 64 keys
           mbar_arrive(&sm.seg_empty[n & 1]);
           for (int x = 0; x < jobs && ok; ++x, ++jc) {
@@ -450,12 +481,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             j.grp = jc & 1;
             const uint32_t kn = rbase + ring_k(i), vn = rbase + ring_v(i, count);
             const int ks = kn % TA_RING, qs = (qc + rt) & 1;
+            j.narrow = narrow;
             j.vslot = vn % TA_RING;
             j.vpar = (vn / TA_RING) & 1;
             j.half = i == half_at;
             j.wait_v = rt == 0;
             j.free_v = rt == nrt - 1;
             j.first = x < 2;
+            j.alone = jobs == 1;
             j.last = x >= jobs - 2;
             if ((i == 0 && !mbar_wait(&sm.q_full[qs], ((qc + rt) >> 1) & 1, abort_flag)) ||
                 (rt == 0 && !mbar_wait(&sm.r_full[ks], (kn / TA_RING) & 1, abort_flag))) {
@@ -487,20 +520,22 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const uint32_t t_s = tmem + grp * 128 + lane_off, t_o = tmem + 256 + lane_off;
     const float c = a.scale * TA_LOG2E;
     uint32_t jc = 0, rbase = 0;
-    uint32_t par_s = 0, par_o = 0, par_ml = 0;  // parities of the next S, of the next O of either group (bits 0 and 1), of the next exchange
+    uint32_t par_s = 0, par_o = 0, par_ml = 0, par_mx = 0, par_lx = 0;  // parities of the next S, of either group's O (bits 0, 1), of exchanges
     bool late = false;                            // this group's last O was somebody else's to wait for
-    const int rn = r / a.G, rg = r - rn * a.G;  // node of the row tile and head of the group
+    const int rn = r / a.G, rg = r - rn * a.G;                // node of the row tile and head of the group
+    const int rn32 = lane / a.G, rg32 = lane - rn32 * a.G;  // the same in a narrow unit
     bool ok = true;
     for (uint32_t n = 0; ok; ++n) {
       const TreeSegment& g = sm.seg[n & 1];
       ok = ta_warp_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
       if (!ok || g.t0 == g.t1) break;
-      const int t0 = g.t0, count = g.t1 - t0, nt = g.nt, nrt = g.nrt, T = g.T, C = g.C, jobs = count * nrt;
+      const bool narrow = g.nrt == 0;
+      const int t0 = g.t0, count = g.t1 - t0, nt = g.nt, nrt = narrow ? 1 : g.nrt, T = g.T, C = g.C, jobs = count * nrt;
       const int x0 = (grp ^ jc) & 1;           // my first job of this segment; then every second one
-      const int rt = nrt == 2 ? x0 : 0, node = g.first + rt * a.npt + rn;
-      const bool valid = rn < a.npt && node < T;
+      const int rt = nrt == 2 ? x0 : 0, node = narrow ? rn32 : g.first + rt * a.npt + rn;
+      const bool valid = (narrow || rn < a.npt) && node < T;
       const unsigned long long sees = valid ? g.sees[node] : 0ull;
-      const long long out_at = ((static_cast<long long>(g.n0) + node) * a.Hq + g.kvh * a.G + rg) * TA_DH;
+      const long long out_at = ((static_cast<long long>(g.n0) + node) * a.Hq + g.kvh * a.G + (narrow ? rg32 : rg)) * TA_DH;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.seg_empty[n & 1]);
       const bool busy = __any_sync(0xffffffffu, valid);
@@ -548,7 +583,71 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             fence_proxy_async();
           }
         }
-        if (busy) {
+        if (narrow) {
+          // ---- at most 32 rows: S holds them four times, warp lg takes 32 of the 128 columns; P goes through shared memory
+          uint32_t sv[32];
+          tmem_ld32(t_s + lg * 32, sv);
+          const uint32_t word = static_cast<uint32_t>((lg & 2 ? hi : lo) >> (lg & 1) * 32);
+          tmem_ld_wait();
+          if (__any_sync(0xffffffffu, word != ~0u)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((word >> e) & 1u)) sv[e] = 0xff800000u;
+          }
+          float mx2[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) mx2[e / 2 & 1] = max3(mx2[e / 2 & 1], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+          sm.mx[grp][lg][lane] = static_cast<uint16_t>(__float_as_uint(fmaxf(mx2[0], mx2[1])) >> 16);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.mx_full[grp]);
+          ok = ta_warp_wait(&sm.mx_full[grp], par_mx, abort_flag);
+          par_mx ^= 1;
+          if (!ok) break;
+          float mx = -INFINITY;  // cut to bf16, the same in all four warps; only a reference point of the exponentials
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx = fmaxf(mx, __uint_as_float(static_cast<uint32_t>(sm.mx[grp][k][lane]) << 16));
+          float alpha = 1.f;
+          const bool grow = (mx - m) * c > 8.f;
+          if (grow) {
+            alpha = ex2_approx((m - mx) * c);
+            m = mx;
+            l *= alpha;
+          }
+          const uint64_t c2 = pair2(c, c), mc2 = pair2(-m * c, -m * c);
+          uint64_t sum[2] = {0ull, 0ull};
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float p0, p1;
+            unpair2(fma2(pair2(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), c2, mc2), p0, p1);
+            p0 = ex2_approx(p0);
+            p1 = ex2_approx(p1);
+            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair2(p0, p1));
+            pk[e >> 1] = pack_bf16x2(p0, p1);
+          }
+          {
+            float s0, s1;
+            unpair2(add2(sum[0], sum[1]), s0, s1);
+            l += s0 + s1;
+          }
+          uint8_t* prow = sm.p[grp] + (lg >> 1) * TA_PSUB + lane * 128;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(prow + ((((lg & 1) * 4 + q) ^ (lane & 7)) << 4)) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+          fence_proxy_async();
+          if (x >= 2 && lg == 0 && __any_sync(0xffffffffu, grow)) {  // the rows of O that count are in the first quarter
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) {
+              uint32_t o[32];
+              tmem_ld32(t_o + grp * 128 + cc * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st32(t_o + grp * 128 + cc * 32, o);
+            }
+            tmem_st_wait();
+          }
+        } else if (busy) {
           uint32_t sv[4][32];
           tmem_ld32(t_s, sv[0]);
           tmem_ld32(t_s + 32, sv[1]);
@@ -641,48 +740,73 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       jc += jobs;
       rbase += 2 * count;
       float a0 = 1.f, a1 = 0.f;  // weights of my own O and of the other group's
+      // Every warp waits for the end of the last segment and says when it is through with this one, so no barrier is ever more than
+      // one phase away from a parity that somebody waits for.
+      if (n > 0) {
+        ok = ta_warp_wait(&sm.o_free[0], (n - 1) & 1, abort_flag) && ta_warp_wait(&sm.o_free[1], (n - 1) & 1, abort_flag);
+        if (!ok) break;
+      }
       if (nrt == 2) {
+        if (lane == 0) mbar_arrive(&sm.o_free[grp ^ 1]);
         ok = ta_warp_wait(&sm.o_full[grp], par_o >> grp & 1, abort_flag);
         par_o ^= 3;
         if (!ok) break;
       } else if (grp != last) {
         if (both) {
-          if (n > 0) ok = ta_warp_wait(&sm.o_free[0], (n - 1) & 1, abort_flag);  // the last pair has been read
-          if (!ok) break;
-          sm.ml[r] = make_float2(m, l);
+          sm.ml[r] = l;
+          if (!narrow || lg == 0) sm.ml[128 + r] = m;
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.ml_full);
+          if (lane == 0) mbar_arrive(&sm.ml_full[grp]);
           late = true;
         }
+        if (lane == 0) {
+          mbar_arrive(&sm.o_free[0]);
+          mbar_arrive(&sm.o_free[1]);
+        }
         par_o ^= both ? 3 : 1 << last;
-        par_ml ^= both;
         continue;
       } else {
+        float m_other = 0.f, l_other = 0.f;
+        if (narrow) {  // the first warp collects its three neighbours' sums
+          if (lg > 0) {
+            sm.ml[128 + r] = l;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.lx_full[grp]);
+          } else {
+            ok = ta_warp_wait(&sm.lx_full[grp], par_lx, abort_flag);
+            if (!ok) break;
+            l += sm.ml[160 + lane] + sm.ml[192 + lane] + sm.ml[224 + lane];
+          }
+          par_lx ^= 1;
+        }
         if (both) {
-          ok = ta_warp_wait(&sm.ml_full, par_ml, abort_flag);
+          ok = ta_warp_wait(&sm.ml_full[grp ^ 1], par_ml, abort_flag);
+          par_ml ^= 1;
           if (ok) ok = ta_warp_wait(&sm.o_full[grp ^ 1], par_o >> (grp ^ 1) & 1, abort_flag);
           if (!ok) break;
-          const float2 other = sm.ml[r];
-          const float top = fmaxf(m, other.x);
+          l_other = sm.ml[narrow ? lane : r];
+          if (narrow) l_other += sm.ml[32 + lane] + sm.ml[64 + lane] + sm.ml[96 + lane];
+          m_other = sm.ml[128 + (narrow ? lane : r)];
+          const float top = fmaxf(m, m_other);
           a0 = l != 0.f ? ex2_approx(m - top) : 0.f;
-          a1 = other.y != 0.f ? ex2_approx(other.x - top) : 0.f;
-          l = a0 * l + a1 * other.y;
+          a1 = l_other != 0.f ? ex2_approx(m_other - top) : 0.f;
+          l = a0 * l + a1 * l_other;
           m = top;
         }
         ok = ta_warp_wait(&sm.o_full[grp], par_o >> grp & 1, abort_flag);
         par_o ^= both ? 3 : 1 << grp;
-        par_ml ^= both;
         if (!ok) break;
       }
       tc_fence_after();
       const bool whole = t0 == 0 && count == nt;
-      const long long part = (static_cast<long long>(cta) * 2 + (t0 == 0 ? 1 : 0)) * a.part_rows + rt * 128 + r;
+      const long long part = (static_cast<long long>(cta) * 2 + (t0 == 0 ? 1 : 0)) * a.part_rows + rt * 128 + (narrow ? lane : r);
+      const bool mine = valid && !(narrow && lg > 0);  // rows of the result in this warp
       if (whole) {  // a row that sees nothing gives zeros (below), a NaN stays one
         a0 *= 1.f / l;
         a1 *= 1.f / l;
       }
       const uint64_t w0 = pair2(a0, a0), w1 = pair2(a1, a1);
-      if (busy) {
+      if (busy && !(narrow && lg > 0)) {
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
           uint32_t v[32], u[32];
@@ -697,7 +821,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             unpair2(y, f[e], f[e + 1]);
           }
           if (whole) {
-            if (valid) {
+            if (mine) {
               uint4* dst = reinterpret_cast<uint4*>(a.out + out_at + cc * 32);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -706,7 +830,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 dst[e] = sees ? y : make_uint4(0u, 0u, 0u, 0u);
               }
             }
-          } else if (valid) {
+          } else if (mine) {
             float4* dst = reinterpret_cast<float4*>(a.part_o + part * TA_DH + cc * 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
@@ -719,7 +843,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         mbar_arrive(&sm.o_free[grp]);
         if (nrt == 1) mbar_arrive(&sm.o_free[grp ^ 1]);
       }
-      if (valid && !whole) a.part_ml[part] = make_float2(m, l);
+      if (mine && !whole) a.part_ml[part] = make_float2(m, l);
       __syncwarp();
     }
     if (!ok && lane == 0) atomicCAS(a.status, 0, ST_TIMEOUT_TMEM_FULL);
@@ -832,9 +956,11 @@ extern "C" int b200_tree_attn(const void* qkv, long long ld, const void* k_cache
   TreeArgs a;
   a.G = Hq / Hkv;
   a.npt = 128 / a.G;
-  CUtensorMap tq, tn, tk, tv;
+  a.npt32 = 32 / a.G;
+  CUtensorMap tq, tq32, tn, tk, tv;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * Hkv * TA_PAGE;
   int r = ta_map_3d(&tq, qkv, ld, Hq + 2 * Hkv, N, a.G, a.npt);
+  if (!r) r = ta_map_3d(&tq32, qkv, ld, Hq + 2 * Hkv, N, a.G, a.npt32 ? a.npt32 : 1);
   if (!r) r = ta_map_3d(&tn, qkv, ld, Hq + 2 * Hkv, N, 1, TA_MAX_NODES);
   if (!r) r = make_tmap_2d(&tk, k_cache, rows, TA_DH, TA_DH, TA_PAGE, 64, 2, true);
   if (!r) r = make_tmap_2d(&tv, v_cache, rows, TA_DH, TA_DH, TA_PAGE, 64, 2, true);
@@ -869,7 +995,7 @@ extern "C" int b200_tree_attn(const void* qkv, long long ld, const void* k_cache
   }();
   if (regs != TA_REGS) return -4;  // the register split of the groups would wait for registers that the launch did not bring
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  e = launch_pdl(tree_attn_kernel, dim3(sms), dim3(TA_THREADS), smem, st, tq, tn, tk, tv, a);
+  e = launch_pdl(tree_attn_kernel, dim3(sms), dim3(TA_THREADS), smem, st, tq, tq32, tn, tk, tv, a);
   if (e != cudaSuccess) return static_cast<int>(e);
   e = launch_pdl(tree_join_kernel, dim3(sms, (a.part_rows + 31) / 32), dim3(256), 0, st, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
