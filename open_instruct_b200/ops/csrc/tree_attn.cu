@@ -24,10 +24,11 @@
 // beside the other group's products.  P replaces S in tensor memory (bf16), O stays there for the whole unit and is rescaled
 // only when the row maximum has grown by more than 2^8.
 //
-// A narrow unit has at most 32 rows (single tokens and short drafts); one warp per group would then do all the exponentials.
-// Its queries are laid into all four quarters of the row tile, so that every warp of a group finds the same 32 rows in its part of
-// tensor memory and takes 32 of the 128 keys; they agree on the rows' maxima through shared memory, and P goes back through it
-// (rows 0 .. 31 of the operand count; what lies behind them lands in rows of O that nobody reads).
+// A second kernel serves batches whose units have at most 32 rows (single tokens and short drafts).  As rows of a 128-row tile they would leave three quarters
+// of the tensor work and most of the softmax warps to padding - and the padding is paid for in power: at 8 rows a unit the GPU
+// ran at its 1000 W limit with the clock down to 1.5 GHz.  So the products are turned round, S^T = K Q^T and O^T = V^T P^T, with
+// the 128 keys (the 128 dimensions) as the tile's rows and 32 columns: a quarter of the tensor work, every thread of a group
+// has one key and 32 rows, and the result's rows are written by all of its warps.
 #include "common.cuh"
 
 namespace b200 {
@@ -43,7 +44,7 @@ static_assert(TA_REGS_ISSUE + 2 * TA_REGS_SOFTMAX <= 3 * TA_REGS, "the groups' s
 constexpr int TA_SUB = 128 * 64 * 2;     // bytes of one [128 x 64] swizzled sub-tile
 constexpr int TA_TILE = 2 * TA_SUB;      // a [128 keys or rows x 128] bf16 tile
 constexpr int TA_RING = 4;               // two tiles of keys and values in flight (a fifth buffer was measured to change nothing)
-constexpr int TA_PSUB = 32 * 64 * 2;     // a narrow unit's P: two [32 x 64] swizzled sub-tiles
+constexpr int TA_QSUB = 32 * 64 * 2;     // a narrow unit's queries: two [32 x 64] swizzled sub-tiles
 constexpr int TA_MIN_TILES = 2;          // key tiles a CTA takes at least: below that joining the parts costs more than it saves
 constexpr float TA_LOG2E = 1.4426950408889634f;
 
@@ -55,7 +56,7 @@ struct TreeArgs {
   const int* cu;
   const int* parents;
   int B, N, max_nodes, Hq, Hkv;
-  int G, npt, npt32;    // query heads per KV head, nodes per row tile and per 32 rows
+  int G, npt;           // query heads per KV head, nodes per row tile (narrow kernel: of 32 rows)
   int part_rows;        // rows of a part in the workspace
   float scale;
   __nv_bfloat16* out;
@@ -94,7 +95,7 @@ struct TreeShares {
 struct TreeSegment {
   int n0, T, C, nt;      // first row of the sequence in the batch, its nodes, its cached keys, tiles of the unit
   int t0, t1;            // tiles of this segment (none: the CTA is done)
-  int kvh, first, nrt;   // KV head, first node of the unit, row tiles (0: one of at most 32 rows, see below)
+  int kvh, first, nrt;   // KV head, first node of the unit, row tiles
   int y0, y1;            // cache rows of the first tile's pages (-1: none)
   int b;
   unsigned long long sees[TA_MAX_NODES];
@@ -104,21 +105,26 @@ struct TreeSegment {
 __device__ __forceinline__ int ring_k(int i) { return i == 0 ? 0 : 2 * i - 1; }
 __device__ __forceinline__ int ring_v(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
 
+template <bool NARROW>
 struct TreeSmem {
-  uint8_t q[2][TA_TILE];
-  uint8_t p[2][2 * TA_PSUB];  // before the ring: the products read 128 rows from here on
-  uint8_t ring[TA_RING][TA_TILE];
+  static constexpr int RING = NARROW ? TA_RING + 1 : TA_RING;
+  uint8_t q[2][NARROW ? 2 * TA_QSUB : TA_TILE];
+  uint8_t p[NARROW ? 2 : 1][NARROW ? 128 * 32 * 2 : 1024];  // narrow units: the groups' P^T, [128 keys x 32 rows]
+  uint8_t ring[RING][TA_TILE];
   float ml[256];         // maxima and sums on their way to the group that writes a unit's result
-  uint16_t mx[2][4][32]; // narrow units: the row maxima of the four warps of a group, cut to bf16
+  float ls[2][4][32], lm[2][32];  // narrow units: the same, by group, warp and row
+  float mx[2][4][32];    // narrow units: row maxima by group and warp
+  float wt[8][2][32];    // narrow units: a warp's weights of the rows, on their way from one lane to all
+  uint32_t flags[2];     // narrow units: a byte for each warp of a group
   TreeSegment seg[2];
-  uint64_t q_full[2], q_empty[2], r_full[TA_RING], r_empty[TA_RING], s_full[2], p_full[2], o_full[2], o_free[2], seg_full[2], seg_empty[2], ml_full[2], mx_full[2], lx_full[2];
+  uint64_t q_full[2], q_empty[2], r_full[RING], r_empty[RING], s_full[2], p_full[2], o_full[2], o_free[2], seg_full[2], seg_empty[2], ml_full[2], lx_full[2], flag_full[2], mx_full[2];
   int scan[TA_THREADS / 32];
   TreeSeq at;            // the sequence in which the CTA's share begins
   int at_seq, at_off;
   uint32_t tmem_ptr;
   int abort_flag;
 };
-static_assert(sizeof(TreeSmem) <= 232448, "shared memory of a CTA");
+static_assert(sizeof(TreeSmem<false>) <= 232448 && sizeof(TreeSmem<true>) <= 232448, "shared memory of a CTA");
 
 __device__ __forceinline__ uint64_t ta_desc_k(uint32_t tile, int k) { return umma_desc_sw128(tile + (k >> 2) * TA_SUB + (k & 3) * 32, 16, 1024); }
 __device__ __forceinline__ uint64_t ta_desc_mn(uint32_t tile, int k) { return umma_desc_sw128(tile + k * 2048, TA_SUB, 1024); }
@@ -160,19 +166,36 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
   return d;
 }
+__device__ __forceinline__ float warp_max(float x) {
+  float d;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(x));
+  return d;
+}
+// MN-major operand of 32 bf16 (64 bytes) a row, 64-byte swizzle: rows indexed by K, groups of 8 rows 512 bytes apart
+__device__ __forceinline__ uint64_t ta_desc_p(uint32_t addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr & 0x3FFFF) >> 4);
+  d |= static_cast<uint64_t>(8192 >> 4) << 16;
+  d |= static_cast<uint64_t>(512 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(4) << 61;  // SWIZZLE_64B
+  return d;
+}
 // the low n bits, n in 0 .. 64
 __device__ __forceinline__ unsigned long long low_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
+template <bool narrow>
 __global__ void __launch_bounds__(TA_THREADS, 1)
-tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_q32, const __grid_constant__ CUtensorMap tm_node, const __grid_constant__ CUtensorMap tm_k,
+tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_node, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TreeArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  TreeSmem& sm = *reinterpret_cast<TreeSmem*>(smem_raw);
+  typedef TreeSmem<narrow> Smem;
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  constexpr int RING = Smem::RING;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &sm.abort_flag;
   if (tid == 32) {
     prefetch_tensormap(&tm_q);
-    prefetch_tensormap(&tm_q32);
     prefetch_tensormap(&tm_node);
     prefetch_tensormap(&tm_k);
     prefetch_tensormap(&tm_v);
@@ -186,17 +209,22 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_init(&sm.o_full[i], 1);
       mbar_init(&sm.o_free[i], 8);
       mbar_init(&sm.ml_full[i], 4);
-      mbar_init(&sm.lx_full[i], 3);
+      mbar_init(&sm.lx_full[i], 4);
+      mbar_init(&sm.flag_full[i], 4);
       mbar_init(&sm.mx_full[i], 4);
       mbar_init(&sm.seg_full[i], 1);
       mbar_init(&sm.seg_empty[i], 10);  // the TMA and the product threads, eight softmax warps
     }
-    for (int i = 0; i < TA_RING; ++i) {
+    for (int i = 0; i < RING; ++i) {
       mbar_init(&sm.r_full[i], 1);
       mbar_init(&sm.r_empty[i], 1);
     }
     sm.abort_flag = 0;
     fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (narrow) {  // rows that no query fills: finite whatever the memory held
+    for (int i = tid; i < static_cast<int>(sizeof(sm.q) / 16); i += TA_THREADS) reinterpret_cast<uint4*>(sm.q)[i] = make_uint4(0u, 0u, 0u, 0u);
     fence_proxy_async();
   }
   griddep_launch_dependents();
@@ -319,7 +347,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             g.nt = q.nt;
             g.kvh = kvh;
             g.first = first;
-            g.nrt = q.T <= a.npt32 ? 0 : q.T - first > a.npt ? 2 : 1;
+            g.nrt = !narrow && q.T - first > a.npt ? 2 : 1;
             g.b = b;
             if (left <= t1 - t0) {  // the CTA's last: a unit that begins here and goes on elsewhere is joined from its parts
               int4 join = make_int4(0, 0, 0, 0);
@@ -352,8 +380,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         uint32_t rc = 0, qc = 0;  // loads issued into the ring, row tiles issued
         bool ok = true;
         auto ring_slot = [&](uint32_t bytes) -> int {
-          const int s = rc % TA_RING;
-          if (!mbar_wait(&sm.r_empty[s], ((rc / TA_RING) & 1) ^ 1, abort_flag)) return -1;
+          const int s = rc % RING;
+          if (!mbar_wait(&sm.r_empty[s], ((rc / RING) & 1) ^ 1, abort_flag)) return -1;
           mbar_expect_tx(&sm.r_full[s], bytes);
           ++rc;
           return s;
@@ -363,8 +391,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           ok = mbar_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
           if (!ok || g.t0 == g.t1) break;
           const int t0 = g.t0, t1 = g.t1, tree = g.nt - 1, kvh = g.kvh, C = g.C, n0 = g.n0;
-          const bool narrow = g.nrt == 0;
-          const int nrt = narrow ? 1 : g.nrt;
+          const int nrt = g.nrt;
           int yk0 = g.y0, yk1 = g.y1;  // page rows of the next tile of K
           const int q0 = n0 + g.first;
           const int* row = a.table + g.b * a.table_ld;
@@ -373,12 +400,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const int s = qc & 1;
             ok = mbar_wait(&sm.q_empty[s], ((qc >> 1) & 1) ^ 1, abort_flag);
             if (!ok) break;
-            if (narrow) {  // the same rows in every quarter of the tile
-              mbar_expect_tx(&sm.q_full[s], a.G * a.npt32 * 1024);
-              for (int copy = 0; copy < 4; ++copy) {
-                tma_load_3d(sm.q[s] + copy * 4096, &tm_q32, &sm.q_full[s], 0, kvh * a.G, q0);
-                tma_load_3d(sm.q[s] + TA_SUB + copy * 4096, &tm_q32, &sm.q_full[s], 64, kvh * a.G, q0);
-              }
+            if (narrow) {
+              mbar_expect_tx(&sm.q_full[s], a.G * a.npt * 256);
+              tma_load_3d(sm.q[s], &tm_q, &sm.q_full[s], 0, kvh * a.G, q0);
+              tma_load_3d(sm.q[s] + TA_QSUB, &tm_q, &sm.q_full[s], 64, kvh * a.G, q0);
               continue;
             }
             mbar_expect_tx(&sm.q_full[s], a.G * a.npt * 256);
@@ -427,10 +452,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       if (elect_one()) {
         constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, false, false), idesc_s64 = umma_idesc_bf16(128, 64, false, false);
         constexpr uint32_t idesc_o = umma_idesc_bf16(128, 128, false, true);
+        constexpr uint32_t idesc_sn = umma_idesc_bf16(128, 32, false, false), idesc_on = umma_idesc_bf16(128, 32, true, true);
         struct Job {
           int grp, vslot;
           uint32_t vpar;
-          bool narrow, half, wait_v, free_v, first, last, alone;
+          bool half, wait_v, free_v, first, last, alone;
         };
         uint32_t jc = 0, rbase = 0, qc = 0, pc = 0;  // pc: bit g is the parity of group g's next P
         bool ok = true;
@@ -450,10 +476,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           tc_fence_after();
           const uint32_t v = smem_u32(sm.ring[j.vslot]), p = tmem + j.grp * 128, o = tmem + 256 + j.grp * 128;
           const int steps = j.half ? 4 : 8;
-          if (j.narrow) {
+          if (narrow) {
             const uint32_t ps = smem_u32(sm.p[j.grp]);
-            for (int k = 0; k < steps; ++k)
-              umma_ss(o, umma_desc_sw128(ps + (k >> 2) * TA_PSUB + (k & 3) * 32, 16, 1024), ta_desc_mn(v, k), idesc_o, !(j.first && k == 0));
+            for (int k = 0; k < steps; ++k) umma_ss(o, ta_desc_mn(v, k), ta_desc_p(ps + k * 1024), idesc_on, !(j.first && k == 0));
           } else {
             for (int k = 0; k < steps; ++k) umma_ts(o, p + k * 8, ta_desc_mn(v, k), idesc_o, !(j.first && k == 0));
           }
@@ -471,8 +496,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             break;
           }
           if (g.t0 == g.t1) break;
-          const bool narrow = g.nrt == 0;
-          const int count = g.t1 - g.t0, nrt = narrow ? 1 : g.nrt, jobs = count * nrt;
+          const int count = g.t1 - g.t0, nrt = g.nrt, jobs = count * nrt;
           const int half_at = g.C <= (g.nt - 1) * 128 ? g.nt - 1 - g.t0 : -1;  // the tree's tile without a page: 64 keys
           mbar_arrive(&sm.seg_empty[n & 1]);
           for (int x = 0; x < jobs && ok; ++x, ++jc) {
@@ -480,10 +504,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             Job j;
             j.grp = jc & 1;
             const uint32_t kn = rbase + ring_k(i), vn = rbase + ring_v(i, count);
-            const int ks = kn % TA_RING, qs = (qc + rt) & 1;
-            j.narrow = narrow;
-            j.vslot = vn % TA_RING;
-            j.vpar = (vn / TA_RING) & 1;
+            const int ks = kn % RING, qs = (qc + rt) & 1;
+            j.vslot = vn % RING;
+            j.vpar = (vn / RING) & 1;
             j.half = i == half_at;
             j.wait_v = rt == 0;
             j.free_v = rt == nrt - 1;
@@ -491,14 +514,18 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             j.alone = jobs == 1;
             j.last = x >= jobs - 2;
             if ((i == 0 && !mbar_wait(&sm.q_full[qs], ((qc + rt) >> 1) & 1, abort_flag)) ||
-                (rt == 0 && !mbar_wait(&sm.r_full[ks], (kn / TA_RING) & 1, abort_flag))) {
+                (rt == 0 && !mbar_wait(&sm.r_full[ks], (kn / RING) & 1, abort_flag))) {
               ok = give_up(ST_TIMEOUT_FULL);
               break;
             }
             tc_fence_after();
             const uint32_t q = smem_u32(sm.q[qs]), kt = smem_u32(sm.ring[ks]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) umma_ss(tmem + j.grp * 128, ta_desc_k(q, k), ta_desc_k(kt, k), j.half ? idesc_s64 : idesc_s, k != 0);
+            if (narrow) {
+              for (int k = 0; k < 8; ++k)
+                umma_ss(tmem + j.grp * 128, ta_desc_k(kt, k), umma_desc_sw128(q + (k >> 2) * TA_QSUB + (k & 3) * 32, 16, 1024), idesc_sn, k != 0);
+            } else {
+              for (int k = 0; k < 8; ++k) umma_ss(tmem + j.grp * 128, ta_desc_k(q, k), ta_desc_k(kt, k), j.half ? idesc_s64 : idesc_s, k != 0);
+            }
             if (rt == nrt - 1) umma_commit(&sm.r_empty[ks]);
             if (i == count - 1) umma_commit(&sm.q_empty[qs]);
             umma_commit(&sm.s_full[j.grp]);
@@ -520,7 +547,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const uint32_t t_s = tmem + grp * 128 + lane_off, t_o = tmem + 256 + lane_off;
     const float c = a.scale * TA_LOG2E;
     uint32_t jc = 0, rbase = 0;
-    uint32_t par_s = 0, par_o = 0, par_ml = 0, par_mx = 0, par_lx = 0;  // parities of the next S, of either group's O (bits 0, 1), of exchanges
+    uint32_t par_s = 0, par_o = 0, par_ml = 0, par_flag = 0, par_mx = 0, par_lx = 0;  // parities of the next S, of either group's O (bits 0, 1), of exchanges
     bool late = false;                            // this group's last O was somebody else's to wait for
     const int rn = r / a.G, rg = r - rn * a.G;                // node of the row tile and head of the group
     const int rn32 = lane / a.G, rg32 = lane - rn32 * a.G;  // the same in a narrow unit
@@ -529,212 +556,297 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const TreeSegment& g = sm.seg[n & 1];
       ok = ta_warp_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
       if (!ok || g.t0 == g.t1) break;
-      const bool narrow = g.nrt == 0;
       const int t0 = g.t0, count = g.t1 - t0, nt = g.nt, nrt = narrow ? 1 : g.nrt, T = g.T, C = g.C, jobs = count * nrt;
       const int x0 = (grp ^ jc) & 1;           // my first job of this segment; then every second one
-      const int rt = nrt == 2 ? x0 : 0, node = narrow ? rn32 : g.first + rt * a.npt + rn;
+      const int rt = nrt == 2 ? x0 : 0, node = narrow ? rn32 : g.first + rt * a.npt + rn;  // of this thread's row (narrow: of row `lane`)
       const bool valid = (narrow || rn < a.npt) && node < T;
       const unsigned long long sees = valid ? g.sees[node] : 0ull;
-      const long long out_at = ((static_cast<long long>(g.n0) + node) * a.Hq + g.kvh * a.G + (narrow ? rg32 : rg)) * TA_DH;
+      const long long seg_at = (static_cast<long long>(g.n0) * a.Hq + g.kvh * a.G) * TA_DH;  // the sequence's first row in the result
+      const long long out_at = seg_at + (static_cast<long long>(node) * a.Hq + (narrow ? rg32 : rg)) * TA_DH;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.seg_empty[n & 1]);
       const bool busy = __any_sync(0xffffffffu, valid);
-      float m = -INFINITY, l = 0.f;
-      for (int x = x0; x < jobs; x += 2) {
-        const int i = nrt == 2 ? x >> 1 : x, t = t0 + i;
-        ok = ta_warp_wait(&sm.s_full[grp], par_s, abort_flag);
+      float m = narrow ? 0.f : -INFINITY, l = 0.f;
+      // The scores of tile i are there: its keys (as many as 128, fewer in the last tiles) and whether it is the tree's without a
+      // page.  Rows of V that hold no key are cleared: 0 * NaN must not reach the output.
+      auto begin_job = [&](int i, int& keys, bool& half) -> bool {
+        if (!ta_warp_wait(&sm.s_full[grp], par_s, abort_flag)) return false;
         par_s ^= 1;
-        if (ok && late) {  // complete since this S was issued behind it: keeps the parity in step
-          ok = ta_warp_wait(&sm.o_full[grp], (par_o >> grp & 1) ^ 1, abort_flag);
+        if (late) {  // complete since this S was issued behind it: keeps the parity in step
+          if (!ta_warp_wait(&sm.o_full[grp], (par_o >> grp & 1) ^ 1, abort_flag)) return false;
           late = false;
         }
-        if (!ok) break;
         tc_fence_after();
-        // keys of this tile as two words of columns, and the rows of V that hold none (0 * NaN must not reach the output)
-        const int keys = min(128, C - t * 128);
-        unsigned long long lo = ~0ull, hi = ~0ull;
-        bool half = false;
-        if (t == nt - 1 || keys < 128) {
-          int z0 = keys, z1 = 128, z2 = 128, z3 = 128;  // rows [z0, z1) and [z2, z3) of V are empty
-          if (t == nt - 1) {
-            half = keys <= 0;
-            lo = half ? sees : low_bits(keys);
-            hi = half ? 0ull : sees;
-            z0 = max(keys, 0);
-            z1 = half ? 0 : 64;
-            z2 = z1 + T;
-            z3 = z1 + 64;
-          } else {
-            lo = low_bits(keys);
-            hi = low_bits(max(keys - 64, 0));
-          }
-          if (rt == 0 && (z0 < z1 || z2 < z3)) {
-            const uint32_t vn = rbase + ring_v(i, count);
-            ok = ta_warp_wait(&sm.r_full[vn % TA_RING], (vn / TA_RING) & 1, abort_flag);
-            if (!ok) break;
-            if ((r >= z0 && r < z1) || (r >= z2 && r < z3)) {
-              uint4* row = reinterpret_cast<uint4*>(sm.ring[vn % TA_RING] + r * 128);
+        const int t = t0 + i;
+        keys = min(128, C - t * 128);
+        half = t == nt - 1 && keys <= 0;
+        if (rt > 0 || (t < nt - 1 && keys == 128)) return true;
+        int z0 = keys, z1 = 128, z2 = 128, z3 = 128;  // rows [z0, z1) and [z2, z3) of V are empty
+        if (t == nt - 1) {
+          z0 = max(keys, 0);
+          z1 = half ? 0 : 64;
+          z2 = z1 + T;
+          z3 = z1 + 64;
+        }
+        const uint32_t vn = rbase + ring_v(i, count);
+        if (!ta_warp_wait(&sm.r_full[vn % RING], (vn / RING) & 1, abort_flag)) return false;
+        if ((r >= z0 && r < z1) || (r >= z2 && r < z3)) {
+          uint4* row = reinterpret_cast<uint4*>(sm.ring[vn % RING] + r * 128);
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const int at = (q + lane) & 7;  // neighbouring rows start in different banks
-                row[at] = row[at + TA_SUB / 16] = make_uint4(0u, 0u, 0u, 0u);
-              }
-            }
-            fence_proxy_async();
+          for (int q = 0; q < 8; ++q) {
+            const int at = (q + lane) & 7;  // neighbouring rows start in different banks
+            row[at] = row[at + TA_SUB / 16] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
-        if (narrow) {
-          // ---- at most 32 rows: S holds them four times, warp lg takes 32 of the 128 columns; P goes through shared memory
+        fence_proxy_async();
+        return true;
+      };
+      if constexpr (narrow) {
+        uint64_t nm[16], ln[16];  // reference points (negated) and sums of the 32 rows, this thread's keys
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nm[e] = ln[e] = 0ull;
+        for (int x = x0; x < jobs; x += 2) {
+          const int t = t0 + x;
+          int keys;
+          bool half;
+          ok = begin_job(x, keys, half);
+          if (!ok) break;
+          // ---- a thread has one key and all 32 rows.  The exponentials are taken against a reference point that starts at 0 and moves
+          // to the rows' maxima only if a score exceeds it by 2^40, or if none of a unit's first scores comes up to 2^-40 of it:
+          // fp32 and bf16 hold 2^+-126, so in between only the sums' exponents differ.
+          uint32_t word = ~0u;  // the rows that see this key
+          if (t == nt - 1) {
+            const int node0 = (half ? lg : lg - 2) * 32;  // keys of the tree in this warp
+            word = r < keys ? ~0u : 0u;
+            if (node0 == 0) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const uint32_t rows = __ballot_sync(0xffffffffu, (sees >> e) & 1ull);
+                if (lane == e) word = rows;
+              }
+            }
+          } else if (r >= keys) {
+            word = 0u;
+          }
           uint32_t sv[32];
-          tmem_ld32(t_s + lg * 32, sv);
-          const uint32_t word = static_cast<uint32_t>((lg & 2 ? hi : lo) >> (lg & 1) * 32);
+          tmem_ld32(t_s, sv);
           tmem_ld_wait();
           if (__any_sync(0xffffffffu, word != ~0u)) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!((word >> e) & 1u)) sv[e] = 0xff800000u;
           }
-          float mx2[2] = {-INFINITY, -INFINITY};
+          const uint64_t c2 = pair2(c, c);
+          float xs[32];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) mx2[e / 2 & 1] = max3(mx2[e / 2 & 1], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
-          sm.mx[grp][lg][lane] = static_cast<uint16_t>(__float_as_uint(fmaxf(mx2[0], mx2[1])) >> 16);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.mx_full[grp]);
-          ok = ta_warp_wait(&sm.mx_full[grp], par_mx, abort_flag);
-          par_mx ^= 1;
+          for (int e = 0; e < 16; ++e) unpair2(fma2(pair2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), c2, nm[e]), xs[2 * e], xs[2 * e + 1]);
+          float hi2[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) hi2[e / 2 & 1] = max3(hi2[e / 2 & 1], xs[e], xs[e + 1]);
+          uint32_t flag = __any_sync(0xffffffffu, fmaxf(hi2[0], hi2[1]) > 40.f) ? 1u : 0u;
+          if (x < 2) {
+            float low = INFINITY;
+            const int rows = T * a.G;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) low = e < rows ? fminf(low, xs[e]) : low;
+            flag |= __any_sync(0xffffffffu, low > -40.f) ? 2u : 0u;  // one key that is not far below the reference for any row
+          } else {
+            flag |= 2u;
+          }
+          if (lane == 0) {
+            reinterpret_cast<volatile uint8_t*>(&sm.flags[grp])[lg] = static_cast<uint8_t>(flag);
+            mbar_arrive(&sm.flag_full[grp]);
+          }
+          ok = ta_warp_wait(&sm.flag_full[grp], par_flag, abort_flag);
+          par_flag ^= 1;
           if (!ok) break;
-          float mx = -INFINITY;  // cut to bf16, the same in all four warps; only a reference point of the exponentials
+          const uint32_t flags = *reinterpret_cast<volatile uint32_t*>(&sm.flags[grp]);
+          if ((flags & 0x01010101u) || !(flags & 0x02020202u)) {
+            // move the rows' reference points to their maxima (after the first scores: only upwards)
+            float top = 0.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mx = fmaxf(mx, __uint_as_float(static_cast<uint32_t>(sm.mx[grp][k][lane]) << 16));
-          float alpha = 1.f;
-          const bool grow = (mx - m) * c > 8.f;
-          if (grow) {
-            alpha = ex2_approx((m - mx) * c);
-            m = mx;
-            l *= alpha;
-          }
-          const uint64_t c2 = pair2(c, c), mc2 = pair2(-m * c, -m * c);
-          uint64_t sum[2] = {0ull, 0ull};
-          uint32_t pk[16];
+            for (int e = 0; e < 32; ++e) {
+              const float v = warp_max(xs[e]);
+              if (lane == e) top = v;
+            }
+            sm.mx[grp][lg][lane] = top;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.mx_full[grp]);
+            ok = ta_warp_wait(&sm.mx_full[grp], par_mx, abort_flag);
+            par_mx ^= 1;
+            if (!ok) break;
+            top = fmaxf(fmaxf(sm.mx[grp][0][lane], sm.mx[grp][1][lane]), fmaxf(sm.mx[grp][2][lane], sm.mx[grp][3][lane]));
+            if (top == -INFINITY || (x >= 2 && top < 0.f)) top = 0.f;  // a row without a key so far stays where it is
+            m += top;
+            sm.wt[warp - 4][0][lane] = -top;
+            sm.wt[warp - 4][1][lane] = x < 2 ? 1.f : ex2_approx(-top);
+            __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float p0, p1;
-            unpair2(fma2(pair2(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), c2, mc2), p0, p1);
-            p0 = ex2_approx(p0);
-            p1 = ex2_approx(p1);
-            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair2(p0, p1));
-            pk[e >> 1] = pack_bf16x2(p0, p1);
-          }
-          {
-            float s0, s1;
-            unpair2(add2(sum[0], sum[1]), s0, s1);
-            l += s0 + s1;
-          }
-          uint8_t* prow = sm.p[grp] + (lg >> 1) * TA_PSUB + lane * 128;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4*>(prow + ((((lg & 1) * 4 + q) ^ (lane & 7)) << 4)) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
-          fence_proxy_async();
-          if (x >= 2 && lg == 0 && __any_sync(0xffffffffu, grow)) {  // the rows of O that count are in the first quarter
-#pragma unroll
-            for (int cc = 0; cc < 4; ++cc) {
+            for (int e = 0; e < 32; e += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(&sm.wt[warp - 4][0][e]), w = *reinterpret_cast<const float4*>(&sm.wt[warp - 4][1][e]);
+              nm[e / 2] = add2(nm[e / 2], pair2(v.x, v.y));
+              nm[e / 2 + 1] = add2(nm[e / 2 + 1], pair2(v.z, v.w));
+              ln[e / 2] = mul2(ln[e / 2], pair2(w.x, w.y));
+              ln[e / 2 + 1] = mul2(ln[e / 2 + 1], pair2(w.z, w.w));
+              xs[e] += v.x;
+              xs[e + 1] += v.y;
+              xs[e + 2] += v.z;
+              xs[e + 3] += v.w;
+            }
+            if (x >= 2) {
               uint32_t o[32];
-              tmem_ld32(t_o + grp * 128 + cc * 32, o);
+              tmem_ld32(t_o + grp * 128, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st32(t_o + grp * 128 + cc * 32, o);
+              for (int e = 0; e < 32; e += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(&sm.wt[warp - 4][1][e]);
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * w.x);
+                o[e + 1] = __float_as_uint(__uint_as_float(o[e + 1]) * w.y);
+                o[e + 2] = __float_as_uint(__uint_as_float(o[e + 2]) * w.z);
+                o[e + 3] = __float_as_uint(__uint_as_float(o[e + 3]) * w.w);
+              }
+              tmem_st32(t_o + grp * 128, o);
+              tmem_st_wait();
             }
-            tmem_st_wait();
+            __syncwarp();
           }
-        } else if (busy) {
-          uint32_t sv[4][32];
-          tmem_ld32(t_s, sv[0]);
-          tmem_ld32(t_s + 32, sv[1]);
-          if (!half) {
-            tmem_ld32(t_s + 64, sv[2]);
-            tmem_ld32(t_s + 96, sv[3]);
+          uint8_t* prow = sm.p[grp] + r * 64;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i2 = q * 4 + e;
+              const float p0 = ex2_approx(xs[2 * i2]), p1 = ex2_approx(xs[2 * i2 + 1]);
+              ln[i2] = add2(ln[i2], pair2(p0, p1));
+              pk[e] = pack_bf16x2(p0, p1);
+            }
+            *reinterpret_cast<uint4*>(prow + ((q ^ (r >> 1 & 3)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
           }
-          tmem_ld_wait();
-          const bool masked = (lo & hi) != ~0ull;
-          if (masked) {
-            const uint32_t words[4] = {static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
-                                       static_cast<uint32_t>(hi >> 32)};
+          fence_proxy_async();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full[grp]);
+        }
+        if (!ok) break;
+        // 32 sums over the warp's keys: halve the rows and the lanes that share them, until lane i has row i
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) unpair2(ln[e], v[2 * e], v[2 * e + 1]);
+#pragma unroll
+        for (int h = 16; h > 0; h >>= 1) {
+          const bool upper = lane & h;
+#pragma unroll
+          for (int e = 0; e < h; ++e) {
+            const float send = upper ? v[e] : v[e + h], keep = upper ? v[e + h] : v[e];
+            v[e] = keep + __shfl_xor_sync(0xffffffffu, send, h);
+          }
+        }
+        l = sees ? v[0] : 0.f;
+      } else {
+        for (int x = x0; x < jobs; x += 2) {
+          const int i = nrt == 2 ? x >> 1 : x, t = t0 + i;
+          int keys;
+          bool half;
+          ok = begin_job(i, keys, half);
+          if (!ok) break;
+          unsigned long long lo = ~0ull, hi = ~0ull;  // keys of this tile that the row sees
+          if (t == nt - 1) {
+            lo = half ? sees : low_bits(keys);
+            hi = half ? 0ull : sees;
+          } else if (keys < 128) {
+            lo = low_bits(keys);
+            hi = low_bits(max(keys - 64, 0));
+          }
+          if (busy) {
+            uint32_t sv[4][32];
+            tmem_ld32(t_s, sv[0]);
+            tmem_ld32(t_s + 32, sv[1]);
+            if (!half) {
+              tmem_ld32(t_s + 64, sv[2]);
+              tmem_ld32(t_s + 96, sv[3]);
+            }
+            tmem_ld_wait();
+            const bool masked = (lo & hi) != ~0ull;
+            if (masked) {
+              const uint32_t words[4] = {static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
+                                         static_cast<uint32_t>(hi >> 32)};
+#pragma unroll
+              for (int cc = 0; cc < 4; ++cc)
+                if (cc < 2 || !half) {
+#pragma unroll
+                  for (int e = 0; e < 32; ++e)
+                    if (!((words[cc] >> e) & 1u)) sv[cc][e] = 0xff800000u;
+                }
+            }
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int cc = 0; cc < 4; ++cc)
               if (cc < 2 || !half) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (!((words[cc] >> e) & 1u)) sv[cc][e] = 0xff800000u;
+                for (int e = 0; e < 32; e += 2)
+                  mx4[e / 2 & 3] = max3(mx4[e / 2 & 3], __uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1]));
               }
-          }
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int cc = 0; cc < 4; ++cc)
-            if (cc < 2 || !half) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 2)
-                mx4[e / 2 & 3] = max3(mx4[e / 2 & 3], __uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1]));
+            const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
+            float alpha = 1.f;
+            const bool grow = (mx - m) * c > 8.f;
+            if (grow) {
+              alpha = ex2_approx((m - mx) * c);
+              m = mx;
+              l *= alpha;
             }
-          const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
-          float alpha = 1.f;
-          const bool grow = (mx - m) * c > 8.f;
-          if (grow) {
-            alpha = ex2_approx((m - mx) * c);
-            m = mx;
-            l *= alpha;
-          }
-          const uint64_t c2 = pair2(c, c), mc2 = pair2(-m * c, -m * c);
-          uint64_t sum[2] = {0ull, 0ull};  // two pairs of zeros
-#pragma unroll
-          for (int cc = 0; cc < 4; ++cc) {
-            if (cc < 2 || !half) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const uint64_t x = fma2(pair2(__uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1])), c2, mc2);
-                float p0, p1;
-                unpair2(x, p0, p1);
-                p0 = ex2_approx(p0);
-                p1 = ex2_approx(p1);
-                sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair2(p0, p1));
-                pk[e >> 1] = pack_bf16x2(p0, p1);
-              }
-              tmem_st16(t_s + cc * 16, pk);
-            }
-          }
-          {
-            float s0, s1;
-            unpair2(add2(sum[0], sum[1]), s0, s1);
-            l += s0 + s1;
-          }
-          // S of this job was issued after every earlier P V of this group, so O is at rest here
-          if (x >= 2 && __any_sync(0xffffffffu, grow)) {
+            const uint64_t c2 = pair2(c, c), mc2 = pair2(-m * c, -m * c);
+            uint64_t sum[2] = {0ull, 0ull};  // two pairs of zeros
 #pragma unroll
             for (int cc = 0; cc < 4; ++cc) {
-              uint32_t o[32];
-              tmem_ld32(t_o + grp * 128 + cc * 32, o);
-              tmem_ld_wait();
+              if (cc < 2 || !half) {
+                uint32_t pk[16];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st32(t_o + grp * 128 + cc * 32, o);
+                for (int e = 0; e < 32; e += 2) {
+                  const uint64_t x = fma2(pair2(__uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1])), c2, mc2);
+                  float p0, p1;
+                  unpair2(x, p0, p1);
+                  p0 = ex2_approx(p0);
+                  p1 = ex2_approx(p1);
+                  sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair2(p0, p1));
+                  pk[e >> 1] = pack_bf16x2(p0, p1);
+                }
+                tmem_st16(t_s + cc * 16, pk);
+              }
             }
+            {
+              float s0, s1;
+              unpair2(add2(sum[0], sum[1]), s0, s1);
+              l += s0 + s1;
+            }
+            // S of this job was issued after every earlier P V of this group, so O is at rest here
+            if (x >= 2 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+              for (int cc = 0; cc < 4; ++cc) {
+                uint32_t o[32];
+                tmem_ld32(t_o + grp * 128 + cc * 32, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st32(t_o + grp * 128 + cc * 32, o);
+              }
+            }
+            tmem_st_wait();
           }
-          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full[grp]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[grp]);
+        if (!ok) break;
+        if (!sees) {
+          m = -INFINITY;
+          l = 0.f;
+        }
+        m *= c;  // base-2 scale from here on
       }
-      if (!ok) break;
 
       // ---- end of the segment: the result or a part of it.  Two row tiles: each group writes its own.  One: the group of the last
       // job joins both, the other hands over its maxima and sums and goes on with the next unit.
-      if (!sees) {
-        m = -INFINITY;
-        l = 0.f;
-      }
-      m *= c;  // base-2 scale from here on
       const int last = (jc + jobs - 1) & 1;
       const bool both = nrt == 1 && jobs > 1;
       jc += jobs;
@@ -753,8 +865,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (!ok) break;
       } else if (grp != last) {
         if (both) {
-          sm.ml[r] = l;
-          if (!narrow || lg == 0) sm.ml[128 + r] = m;
+          if (narrow) {
+            sm.ls[grp][lg][lane] = l;
+            sm.lm[grp][lane] = m;
+          } else {
+            sm.ml[r] = l;
+            sm.ml[128 + r] = m;
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.ml_full[grp]);
           late = true;
@@ -767,26 +884,28 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         continue;
       } else {
         float m_other = 0.f, l_other = 0.f;
-        if (narrow) {  // the first warp collects its three neighbours' sums
-          if (lg > 0) {
-            sm.ml[128 + r] = l;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.lx_full[grp]);
-          } else {
-            ok = ta_warp_wait(&sm.lx_full[grp], par_lx, abort_flag);
-            if (!ok) break;
-            l += sm.ml[160 + lane] + sm.ml[192 + lane] + sm.ml[224 + lane];
-          }
+        if (narrow) {
+          sm.ls[grp][lg][lane] = l;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.lx_full[grp]);
+          ok = ta_warp_wait(&sm.lx_full[grp], par_lx, abort_flag);
           par_lx ^= 1;
+          if (!ok) break;
+          l = (sm.ls[grp][0][lane] + sm.ls[grp][1][lane]) + (sm.ls[grp][2][lane] + sm.ls[grp][3][lane]);
         }
         if (both) {
           ok = ta_warp_wait(&sm.ml_full[grp ^ 1], par_ml, abort_flag);
           par_ml ^= 1;
           if (ok) ok = ta_warp_wait(&sm.o_full[grp ^ 1], par_o >> (grp ^ 1) & 1, abort_flag);
           if (!ok) break;
-          l_other = sm.ml[narrow ? lane : r];
-          if (narrow) l_other += sm.ml[32 + lane] + sm.ml[64 + lane] + sm.ml[96 + lane];
-          m_other = sm.ml[128 + (narrow ? lane : r)];
+          if (narrow) {
+            const float* o = &sm.ls[grp ^ 1][0][lane];
+            l_other = (o[0] + o[32]) + (o[64] + o[96]);
+            m_other = sm.lm[grp ^ 1][lane];
+          } else {
+            l_other = sm.ml[r];
+            m_other = sm.ml[128 + r];
+          }
           const float top = fmaxf(m, m_other);
           a0 = l != 0.f ? ex2_approx(m - top) : 0.f;
           a1 = l_other != 0.f ? ex2_approx(m_other - top) : 0.f;
@@ -800,13 +919,64 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       tc_fence_after();
       const bool whole = t0 == 0 && count == nt;
       const long long part = (static_cast<long long>(cta) * 2 + (t0 == 0 ? 1 : 0)) * a.part_rows + rt * 128 + (narrow ? lane : r);
-      const bool mine = valid && !(narrow && lg > 0);  // rows of the result in this warp
+      if constexpr (narrow) {
+        // O^T: a thread has one dimension (r) of all 32 rows; the rows' weights come from the lanes that hold them
+        const float inv = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;  // an empty row gives zeros, a NaN stays one
+        sm.wt[warp - 4][0][lane] = a0 * inv;
+        sm.wt[warp - 4][1][lane] = a1 * inv;
+        if (!whole && valid && lg == 0) a.part_ml[part] = make_float2(m, l);
+        const int to = valid ? static_cast<int>(out_at - seg_at) : -1;
+        uint32_t v[32], u[32];
+        tmem_ld32(t_o + grp * 128, v);
+        if (both) tmem_ld32(t_o + (grp ^ 1) * 128, u);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(&sm.wt[warp - 4][0][e]), z = *reinterpret_cast<const float4*>(&sm.wt[warp - 4][1][e]);
+          f[e] = w.x * __uint_as_float(v[e]);
+          f[e + 1] = w.y * __uint_as_float(v[e + 1]);
+          f[e + 2] = w.z * __uint_as_float(v[e + 2]);
+          f[e + 3] = w.w * __uint_as_float(v[e + 3]);
+          if (both) {
+            f[e] = fmaf(z.x, __uint_as_float(u[e]), f[e]);
+            f[e + 1] = fmaf(z.y, __uint_as_float(u[e + 1]), f[e + 1]);
+            f[e + 2] = fmaf(z.z, __uint_as_float(u[e + 2]), f[e + 2]);
+            f[e + 3] = fmaf(z.w, __uint_as_float(u[e + 3]), f[e + 3]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.o_free[0]);
+          mbar_arrive(&sm.o_free[1]);
+        }
+        const int rows = T * a.G;
+        if (whole) {
+          __nv_bfloat16* dst = a.out + seg_at + (r & ~1);  // two neighbouring dimensions of every second row
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            if (e >= rows) break;
+            const bool odd = lane & 1;
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? f[e] : f[e + 1], 1);
+            const int row = __shfl_sync(0xffffffffu, to, e + (lane & 1));
+            if (row >= 0) *reinterpret_cast<uint32_t*>(dst + row) = odd ? pack_bf16x2(got, f[e + 1]) : pack_bf16x2(f[e], got);
+          }
+        } else {
+          float* dst = a.part_o + (part - lane) * TA_DH + r;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (e < rows) dst[e * TA_DH] = f[e];
+        }
+        continue;
+      }
       if (whole) {  // a row that sees nothing gives zeros (below), a NaN stays one
         a0 *= 1.f / l;
         a1 *= 1.f / l;
       }
       const uint64_t w0 = pair2(a0, a0), w1 = pair2(a1, a1);
-      if (busy && !(narrow && lg > 0)) {
+      if (busy) {
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
           uint32_t v[32], u[32];
@@ -821,7 +991,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             unpair2(y, f[e], f[e + 1]);
           }
           if (whole) {
-            if (mine) {
+            if (valid) {
               uint4* dst = reinterpret_cast<uint4*>(a.out + out_at + cc * 32);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -830,7 +1000,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 dst[e] = sees ? y : make_uint4(0u, 0u, 0u, 0u);
               }
             }
-          } else if (mine) {
+          } else if (valid) {
             float4* dst = reinterpret_cast<float4*>(a.part_o + part * TA_DH + cc * 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
@@ -843,7 +1013,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         mbar_arrive(&sm.o_free[grp]);
         if (nrt == 1) mbar_arrive(&sm.o_free[grp ^ 1]);
       }
-      if (mine && !whole) a.part_ml[part] = make_float2(m, l);
+      if (valid && !whole) a.part_ml[part] = make_float2(m, l);
       __syncwarp();
     }
     if (!ok && lane == 0) atomicCAS(a.status, 0, ST_TIMEOUT_TMEM_FULL);
@@ -944,6 +1114,22 @@ static int ta_map_3d(CUtensorMap* map, const void* qkv, long long ld, int heads,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE));
 }
 
+template <bool narrow>
+static int ta_launch(const CUtensorMap& tq, const CUtensorMap& tn, const CUtensorMap& tk, const CUtensorMap& tv, const TreeArgs& a, int sms,
+                     cudaStream_t st) {
+  const auto kern = tree_attn_kernel<narrow>;
+  const int smem = sizeof(TreeSmem<narrow>);
+  static std::atomic<unsigned long long> cfg{0};
+  const cudaError_t e = opt_in_shared_memory(kern, smem, cfg);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  static const int regs = [&] {
+    cudaFuncAttributes f = {};
+    return cudaFuncGetAttributes(&f, kern) == cudaSuccess ? f.numRegs : 0;
+  }();
+  if (regs != TA_REGS) return -4;  // the register split of the groups would wait for registers that the launch did not bring
+  return static_cast<int>(launch_pdl(kern, dim3(sms), dim3(TA_THREADS), smem, st, tq, tn, tk, tv, a));
+}
+
 extern "C" int b200_tree_attn(const void* qkv, long long ld, const void* k_cache, const void* v_cache, int num_blocks, const int* table,
                               long long table_ld, int max_blocks, const int* ctx, const int* cu, const int* parents, int B, int N,
                               int max_nodes, int Hq, int Hkv, int Dh, float scale, void* out, void* scratch, int* status, void* stream) {
@@ -955,12 +1141,12 @@ extern "C" int b200_tree_attn(const void* qkv, long long ld, const void* k_cache
   if (static_cast<double>(B) * Hkv * ((max_nodes + 2 * (128 / (Hq / Hkv)) - 1) / (2 * (128 / (Hq / Hkv)))) * (max_blocks / 2 + 2) >= 2147483648.0) return -3;
   TreeArgs a;
   a.G = Hq / Hkv;
-  a.npt = 128 / a.G;
-  a.npt32 = 32 / a.G;
-  CUtensorMap tq, tq32, tn, tk, tv;
+  // the narrow kernel where every tree fits into 32 rows
+  const bool narrow = max_nodes * a.G <= 32;
+  a.npt = (narrow ? 32 : 128) / a.G;
+  CUtensorMap tq, tn, tk, tv;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * Hkv * TA_PAGE;
   int r = ta_map_3d(&tq, qkv, ld, Hq + 2 * Hkv, N, a.G, a.npt);
-  if (!r) r = ta_map_3d(&tq32, qkv, ld, Hq + 2 * Hkv, N, a.G, a.npt32 ? a.npt32 : 1);
   if (!r) r = ta_map_3d(&tn, qkv, ld, Hq + 2 * Hkv, N, 1, TA_MAX_NODES);
   if (!r) r = make_tmap_2d(&tk, k_cache, rows, TA_DH, TA_DH, TA_PAGE, 64, 2, true);
   if (!r) r = make_tmap_2d(&tv, v_cache, rows, TA_DH, TA_DH, TA_PAGE, 64, 2, true);
@@ -985,18 +1171,9 @@ extern "C" int b200_tree_attn(const void* qkv, long long ld, const void* k_cache
   a.part_o = reinterpret_cast<float*>(a.joins + sms);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<long long>(sms) * 2 * a.part_rows * TA_DH);
   a.status = status;
-  const int smem = sizeof(TreeSmem);
-  static std::atomic<unsigned long long> cfg{0};
-  cudaError_t e = opt_in_shared_memory(tree_attn_kernel, smem, cfg);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  static const int regs = [] {
-    cudaFuncAttributes f = {};
-    return cudaFuncGetAttributes(&f, tree_attn_kernel) == cudaSuccess ? f.numRegs : 0;
-  }();
-  if (regs != TA_REGS) return -4;  // the register split of the groups would wait for registers that the launch did not bring
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  e = launch_pdl(tree_attn_kernel, dim3(sms), dim3(TA_THREADS), smem, st, tq, tq32, tn, tk, tv, a);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  e = launch_pdl(tree_join_kernel, dim3(sms, (a.part_rows + 31) / 32), dim3(256), 0, st, a);
+  r = narrow ? ta_launch<true>(tq, tn, tk, tv, a, sms, st) : ta_launch<false>(tq, tn, tk, tv, a, sms, st);
+  if (r) return r;
+  const cudaError_t e = launch_pdl(tree_join_kernel, dim3(sms, (a.part_rows + 31) / 32), dim3(256), 0, st, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
