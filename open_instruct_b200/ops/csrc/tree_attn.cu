@@ -415,7 +415,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             return static_cast<int>((min(static_cast<unsigned>(row[p]), static_cast<unsigned>(a.num_blocks)) * a.Hkv + kvh) * TA_PAGE);
           };
           auto load_tile = [&](const CUtensorMap* cache, int head, int t, int y0, int y1) -> bool {
-            const int s = ring_slot((t == tree && y0 < 0) || (t != tree && y1 < 0) ? TA_TILE / 2 : TA_TILE);
+            const int s = ring_slot((y0 >= 0 ? TA_TILE / 2 : 0) + (t == tree ? a.max_nodes * TA_DH * 2 : y1 >= 0 ? TA_TILE / 2 : 0));
             if (s < 0) return false;
             uint8_t* dst = sm.ring[s];
             if (y0 >= 0) {
@@ -1147,7 +1147,7 @@ extern "C" int b200_tree_attn(const void* qkv, long long ld, const void* k_cache
   CUtensorMap tq, tn, tk, tv;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * Hkv * TA_PAGE;
   int r = ta_map_3d(&tq, qkv, ld, Hq + 2 * Hkv, N, a.G, a.npt);
-  if (!r) r = ta_map_3d(&tn, qkv, ld, Hq + 2 * Hkv, N, 1, TA_MAX_NODES);
+  if (!r) r = ta_map_3d(&tn, qkv, ld, Hq + 2 * Hkv, N, 1, max_nodes);
   if (!r) r = make_tmap_2d(&tk, k_cache, rows, TA_DH, TA_DH, TA_PAGE, 64, 2, true);
   if (!r) r = make_tmap_2d(&tv, v_cache, rows, TA_DH, TA_DH, TA_PAGE, 64, 2, true);
   if (r) return 10000 + r;
