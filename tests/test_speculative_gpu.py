@@ -262,7 +262,10 @@ def test_verification_stream_and_graph():
                 live[k].copy_(v)
         graph.replay()
         torch.cuda.synchronize()
-        assert all(torch.equal(p, q) for p, q in zip(out, want))
+        assert all(torch.equal(p, q) for p, q in zip(out[:3], want[:3]))
+        # the clone's rows start at other 16-byte offsets, so a row's sum is grouped differently: each result is within
+        # logprob_bound of the exact value, the two within twice that of each other
+        assert (out[3] - want[3]).abs().max() <= 2 * logprob_bound(32003)
 
 
 @pytest.mark.parametrize("bad", [False, True])
