@@ -10,14 +10,18 @@
 // from r: the first token whose cumulative sum exceeds u_sample[b] times the total.  So every emitted token is distributed
 // as the target's own sample, whatever was drafted.
 //
-// Two kernels.  verify_stats_kernel reads every node's logits once (that is the whole cost: 2 bytes for each logit) and leaves the
-// maximum and the sum of exponentials of every 16384-column chunk of a row.  verify_walk_kernel has a cluster of eight CTAs for
-// each sequence: all of them take the same walk (the probabilities of all nodes' tokens are gathered before it, so it runs out of
-// shared memory), then each has an eighth of the vocabulary of the last node's row for the final draw.
+// Four kernels.  verify_stats_kernel reads every node's logits once - that is the cost of the whole: 2 bytes for each logit, at
+// 16 exponentials a cycle and SM about 0.7 of the time that HBM needs for them - and leaves the maximum and the sum of
+// exponentials of every 2048-column piece of a row.  verify_walk_kernel gathers the probabilities of all nodes' tokens and walks
+// every tree out of shared memory (with draft probabilities a cluster of eight CTAs, which sums the residuals between siblings).
+// verify_sums_kernel sums what is left in every 8192-column chunk of the row in which a walk ended, verify_pick_kernel finds the
+// token in the chunk where the sum passes the coin's share.
 //
-// A sum that decides a token is held in fp64, its terms exp(z / temperature - max) in fp32: a vocabulary of 10^5 tokens has
-// bins of 10^-5 and less, and fp32 partial sums would move their borders by a share of that.  The statistics' exponentials
-// come from the special-function unit (2^-22 of themselves, like the log-probabilities that leave through fp32).
+// A sum that decides a token needs more than fp32, though its terms exp(z / temperature - max) are fp32: a vocabulary of 10^5
+// tokens has bins of 10^-5 and less, and fp32 partial sums would move their borders by a share of that.  Every thread adds up
+// its terms as an unevaluated sum of two fp32 numbers (about 48 bits, six additions a term), threads and chunks are joined
+// in fp64.  The statistics' exponentials come from the special-function unit (2^-22 of themselves, like the log-probabilities that
+// leave through fp32).
 #include "common.cuh"
 
 #include <cooperative_groups.h>
@@ -27,11 +31,14 @@ namespace b200 {
 constexpr int SP_PAGE = 64;
 constexpr int SP_DH = 128;
 constexpr int SP_MAX_NODES = 64;
-constexpr int SP_LOADS = 8;                               // 16-byte loads of a thread of the statistics kernel
+constexpr int SP_LOADS = 8;                          // 16-byte loads of a lane for one piece of a row
+constexpr int SP_PIECE = SP_LOADS * 32;              // granules of a piece (2048 logits), the work of one warp at a time
 constexpr int SP_STAT_THREADS = 256;
-constexpr int SP_CHUNK = SP_LOADS * SP_STAT_THREADS;      // 16-byte granules of a chunk (16384 logits)
+constexpr int SP_STAT_CTAS = 2;                      // resident on an SM
+constexpr int SP_SUM_THREADS = 256;
+constexpr int SP_CHUNK = 1024;                       // granules of a chunk of the last draw (8192 logits), threads of the kernel that picks in it
 constexpr int SP_CLUSTER = 8;
-constexpr int SP_THREADS = 512;
+constexpr int SP_THREADS = 512;                      // of a walking CTA with draft probabilities; 256 without
 constexpr float SP_LOG2E = 1.4426950408889634f;
 
 // A row of logits as aligned 16-byte granules of eight: rows of an odd vocabulary start anywhere, so a row begins `skip` elements
@@ -47,7 +54,10 @@ struct LogitRow {
   }
   __device__ __forceinline__ uint4 load(int g) const {
     if (g >= count) return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
-    uint4 v = __ldg(granules + g);
+    return __ldg(granules + g);
+  }
+  // the first and the last granule of the row, cut to it
+  __device__ __forceinline__ void trim(uint4& v, int g) const {
     if (g == 0 || g == count - 1) {
       uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -57,8 +67,18 @@ struct LogitRow {
       }
       v = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    return v;
   }
+};
+
+// What verify_walk_kernel leaves for the last draw of a sequence.
+struct WalkEnd {
+  double total;              // sum of exp(z / temperature - top) over the row
+  float2 inv_total;          // its reciprocal, as two fp32 numbers
+  float2 rz[SP_MAX_NODES];   // reciprocals of the residuals' sums (draft probabilities given)
+  int gone[SP_MAX_NODES];    // rejected tokens (point-mass drafts)
+  float top;                 // largest z / temperature of the row
+  int node;                  // batch row in which the walk ended, -1: nothing is left to draw
+  int k, nz, ngone, less;    // tokens emitted so far; residuals, rejected tokens; whether one more rejection has to be taken off
 };
 
 struct VerifyArgs {
@@ -70,7 +90,7 @@ struct VerifyArgs {
   const long long* tokens;
   const int* parents;
   const int* cu;
-  int B, N, max_nodes, chunks;
+  int B, N, max_nodes, pieces, chunks;
   const float* temperature;
   const float* u_accept;
   const float* u_sample;
@@ -78,83 +98,158 @@ struct VerifyArgs {
   long long* out_tokens;
   int* path;
   float* logprobs;
-  float4* part;  // [N][chunks]: maximum, sum of exponentials relative to it, its first column (temperature 0)
+  float2* part;   // [N][pieces]: maximum, sum of exponentials relative to it
+  int* first;     // [N][pieces]: its first column (rows at temperature 0 only)
+  WalkEnd* end;   // [B]
+  double* sums;   // [B][chunks]: what is left in a chunk
 };
 
-// One CTA per (sequence, node, chunk).
-__global__ void __launch_bounds__(SP_STAT_THREADS, 4) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
-  __shared__ float smax[SP_STAT_THREADS / 32], ssum[SP_STAT_THREADS / 32];
-  __shared__ int sidx[SP_STAT_THREADS / 32];
+// A number as the unevaluated sum of two fp32 numbers, |lo| <= half a step of hi; about 48 bits.
+struct Two {
+  float hi, lo;
+};
+__device__ __forceinline__ Two two_sum(float x, float y) {  // exact (Knuth)
+  const float s = __fadd_rn(x, y), t = __fsub_rn(s, x);
+  return {s, __fadd_rn(__fsub_rn(x, __fsub_rn(s, t)), __fsub_rn(y, t))};
+}
+__device__ __forceinline__ Two two_norm(float x, float y) {  // |x| >= |y|
+  const float s = __fadd_rn(x, y);
+  return {s, __fsub_rn(y, __fsub_rn(s, x))};
+}
+__device__ __forceinline__ Two two_mul(const Two& x, const Two& y) {
+  const float p = __fmul_rn(x.hi, y.hi);
+  return two_norm(p, __fadd_rn(__fmaf_rn(x.hi, y.hi, -p), __fmaf_rn(x.hi, y.lo, __fmul_rn(x.lo, y.hi))));
+}
+__device__ __forceinline__ Two two_minus(const Two& x, float y) {
+  const Two s = two_sum(x.hi, -y);
+  return two_norm(s.hi, __fadd_rn(s.lo, x.lo));
+}
+__device__ __forceinline__ void two_add(Two& sum, const Two& x) {  // the running sum: hi exact, what it drops goes to lo
+  const Two s = two_sum(sum.hi, x.hi);
+  sum.hi = s.hi;
+  sum.lo = __fadd_rn(sum.lo, __fadd_rn(s.lo, x.lo));
+}
+__device__ __forceinline__ Two two_of(double x) {
+  const float hi = static_cast<float>(x);
+  return {hi, static_cast<float>(x - static_cast<double>(hi))};
+}
+__device__ __forceinline__ double two_double(const Two& x) { return static_cast<double>(x.hi) + static_cast<double>(x.lo); }
+
+// log of a positive sum: the exponent's share in fp64, the logarithm of the mantissa in fp32 (off by less than 2^-23)
+__device__ __forceinline__ double sp_log(double x) {
+  const float f = static_cast<float>(x);
+  const int bits = __float_as_int(f), e = (bits >> 23) - 127;
+  const float m = __int_as_float((bits & 0x7fffff) | 0x3f800000);  // 1 .. 2
+  return static_cast<double>(e) * 0.69314718055994530942 + (static_cast<double>(logf(m)) + (x - static_cast<double>(f)) / static_cast<double>(f));
+}
+
+__device__ __forceinline__ float sp_weight(float z, float temp, float top) { return expf(__fsub_rn(temp == 1.f ? z : __fdiv_rn(z, temp), top)); }
+__device__ __forceinline__ float sp_logit(const uint4& v, int e) {
+  const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
+  return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+}
+__device__ __forceinline__ void sp_span(const VerifyArgs& a, int b, int& n0, int& T) {
+  n0 = min(max(a.cu[b], 0), a.N);
+  T = min(min(max(a.cu[b + 1] - n0, 0), a.max_nodes), a.N - n0);
+}
+
+// Every warp has a run of pieces of its own (rows in order) and asks for the next piece before it works on this one.
+__global__ void __launch_bounds__(SP_STAT_THREADS, SP_STAT_CTAS) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
   griddep_launch_dependents();
   griddep_wait();
-  const int c = blockIdx.x % a.chunks, bj = blockIdx.x / a.chunks, j = bj % a.max_nodes, b = bj / a.max_nodes;
-  const int n0 = min(max(a.cu[b], 0), a.N), T = min(min(max(a.cu[b + 1] - n0, 0), a.max_nodes), a.N - n0);
-  const float temp = a.temperature[b];
-  if (j >= T) return;
-  const bool greedy = !(temp > 0.f);
-  const float k = SP_LOG2E / (greedy ? 1.f : temp);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const LogitRow row(a.logits + (n0 + j) * a.ld, a.V);
-  const int g0 = c * SP_CHUNK + tid;
-  uint4 v[SP_LOADS];
-#pragma unroll
-  for (int i = 0; i < SP_LOADS; ++i) v[i] = row.load(g0 + i * SP_STAT_THREADS);
-  __nv_bfloat162 top2 = *reinterpret_cast<const __nv_bfloat162*>(&v[0].x);
-#pragma unroll
-  for (int i = 0; i < SP_LOADS; ++i) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v[i]);
-    top2 = __hmax2(top2, __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  const int lane = threadIdx.x & 31;
+  const long long warps = static_cast<long long>(gridDim.x) * (SP_STAT_THREADS / 32);
+  const long long me = static_cast<long long>(blockIdx.x) * (SP_STAT_THREADS / 32) + (threadIdx.x >> 5);
+  const long long items = static_cast<long long>(a.N) * a.pieces;
+  long long item = items * me / warps;
+  const long long end = items * (me + 1) / warps;
+  if (item >= end) return;
+  int n = static_cast<int>(item / a.pieces), piece = static_cast<int>(item % a.pieces);
+  // the sequence of the first row: the last b with cu[b] <= n, 32 candidates at a time
+  int lo = 0, hi = a.B;  // cu[lo] <= n (or lo = 0), cu[hi] > n (or hi = B)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at < hi && (lane == 0 || a.cu[at] <= n));
+    const int k = 31 - __clz(static_cast<int>(below));
+    hi = min(hi, lo + (k + 1) * step);
+    lo += k * step;
   }
-  float top = fmaxf(__low2float(top2), __high2float(top2));
+  int b = lo, next_start = a.cu[b + 1];
+  auto settle = [&] {  // the sequence of row n; rows of no sequence take any temperature, nobody reads them
+    while (n >= next_start && b + 1 < a.B) next_start = a.cu[++b + 1];
+    return a.temperature[b];
+  };
+  float temp = settle();
+  LogitRow row(a.logits + n * a.ld, a.V);
+  uint4 v[SP_LOADS], w[SP_LOADS];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.f : top;  // a warp without a finite logit sums to zero
-  float s4[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < SP_LOADS; ++i) v[i] = row.load(piece * SP_PIECE + i * 32 + lane);
+  while (true) {
+    const int n_now = n, piece_now = piece;
+    const LogitRow row_now = row;
+    const float temp_now = temp;
+    const bool more = ++item < end;
+    if (more) {
+      if (++piece == a.pieces) {
+        piece = 0;
+        ++n;
+        row = LogitRow(a.logits + n * a.ld, a.V);
+      }
 #pragma unroll
-  for (int i = 0; i < SP_LOADS; ++i) {
-    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s4[e] += ex2_approx((__uint_as_float(w[e] << 16) - base) * k);
-      s4[e] += ex2_approx((__uint_as_float(w[e] & 0xffff0000u) - base) * k);
+      for (int i = 0; i < SP_LOADS; ++i) w[i] = row.load(piece * SP_PIECE + i * 32 + lane);
+      if (piece == 0) temp = settle();
     }
-  }
-  float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    const int g0 = piece_now * SP_PIECE + lane;
+    if (piece_now == 0 || (piece_now + 1) * SP_PIECE >= row_now.count) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) {
-    smax[warp] = top;
-    ssum[warp] = sum;
-  }
-  __syncthreads();
-  float m = smax[0];
+      for (int i = 0; i < SP_LOADS; ++i)
+        if (g0 + i * 32 < row_now.count) row_now.trim(v[i], g0 + i * 32);
+    }
+    const bool greedy = !(temp_now > 0.f);
+    const float k = SP_LOG2E / (greedy ? 1.f : temp_now);
+    __nv_bfloat162 top2 = *reinterpret_cast<const __nv_bfloat162*>(&v[0].x);
 #pragma unroll
-  for (int w = 1; w < SP_STAT_THREADS / 32; ++w) m = fmaxf(m, smax[w]);
-  int first = 0x7fffffff;
-  if (greedy) {
+    for (int i = 0; i < SP_LOADS; ++i) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v[i]);
+      top2 = __hmax2(top2, __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    }
+    float top = fmaxf(__low2float(top2), __high2float(top2));
 #pragma unroll
-    for (int i = SP_LOADS - 1; i >= 0; --i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.f : top;  // a piece without a finite logit sums to zero
+    const uint64_t minus = pair2(-base, -base), scale = pair2(k, k);
+    uint64_t s2[2] = {0ull, 0ull};
 #pragma unroll
-      for (int e = 7; e >= 0; --e) {
-        const float z = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-        if (z == m) first = (g0 + i * SP_STAT_THREADS) * 8 - row.skip + e;
+    for (int i = 0; i < SP_LOADS; ++i) {
+      const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float p0, p1;
+        unpair2(mul2(add2(pair2(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u)), minus), scale), p0, p1);
+        s2[e & 1] = add2(s2[e & 1], pair2(ex2_approx(p0), ex2_approx(p1)));
       }
     }
+    float s0, s1;
+    unpair2(add2(s2[0], s2[1]), s0, s1);
+    float sum = s0 + s1;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-    if (lane == 0) sidx[warp] = first;
-    __syncthreads();
-    first = sidx[0];
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const long long at = static_cast<long long>(n_now) * a.pieces + piece_now;
+    if (greedy) {
+      int first = 0x7fffffff;
 #pragma unroll
-    for (int w = 1; w < SP_STAT_THREADS / 32; ++w) first = min(first, sidx[w]);
-  }
-  if (tid == 0) {
-    float s = 0.f;
+      for (int i = SP_LOADS - 1; i >= 0; --i)
 #pragma unroll
-    for (int w = 0; w < SP_STAT_THREADS / 32; ++w)
-      if (ssum[w] != 0.f) s += ssum[w] * ex2_approx((smax[w] - m) * k);
-    a.part[static_cast<long long>(n0 + j) * a.chunks + c] = make_float4(m, s, __int_as_float(first), 0.f);
+        for (int e = 7; e >= 0; --e)
+          if (sp_logit(v[i], e) == top) first = (g0 + i * 32) * 8 - row_now.skip + e;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      if (lane == 0) a.first[at] = first;
+    }
+    if (lane == 0) a.part[at] = make_float2(top, sum);
+    if (!more) break;
+#pragma unroll
+    for (int i = 0; i < SP_LOADS; ++i) v[i] = w[i];
   }
 }
 
@@ -162,47 +257,61 @@ struct WalkSmem {
   double total[SP_MAX_NODES];          // sum of exp(z / temperature - top) over a node's row
   double p[SP_MAX_NODES];              // probability of a node's token in its parent's row
   double q[SP_MAX_NODES];              // draft probability of the same
-  double rz[SP_MAX_NODES];             // reciprocals of the residuals' sums so far (draft probabilities given)
+  float2 rz[SP_MAX_NODES];             // reciprocals of the residuals' sums so far (draft probabilities given), as two fp32 numbers
   double warp_sum[SP_THREADS / 32];
   double cta_sum[2][SP_CLUSTER];       // partial sums of the cluster's CTAs, two passes in turn
-  int cta_last[2][SP_CLUSTER];
   float top[SP_MAX_NODES];             // largest z / temperature of a node's row
   float u[SP_MAX_NODES];
   int best[SP_MAX_NODES];
   int parent[SP_MAX_NODES];
   int token[SP_MAX_NODES];             // -1: not in the vocabulary
   int gone[SP_MAX_NODES];              // rejected tokens of the current node (point-mass drafts)
-  int warp_last[SP_THREADS / 32];
   int ngone, nz, cur, k, next, step, pending;
   int accepted[SP_MAX_NODES];          // positions of the accepted nodes
 };
 
-__global__ void __cluster_dims__(SP_CLUSTER, 1, 1) __launch_bounds__(SP_THREADS) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
+// What is left of a token's probability after nz residuals, and one more if `less`.
+__device__ __forceinline__ Two sp_residual(Two p, float q, const float2* rz, int nz, bool less) {
+  for (int j = 0; j < nz; ++j) {
+    p = two_minus(p, q);
+    p = p.hi > 0.f ? two_mul(p, Two{rz[j].x, rz[j].y}) : Two{0.f, 0.f};
+  }
+  if (less) {
+    p = two_minus(p, q);
+    if (!(p.hi > 0.f)) p = Two{0.f, 0.f};
+  }
+  return p;
+}
+
+// One CTA for a sequence, with draft probabilities a cluster of eight whose CTAs all take the same walk.
+template <bool DRAFT>
+__device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
   namespace cg = cooperative_groups;
-  __shared__ WalkSmem sm;
-  cg::cluster_group cluster = cg::this_cluster();
   griddep_launch_dependents();
   griddep_wait();
-  const int b = blockIdx.x / SP_CLUSTER, rank = blockIdx.x % SP_CLUSTER;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n0 = min(max(a.cu[b], 0), a.N), T = min(min(max(a.cu[b + 1] - n0, 0), a.max_nodes), a.N - n0);
+  const int b = DRAFT ? blockIdx.x / SP_CLUSTER : blockIdx.x, rank = DRAFT ? blockIdx.x % SP_CLUSTER : 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+  int n0, T;
+  sp_span(a, b, n0, T);
   const float t_in = a.temperature[b];
   const bool greedy = !(t_in > 0.f);
   const float temp = greedy ? 1.f : t_in, k2 = SP_LOG2E / temp;
   const long long o0 = static_cast<long long>(b) * a.max_nodes;
   if (T == 0) {
     if (rank == 0) {
-      for (int i = tid; i < a.max_nodes; i += SP_THREADS) {
+      for (int i = tid; i < a.max_nodes; i += threads) {
         a.out_tokens[o0 + i] = -1;
         a.path[o0 + i] = -1;
         a.logprobs[o0 + i] = 0.f;
       }
-      if (tid == 0) a.count[b] = 0;
+      if (tid == 0) {
+        a.count[b] = 0;
+        a.end[b].node = -1;
+      }
     }
     return;
   }
-
-  if (!greedy) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA runs: its shared memory may be written to
+  if (DRAFT && !greedy) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA runs: its shared memory may be written to
 
   // ---- every node's row statistics and the probability of every node's token, whether the walk will need it or not
   if (tid < T) {
@@ -211,39 +320,42 @@ __global__ void __cluster_dims__(SP_CLUSTER, 1, 1) __launch_bounds__(SP_THREADS)
     sm.token[tid] = x >= 0 && x < a.V ? static_cast<int>(x) : -1;
     sm.u[tid] = a.u_accept[n0 + tid];
   }
-  for (int j = warp; j < T; j += SP_THREADS / 32) {
-    const float4* part = a.part + static_cast<long long>(n0 + j) * a.chunks;
-    float m = -INFINITY;
-    for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, part[c].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    double s = 0.0;
-    int first = 0x7fffffff;
-    for (int c = lane; c < a.chunks; c += 32) {
-      const float4 f = part[c];
-      if (f.y != 0.f) s += static_cast<double>(f.y) * static_cast<double>(ex2_approx((f.x - m) * k2));
-      if (f.x == m) first = min(first, __float_as_int(f.z));
+  for (int j = warp; j < T; j += threads / 32) {
+    const long long at = static_cast<long long>(n0 + j) * a.pieces;
+    float m = -INFINITY, s = 0.f;  // this lane's pieces, relative to their maximum
+    for (int c = lane; c < a.pieces; c += 32) {
+      const float2 f = a.part[at + c];
+      const float to = fmaxf(m, f.x);
+      if (to > -INFINITY) s = s * ex2_approx((m - to) * k2) + f.y * ex2_approx((f.x - to) * k2);
+      m = to;
     }
+    float all = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+    for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+    double d = s != 0.f ? static_cast<double>(s) * static_cast<double>(ex2_approx((m - all) * k2)) : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    int first = 0x7fffffff;
+    if (greedy) {
+      for (int c = lane; c < a.pieces; c += 32)
+        if (a.part[at + c].x == all) first = min(first, a.first[at + c]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
     }
     if (lane == 0) {
-      sm.top[j] = __fdiv_rn(m, temp);
-      sm.total[j] = s;
+      sm.top[j] = __fdiv_rn(all, temp);
+      sm.total[j] = d;
       sm.best[j] = first >= 0 && first < a.V ? first : 0;
     }
   }
   __syncthreads();
-  auto weight = [&](float z, float top) { return expf(__fsub_rn(temp == 1.f ? z : __fdiv_rn(z, temp), top)); };
   if (tid > 0 && tid < T) {
     const int up = sm.parent[tid], x = sm.token[tid];
     double p = 0.0, q = 0.0;
     if (up >= 0 && up < tid && x >= 0) {
       p = greedy ? (x == sm.best[up] ? 1.0 : 0.0)
-                 : static_cast<double>(weight(__bfloat162float(a.logits[(n0 + up) * a.ld + x]), sm.top[up])) / sm.total[up];
-      q = a.draft ? static_cast<double>(a.draft[(n0 + up) * a.draft_ld + x]) : 1.0;
+                 : static_cast<double>(sp_weight(__bfloat162float(a.logits[(n0 + up) * a.ld + x]), temp, sm.top[up])) / sm.total[up];
+      q = DRAFT ? static_cast<double>(a.draft[(n0 + up) * a.draft_ld + x]) : 1.0;
     }
     sm.p[tid] = p;
     sm.q[tid] = q;
@@ -251,95 +363,42 @@ __global__ void __cluster_dims__(SP_CLUSTER, 1, 1) __launch_bounds__(SP_THREADS)
   if (tid == 0) sm.cur = sm.k = sm.ngone = sm.nz = sm.pending = 0, sm.next = 1;
   __syncthreads();
 
-  // Sum over the vocabulary of what is left at the current node: with draft probabilities the residual after sm.nz
-  // rejections, less q once more if `less`; without them the weights of the tokens that are not gone.  Returns the cluster's sum;
-  // a thread's own share (consecutive tokens) in `mine`, the sum of everything before it in `before`, its last token with
-  // weight and the cluster's last one.
-  const double* rz = sm.rz;
   int pass = 0;
-  auto left_of = [&](double w, double inv_total, float q, int nz, bool less) {
-    double r = w * inv_total;
-    for (int j = 0; j < nz; ++j) r = fmax(r - static_cast<double>(q), 0.0) * rz[j];
-    return less ? fmax(r - static_cast<double>(q), 0.0) : r;
-  };
-  const int per = ((a.V + 14) / 8 + SP_CLUSTER * SP_THREADS - 1) / (SP_CLUSTER * SP_THREADS);  // granules of a thread
-  const int g0 = (rank * SP_THREADS + tid) * per;
-  auto visit = [&](bool less, auto&& f) {  // f(token, what is left of it) over this thread's tokens in their order, until it says so
-    const int node = sm.cur, nz = sm.nz, ngone = sm.ngone;
+  // the sum of max(r - q, 0) over the vocabulary at the current node, the same in every CTA of the cluster
+  auto residual_sum = [&] {
+    const int node = sm.cur, nz = sm.nz;
     const LogitRow row(a.logits + (n0 + node) * a.ld, a.V);
-    const float* q = a.draft ? a.draft + (n0 + node) * a.draft_ld : nullptr;
+    const float* q = a.draft + (n0 + node) * a.draft_ld;
     const float top = sm.top[node];
-    const double inv = 1.0 / sm.total[node];
-    for (int g = g0; g < g0 + per && g < row.count; ++g) {
+    const Two inv = two_of(1.0 / sm.total[node]);
+    Two part = {0.f, 0.f};
+    for (int g = rank * threads + tid; g < row.count; g += SP_CLUSTER * threads) {
       const uint4 v = row.load(g);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
       const int e0 = g * 8 - row.skip;
-      uint32_t drop = 0;
-      for (int j = 0; j < ngone; ++j) {
-        const int d = sm.gone[j] - e0;
-        if (d >= 0 && d < 8) drop |= 1u << d;
-      }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (e0 + e < 0 || e0 + e >= a.V) continue;
-        const float z = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-        const double x = static_cast<double>(weight(z, top));
-        const double r = q ? left_of(x, inv, __ldg(q + e0 + e), nz, less) : (drop >> e & 1u) ? 0.0 : x;
-        if (!f(e0 + e, r)) return;
-      }
+      for (int e = 0; e < 8; ++e)
+        if (e0 + e >= 0 && e0 + e < a.V)
+          two_add(part, sp_residual(two_mul(inv, Two{sp_weight(sp_logit(v, e), temp, top), 0.f}), __ldg(q + e0 + e), sm.rz, nz, true));
     }
-  };
-  auto cluster_sum = [&](bool less, double& mine, double& before, int& last) {
-    mine = 0.0;
-    int my_last = -1;
-    visit(less, [&](int e, double r) {
-      mine += r;
-      if (r > 0.0) my_last = e;
-      return true;
-    });
-    double incl = mine;
+    double mine = two_double(part);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) my_last = max(my_last, __shfl_xor_sync(0xffffffffu, my_last, o));
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sm.warp_sum[warp] = mine;
     __syncthreads();
-    if (lane == 31) {
-      sm.warp_sum[warp] = incl;
-      sm.warp_last[warp] = my_last;
-    }
-    __syncthreads();
-    double below = 0.0, all = 0.0;
-    int cta_last = -1;
-#pragma unroll
-    for (int w = 0; w < SP_THREADS / 32; ++w) {
-      if (w < warp) below += sm.warp_sum[w];
-      all += sm.warp_sum[w];
-      cta_last = max(cta_last, sm.warp_last[w]);
-    }
+    double all = 0.0;
+    for (int w = 0; w < threads / 32; ++w) all += sm.warp_sum[w];
+    cg::cluster_group cluster = cg::this_cluster();
     if (pass == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (tid < SP_CLUSTER) {
-      WalkSmem* other = cluster.map_shared_rank(&sm, tid);
-      other->cta_sum[pass & 1][rank] = all;
-      other->cta_last[pass & 1][rank] = cta_last;
-    }
+    if (tid < SP_CLUSTER) cluster.map_shared_rank(&sm, tid)->cta_sum[pass & 1][rank] = all;
     cluster.sync();
-    double lower = 0.0, sum = 0.0;
-    last = -1;
+    double sum = 0.0;
 #pragma unroll
-    for (int c = 0; c < SP_CLUSTER; ++c) {
-      if (c < rank) lower += sm.cta_sum[pass & 1][c];
-      sum += sm.cta_sum[pass & 1][c];
-      last = max(last, sm.cta_last[pass & 1][c]);
-    }
-    before = lower + below + (incl - mine);
+    for (int c = 0; c < SP_CLUSTER; ++c) sum += sm.cta_sum[pass & 1][c];
     ++pass;
     return sum;
   };
 
-  // ---- the walk: one warp, until the tokens run out or a residual has to be summed
+  // ---- the walk: one warp, until the nodes run out or a residual has to be summed
   while (true) {
     if (warp == 0) {
       int cur = sm.cur, k = sm.k, ngone = sm.ngone, next = sm.next, pending = sm.pending;
@@ -362,13 +421,13 @@ __global__ void __cluster_dims__(SP_CLUSTER, 1, 1) __launch_bounds__(SP_THREADS)
         }
         const int x = sm.token[j];
         double r = sm.p[j];
-        if (a.draft) {
-          for (int i = 0; i < sm.nz; ++i) r = fmax(r - sm.q[j], 0.0) * rz[i];
+        if (DRAFT) {
+          r = two_double(sp_residual(two_of(r), static_cast<float>(sm.q[j]), sm.rz, sm.nz, false));
         } else {
           for (int i = 0; i < ngone; ++i)
             if (sm.gone[i] == x) r = 0.0;
         }
-        const double need = static_cast<double>(sm.u[j]) * (a.draft ? sm.q[j] : rest);
+        const double need = static_cast<double>(sm.u[j]) * (DRAFT ? sm.q[j] : rest);
         next = j + 1;
         __syncwarp();
         if (x >= 0 && need < r) {
@@ -380,7 +439,7 @@ __global__ void __cluster_dims__(SP_CLUSTER, 1, 1) __launch_bounds__(SP_THREADS)
           cur = j;
           ngone = 0;
           rest = 1.0;
-        } else if (a.draft) {
+        } else if (DRAFT) {
           pending = 1;
         } else if (x >= 0 && r > 0.0) {
           if (lane == 0) sm.gone[ngone] = x;
@@ -399,63 +458,256 @@ __global__ void __cluster_dims__(SP_CLUSTER, 1, 1) __launch_bounds__(SP_THREADS)
       }
     }
     __syncthreads();
-    if (!sm.step) break;
-    double mine, before;
-    int last;
-    const double sum = greedy ? (sm.nz == 0 ? 1.0 : 0.0) : cluster_sum(true, mine, before, last);
+    if (!DRAFT || !sm.step) break;
+    // at temperature 0 all mass is on one token and stays there, whatever is taken off
+    const double sum = greedy ? 0.0 : residual_sum();
     __syncthreads();
     if (tid == 0) {
-      if (!greedy && sum > 0.0) sm.rz[sm.nz++] = 1.0 / sum;
+      if (sum > 0.0) {  // else nothing is left: the residual stays what it was
+        const Two r = two_of(1.0 / sum);
+        sm.rz[sm.nz++] = make_float2(r.hi, r.lo);
+      }
       sm.pending = 0;
     }
     __syncthreads();
   }
+  if (DRAFT && !greedy && pass == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
+  if (rank != 0) return;
   const int node = sm.cur, k = sm.k;
   auto logprob = [&](int at, int x) {
     const float z = __bfloat162float(a.logits[(n0 + at) * a.ld + x]);
-    return static_cast<float>(static_cast<double>(__fsub_rn(__fdiv_rn(z, temp), sm.top[at])) - log(sm.total[at]));
+    return static_cast<float>(static_cast<double>(__fsub_rn(__fdiv_rn(z, temp), sm.top[at])) - sp_log(sm.total[at]));
   };
-  auto finish = [&](int x) {
-    a.out_tokens[o0 + k] = x;
-    a.logprobs[o0 + k] = logprob(node, x);
-  };
-  if (rank == 0) {
-    for (int i = tid; i < a.max_nodes; i += SP_THREADS) {
-      const int j = i < k ? sm.accepted[i] : 0;
-      if (i != k) {
-        a.out_tokens[o0 + i] = i < k ? sm.token[j] : -1;
-        a.logprobs[o0 + i] = i < k ? logprob(sm.parent[j], sm.token[j]) : 0.f;
-      }
-      a.path[o0 + i] = i == 0 ? n0 : i <= k ? n0 + sm.accepted[i - 1] : -1;
+  for (int i = tid; i < a.max_nodes; i += threads) {
+    const bool last = greedy && i == k;  // an accepted draft, or at temperature 0 the last token
+    const int j = i < k ? sm.accepted[i] : 0, at = last ? node : sm.parent[j], x = last ? sm.best[node] : sm.token[j];
+    a.out_tokens[o0 + i] = i < k || last ? x : -1;
+    a.logprobs[o0 + i] = i < k || last ? logprob(at, x) : 0.f;
+    a.path[o0 + i] = i == 0 ? n0 : i <= k ? n0 + sm.accepted[i - 1] : -1;
+  }
+  WalkEnd& e = a.end[b];
+  if (tid == 0) {
+    a.count[b] = k + 1;
+    e.node = greedy ? -1 : n0 + node;
+    e.k = k;
+    e.nz = sm.nz;
+    e.ngone = sm.ngone;
+    e.less = sm.pending;
+    e.top = sm.top[node];
+    e.total = sm.total[node];
+    const Two inv = two_of(1.0 / sm.total[node]);
+    e.inv_total = make_float2(inv.hi, inv.lo);
+  }
+  if (tid < (DRAFT ? sm.nz : sm.ngone)) {
+    if (DRAFT) e.rz[tid] = sm.rz[tid];
+    else e.gone[tid] = sm.gone[tid];
+  }
+}
+
+__global__ void __launch_bounds__(SP_THREADS / 2) verify_walk_kernel(const __grid_constant__ VerifyArgs a) {
+  __shared__ WalkSmem sm;
+  verify_walk<false>(a, sm);
+}
+__global__ void __cluster_dims__(SP_CLUSTER, 1, 1) __launch_bounds__(SP_THREADS) verify_walk_draft_kernel(const __grid_constant__ VerifyArgs a) {
+  __shared__ WalkSmem sm;
+  verify_walk<true>(a, sm);
+}
+
+// What is left of the tokens of the row in which a walk ended: weights (point-mass drafts) or probabilities.
+template <bool DRAFT>
+struct LastRow {
+  LogitRow row;
+  const float* q;
+  const WalkEnd* end;
+  float temp, top;
+  Two inv;
+  int nz, ngone;
+  bool q4;  // granules of q are 16-byte aligned
+  __device__ __forceinline__ LastRow(const VerifyArgs& a, const WalkEnd& e, float temperature)
+      : row(a.logits + e.node * a.ld, a.V), q(DRAFT ? a.draft + e.node * a.draft_ld : nullptr), end(&e), temp(temperature), top(e.top),
+        inv{e.inv_total.x, e.inv_total.y}, nz(e.nz), ngone(e.ngone) {
+    q4 = DRAFT && ((reinterpret_cast<uintptr_t>(q) - 4 * row.skip) & 15) == 0;
+  }
+  // f(k, what is left of it) for the tokens of granule g that have anything left, in their order
+  template <typename F>
+  __device__ __forceinline__ void left(const uint4& v, int g, bool less, F&& f) const {
+    const int e0 = g * 8 - row.skip;
+    uint32_t drop = 0;  // outside of the row, or rejected
+    if (g == 0 || g >= row.count - 1) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (e0 + k < 0 || e0 + k >= row.V) drop |= 1u << k;
     }
-    if (tid == 0) a.count[b] = k + 1;
+    if (!DRAFT)
+      for (int j = 0; j < ngone; ++j) {
+        const int d = end->gone[j] - e0;
+        if (d >= 0 && d < 8) drop |= 1u << d;
+      }
+    float qs[8];
+    if (DRAFT) {
+      if (q4 && !drop) {
+        const float4 lo = __ldg(reinterpret_cast<const float4*>(q + e0)), hi = __ldg(reinterpret_cast<const float4*>(q + e0) + 1);
+        qs[0] = lo.x, qs[1] = lo.y, qs[2] = lo.z, qs[3] = lo.w, qs[4] = hi.x, qs[5] = hi.y, qs[6] = hi.z, qs[7] = hi.w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) qs[k] = (drop >> k & 1u) ? 0.f : __ldg(q + e0 + k);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float w = sp_weight(sp_logit(v, k), temp, top);
+      Two r = {(drop >> k & 1u) ? 0.f : w, 0.f};
+      if (DRAFT) {
+        if (nz == 0) {  // the common case without the loop: w * inv - q, hi and lo
+          const float p = __fmul_rn(r.hi, inv.hi), lo = __fmaf_rn(r.hi, inv.lo, __fmaf_rn(r.hi, inv.hi, -p));
+          const Two d = two_sum(p, less ? -qs[k] : 0.f);
+          r = two_norm(d.hi, __fadd_rn(d.lo, lo));
+        } else {
+          r = sp_residual(two_mul(inv, r), qs[k], end->rz, nz, less);
+        }
+      }
+      if (r.hi > 0.f) f(k, r);
+    }
   }
-  if (greedy) {  // all mass is on one token, and it stays there: its draft would have been accepted
-    if (rank == 0 && tid == 0) finish(sm.best[node]);
-    return;
+};
+
+template <bool DRAFT>
+__global__ void __launch_bounds__(SP_SUM_THREADS) verify_sums_kernel(const __grid_constant__ VerifyArgs a) {
+  constexpr int PER = SP_CHUNK / SP_SUM_THREADS;
+  __shared__ uint4 held[PER][SP_SUM_THREADS];
+  __shared__ double ssum[SP_SUM_THREADS / 32];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int c = blockIdx.x % a.chunks, b = blockIdx.x / a.chunks;
+  const WalkEnd& e = a.end[b];
+  if (e.node < 0) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const LastRow<DRAFT> last(a, e, a.temperature[b]);
+  // all loads first, the work on them in a loop (unrolled, it was ten times slower: it did not fit the instruction cache)
+#pragma unroll
+  for (int i = 0; i < PER; ++i) held[i][tid] = last.row.load(c * SP_CHUNK + i * SP_SUM_THREADS + tid);
+  const bool less = e.less != 0;
+  Two part = {0.f, 0.f};
+#pragma unroll 1
+  for (int i = 0; i < PER; ++i) last.left(held[i][tid], c * SP_CHUNK + i * SP_SUM_THREADS + tid, less, [&](int, const Two& r) { two_add(part, r); });
+  double sum = two_double(part);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) ssum[warp] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < SP_SUM_THREADS / 32; ++w) sum += ssum[w];
+    a.sums[static_cast<long long>(b) * a.chunks + c] = sum;
   }
-  // ---- the last token: the first whose cumulative sum exceeds the coin's share of what is left
-  double mine, before;
-  int last;
-  bool less = sm.pending != 0;
-  double sum = cluster_sum(less, mine, before, last);
-  if (less && !(sum > 0.0)) {  // nothing is left: the residual before this rejection
-    less = false;
-    sum = cluster_sum(less, mine, before, last);
+}
+
+// One CTA per sequence, a thread for every granule of a chunk.
+template <bool DRAFT>
+__global__ void __launch_bounds__(SP_CHUNK) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
+  __shared__ double ssum[SP_CHUNK / 32];
+  __shared__ int pick, tail;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const WalkEnd& e = a.end[b];
+  if (e.node < 0) return;
+  const float temp = a.temperature[b];
+  const double u = static_cast<double>(a.u_sample[b]);
+  const double* sums = a.sums + static_cast<long long>(b) * a.chunks;
+  const LastRow<DRAFT> last(a, e, temp);
+  bool less = e.less != 0;
+  if (tid == 0) {
+    pick = a.V;
+    tail = -1;
   }
-  const double target = static_cast<double>(a.u_sample[b]) * sum;
-  if (before <= target && before + mine > target) {
-    double c = before;
-    int pick = -1;
-    visit(less, [&](int e, double r) {
-      c += r;
-      if (r > 0.0) pick = e;
-      return !(c > target);
+  // One chunk: the token in which the cumulative sum (`before` at the chunk's beginning) passes `target`, if it does, to
+  // `pick`, the last token with weight to `tail`.  Returns the cumulative sum at the chunk's end.
+  auto look = [&](int chunk, double before, double target) {
+    const int g = chunk * SP_CHUNK + tid;
+    const uint4 v = last.row.load(g);
+    Two part = {0.f, 0.f};
+    int mine_last = -1;
+    last.left(v, g, less, [&](int k, const Two& r) {
+      two_add(part, r);
+      mine_last = g * 8 - last.row.skip + k;
     });
-    finish(pick);
-  } else if (rank == 0 && tid == 0 && !(sum > target)) {
-    finish(max(last, 0));  // a coin of the last share, or a row without weight
+    const double mine = two_double(part);
+    double incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    __syncthreads();
+    if (lane == 31) ssum[warp] = incl;
+    __syncthreads();
+    double warps = lane < SP_CHUNK / 32 ? ssum[lane] : 0.0, upto = warps;  // the warps' sums, added up by every warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const double all = __shfl_sync(0xffffffffu, upto, 31);
+    const double from = before + (__shfl_sync(0xffffffffu, upto - warps, warp) + (incl - mine));
+    if (mine_last >= 0) atomicMax(&tail, mine_last);
+    if (from <= target && from + mine > target) {
+      int found = -1;
+      double c = from;
+      last.left(v, g, less, [&](int k, const Two& r) {
+        if (c <= target) found = g * 8 - last.row.skip + k;
+        c += two_double(r);
+      });
+      if (found >= 0) atomicMin(&pick, found);  // one thread, or two at a border that rounding moved
+    }
+    __syncthreads();
+    return before + all;
+  };
+  double sum = 0.0;
+  for (int c = lane; c < a.chunks; c += 32) sum += sums[c];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const double target = u * sum;
+  // the chunk in which the sum passes the coin's share: every warp adds the chunks up, 32 at a time
+  double before = 0.0;
+  int chunk = -1;
+  for (int c0 = 0; c0 < a.chunks && chunk < 0; c0 += 32) {
+    const double x = c0 + lane < a.chunks ? sums[c0 + lane] : 0.0;
+    double upto = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, before + upto > target);
+    if (over) {
+      const int at = __ffs(static_cast<int>(over)) - 1;
+      chunk = c0 + at;
+      before += __shfl_sync(0xffffffffu, upto - x, at);
+    } else {
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  __syncthreads();
+  if (sum > 0.0 && chunk >= 0) look(chunk, before, target);
+  __syncthreads();
+  if (pick == a.V && (!(sum > 0.0) || chunk < 0 || tail < 0)) {
+    // Rare: nothing is left (then the residual before the last rejection), or a coin of the last share.  Chunk after chunk.
+    if (!(sum > 0.0)) less = false;
+    double total = 0.0;
+    for (int c = 0; c < a.chunks; ++c) total = look(c, total, INFINITY);
+    double upto = 0.0;
+    for (int c = 0; c < a.chunks; ++c) {
+      upto = look(c, upto, u * total);
+      if (pick < a.V) break;
+    }
+  }
+  if (tid == 0) {
+    const int x = pick < a.V ? pick : max(tail, 0);
+    const float z = __bfloat162float(a.logits[e.node * a.ld + x]);
+    const long long o = static_cast<long long>(b) * a.max_nodes + e.k;
+    a.out_tokens[o] = x;
+    a.logprobs[o] = static_cast<float>(static_cast<double>(__fsub_rn(__fdiv_rn(z, temp), e.top)) - sp_log(e.total));
   }
 }
 
@@ -492,8 +744,31 @@ kv_commit_kernel(const __grid_constant__ CommitLayers layers, int L, long long l
 
 using namespace b200;
 
-// columns of the statistics' chunks, and how many a row has
-static int sp_chunks(int V) { return ((V + 14) / 8 + SP_CHUNK - 1) / SP_CHUNK; }
+// pieces (statistics) and chunks (last draw) of a row that may begin anywhere in its first granule
+static int sp_parts(int V, int granules) { return ((V + 14) / 8 + granules - 1) / granules; }
+
+struct VerifyScratch {
+  long long part, first, end, sums, total;  // offsets in bytes
+  VerifyScratch(int B, int N, int V) {
+    const long long pieces = static_cast<long long>(N) * sp_parts(V, SP_PIECE), chunks = static_cast<long long>(B) * sp_parts(V, SP_CHUNK);
+    auto take = [&](long long bytes) {
+      const long long at = total;
+      total += (bytes + 15) / 16 * 16;
+      return at;
+    };
+    total = 0;
+    part = take(pieces * 8);
+    first = take(pieces * 4);
+    end = take(B * static_cast<long long>(sizeof(WalkEnd)));
+    sums = take(chunks * 8);
+  }
+};
+
+// bytes of workspace that b200_verify_tree needs
+extern "C" long long b200_verify_tree_scratch(int B, int N, int V) {
+  if (B < 0 || N < 0 || V < 1) return -1;
+  return VerifyScratch(B, N, V).total;
+}
 
 extern "C" int b200_verify_tree(const void* logits, long long ld, int V, const float* draft, long long draft_ld, const long long* tokens,
                                 const int* parents, const int* cu, int B, int N, int max_nodes, const float* temperature,
@@ -513,7 +788,8 @@ extern "C" int b200_verify_tree(const void* logits, long long ld, int V, const f
   a.B = B;
   a.N = N;
   a.max_nodes = max_nodes;
-  a.chunks = sp_chunks(V);
+  a.pieces = sp_parts(V, SP_PIECE);
+  a.chunks = sp_parts(V, SP_CHUNK);
   a.temperature = temperature;
   a.u_accept = u_accept;
   a.u_sample = u_sample;
@@ -521,15 +797,28 @@ extern "C" int b200_verify_tree(const void* logits, long long ld, int V, const f
   a.out_tokens = out_tokens;
   a.path = path;
   a.logprobs = logprobs;
-  a.part = reinterpret_cast<float4*>(scratch);
-  const double ctas = static_cast<double>(B) * max_nodes * a.chunks;
-  if (ctas >= 2147483648.0 || static_cast<double>(B) * SP_CLUSTER >= 2147483648.0) return -3;
+  const VerifyScratch at(B, N, V);
+  unsigned char* ws = reinterpret_cast<unsigned char*>(scratch);
+  a.part = reinterpret_cast<float2*>(ws + at.part);
+  a.first = reinterpret_cast<int*>(ws + at.first);
+  a.end = reinterpret_cast<WalkEnd*>(ws + at.end);
+  a.sums = reinterpret_cast<double*>(ws + at.sums);
+  if (static_cast<double>(B) * a.chunks >= 2147483648.0 || static_cast<double>(B) * SP_CLUSTER >= 2147483648.0) return -3;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
   if (N > 0) {
-    const cudaError_t e = launch_pdl(verify_stats_kernel, dim3(static_cast<unsigned>(ctas)), dim3(SP_STAT_THREADS), 0, st, a);
-    if (e != cudaSuccess) return static_cast<int>(e);
+    // a warp for every piece until the GPU is full of them
+    const long long items = static_cast<long long>(N) * a.pieces, warps = SP_STAT_THREADS / 32, most = 148 * SP_STAT_CTAS;
+    const long long ctas = (items + warps - 1) / warps < most ? (items + warps - 1) / warps : most;
+    e = launch_pdl(verify_stats_kernel, dim3(static_cast<unsigned>(ctas)), dim3(SP_STAT_THREADS), 0, st, a);
   }
-  const cudaError_t e = launch_pdl(verify_walk_kernel, dim3(B * SP_CLUSTER), dim3(SP_THREADS), 0, st, a);
+  if (e == cudaSuccess)
+    e = draft ? launch_pdl(verify_walk_draft_kernel, dim3(B * SP_CLUSTER), dim3(SP_THREADS), 0, st, a)
+              : launch_pdl(verify_walk_kernel, dim3(B), dim3(SP_THREADS / 2), 0, st, a);
+  const auto sums = draft ? verify_sums_kernel<true> : verify_sums_kernel<false>;
+  const auto pick = draft ? verify_pick_kernel<true> : verify_pick_kernel<false>;
+  if (e == cudaSuccess) e = launch_pdl(sums, dim3(static_cast<unsigned>(B) * a.chunks), dim3(SP_SUM_THREADS), 0, st, a);
+  if (e == cudaSuccess) e = launch_pdl(pick, dim3(B), dim3(SP_CHUNK), 0, st, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 

@@ -552,7 +552,7 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     out_tokens = torch.empty(B, max_nodes, dtype=torch.int64, device=dev)
     path = torch.empty(B, max_nodes, dtype=torch.int32, device=dev)
     logprobs = torch.empty(B, max_nodes, dtype=torch.float32, device=dev)
-    scratch = torch.empty(N * -(-((V + 14) // 8) // 2048), 4, dtype=torch.float32, device=dev)  # statistics of 16384-column chunks
+    scratch = torch.empty(lib.load_ops().b200_verify_tree_scratch(B, N, V), dtype=torch.uint8, device=dev)
     _call_on(dev, "b200_verify_tree", ptr(logits), logits.stride(0), V, ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0),
              ptr(tokens), ptr(parents), ptr(cu_nodes), B, N, max_nodes, ptr(temperature), ptr(u_accept), ptr(u_sample), ptr(count),
              ptr(out_tokens), ptr(path), ptr(logprobs), ptr(scratch))

@@ -60,10 +60,13 @@ _SIGNATURES = {
     "b200_tree_attn": [P, L, P, P, I, P, L, I, P, P, P, I, I, I, I, I, I, F, P, P, P, P],
     "b200_tree_attn_scratch": [I, I, I],
     "b200_verify_tree": [P, L, I, P, L, P, P, P, I, I, I, P, P, P, P, P, P, P, P, P],
+    "b200_verify_tree_scratch": [I, I, I],
     "b200_kv_commit": [P, I, L, I, P, P, L, I, P, L, I, P, P, I, I, I, I, I, P],
     "b200_attn_fwd": [P, P, P, P, P, I, I, I, I, I, I, F, P],
     "b200_attn_bwd": [P, P, P, P, P, P, P, P, I, I, I, I, I, I, F, P],
 }
+
+_RESULTS = {"b200_verify_tree_scratch": c_longlong}
 
 
 class KernelError(RuntimeError):
@@ -89,7 +92,7 @@ def load_ops():
             if hasattr(lib, name):
                 fn = getattr(lib, name)
                 fn.argtypes = argtypes
-                fn.restype = c_int
+                fn.restype = _RESULTS.get(name, c_int)
         _ops = lib
         return lib
 
@@ -174,7 +177,7 @@ def check_status(sync: bool = True) -> None:
 
 
 # kernels launched per library call (for launch accounting in benchmarks)
-_KERNELS_PER_CALL = {"b200_attn_bwd": 3, "b200_tree_attn": 2, "b200_verify_tree": 2, "b200_rmsnorm_bwd": 2, "b200_sumsq": 2, "b200_allgather_copy": 0}
+_KERNELS_PER_CALL = {"b200_attn_bwd": 3, "b200_tree_attn": 2, "b200_verify_tree": 4, "b200_rmsnorm_bwd": 2, "b200_sumsq": 2, "b200_allgather_copy": 0}
 launch_count = 0
 
 

@@ -228,6 +228,18 @@ def test_verification_edges(drafted):
     assert (got[3].cpu().double() - want[3]).abs().max() <= logprob_bound(300)
 
 
+@pytest.mark.parametrize("vocab", [300, 20011])
+def test_verification_where_a_rejection_leaves_nothing(vocab):
+    """A drafter's row that is nowhere below the target's: the residual is empty and stays what it was, before the next sibling and
+    before the last draw."""
+    a = make_verify([2, 4, 4, 3], vocab, "star", True, temps=(1.0, 0.9), seed=12, device="cuda")
+    a["draft_probs"][:] = 1.0
+    a["u_accept"][:] = 1.0 - 2.0 ** -24
+    a["u_accept"][3] = 0.0
+    a["draft_probs"][6] = 0.5 * torch.softmax(a["logits"][6].float(), -1)   # something is left here
+    _check_verify(a)
+
+
 def test_verification_rows_without_a_finite_logit_stay_in_range():
     from open_instruct_b200.ops import fused
 
