@@ -36,7 +36,7 @@ constexpr int SP_PIECE = SP_LOADS * 32;              // granules of a piece (204
 constexpr int SP_STAT_THREADS = 256;
 constexpr int SP_STAT_CTAS = 2;                      // resident on an SM
 constexpr int SP_SUM_THREADS = 256;
-constexpr int SP_CHUNK = 1024;                       // granules of a chunk of the last draw (8192 logits), threads of the kernel that picks in it
+constexpr int SP_CHUNK = 1024;                       // granules of a chunk of the last draw (8192 logits)
 constexpr int SP_CLUSTER = 8;
 constexpr int SP_THREADS = 512;                      // of a walking CTA with draft probabilities; 256 without
 constexpr float SP_LOG2E = 1.4426950408889634f;
@@ -133,6 +133,23 @@ __device__ __forceinline__ Two two_of(double x) {
   const float hi = static_cast<float>(x);
   return {hi, static_cast<float>(x - static_cast<double>(hi))};
 }
+// Two running sums side by side, one instruction for both.
+struct TwoPair {
+  uint64_t hi, lo;
+  __device__ __forceinline__ void add(uint64_t x) {
+    const uint64_t s = add2(hi, x), t = sub2(s, hi);
+    lo = add2(lo, add2(sub2(hi, sub2(s, t)), sub2(x, t)));
+    hi = s;
+  }
+  __device__ __forceinline__ Two sum() const {
+    float h0, h1, l0, l1;
+    unpair2(hi, h0, h1);
+    unpair2(lo, l0, l1);
+    Two s = {h0, l0};
+    const Two x = two_sum(s.hi, h1);
+    return {x.hi, __fadd_rn(x.lo, __fadd_rn(l0, l1))};
+  }
+};
 __device__ __forceinline__ double two_double(const Two& x) { return static_cast<double>(x.hi) + static_cast<double>(x.lo); }
 
 // log of a positive sum: the exponent's share in fp64, the logarithm of the mantissa in fp32 (off by less than 2^-23)
@@ -283,6 +300,117 @@ __device__ __forceinline__ Two sp_residual(Two p, float q, const float2* rz, int
   return p;
 }
 
+// What is left of the tokens of one row at some point of a walk: weights (point-mass drafts) or probabilities.
+template <bool DRAFT>
+struct LeftRow {
+  LogitRow row;
+  const float* q;
+  const float2* rz;
+  const int* gone;
+  float temp, top;
+  Two inv;
+  int nz, ngone;
+  bool q4;  // granules of q are 16-byte aligned
+  __device__ __forceinline__ LeftRow(const VerifyArgs& a, int n, float temperature, float top_, Two inv_, const float2* rz_, int nz_, const int* gone_,
+                                     int ngone_)
+      : row(a.logits + n * a.ld, a.V), q(DRAFT ? a.draft + n * a.draft_ld : nullptr), rz(rz_), gone(gone_), temp(temperature), top(top_), inv(inv_),
+        nz(nz_), ngone(ngone_) {
+    q4 = DRAFT && ((reinterpret_cast<uintptr_t>(q) - 4 * row.skip) & 15) == 0;
+  }
+  // tokens of granule g that are outside of the row or rejected, as bits
+  __device__ __forceinline__ uint32_t dropped(int g) const {
+    const int e0 = g * 8 - row.skip;
+    uint32_t drop = 0;
+    if (g == 0 || g >= row.count - 1) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (e0 + k < 0 || e0 + k >= row.V) drop |= 1u << k;
+    }
+    if (!DRAFT)
+      for (int j = 0; j < ngone; ++j) {
+        const int d = gone[j] - e0;
+        if (d >= 0 && d < 8) drop |= 1u << d;
+      }
+    return drop;
+  }
+  __device__ __forceinline__ void draft(int g, uint32_t drop, float (&qs)[8]) const {
+    const int e0 = g * 8 - row.skip;
+    if (q4 && !drop) {
+      const float4 lo = __ldg(reinterpret_cast<const float4*>(q + e0)), hi = __ldg(reinterpret_cast<const float4*>(q + e0) + 1);
+      qs[0] = lo.x, qs[1] = lo.y, qs[2] = lo.z, qs[3] = lo.w, qs[4] = hi.x, qs[5] = hi.y, qs[6] = hi.z, qs[7] = hi.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) qs[k] = (drop >> k & 1u) ? 0.f : __ldg(q + e0 + k);
+    }
+  }
+  __device__ __forceinline__ void weights(const uint4& v, uint32_t drop, float (&w)[8]) const {
+    if (temp == 1.f) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = expf(__fsub_rn(sp_logit(v, k), top));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = expf(__fsub_rn(__fdiv_rn(sp_logit(v, k), temp), top));
+    }
+    if (drop) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (drop >> k & 1u) w[k] = 0.f;
+    }
+  }
+  // f(k, what is left of it) for the tokens of granule g that have anything left, in their order
+  template <typename F>
+  __device__ __forceinline__ void left(const uint4& v, int g, bool less, F&& f) const {
+    const uint32_t drop = dropped(g);
+    float qs[8];
+    if (DRAFT) draft(g, drop, qs);
+    float w[8];
+    weights(v, drop, w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      Two r = {w[k], 0.f};
+      if (DRAFT) r = sp_residual(two_mul(inv, r), qs[k], rz, nz, less);
+      if (r.hi > 0.f) f(k, r);
+    }
+  }
+  // the granule's share of a running sum
+  __device__ __forceinline__ void add(const uint4& v, int g, bool less, TwoPair& sum) const {
+    const uint32_t drop = dropped(g);
+    float qs[8];
+    if (DRAFT) draft(g, drop, qs);
+    float w[8];
+    weights(v, drop, w);
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      uint64_t x = pair2(w[k], w[k + 1]);
+      if (DRAFT) {
+        if (nz == 0) {  // the common case: w * inv (- q)
+          const uint64_t ih = pair2(inv.hi, inv.hi), il = pair2(inv.lo, inv.lo), p = mul2(x, ih);
+          uint64_t lo = fma2(x, il, fma2(x, ih, sub2(0ull, p)));
+          uint64_t hi = p;
+          if (less) {
+            const uint64_t y = pair2(-qs[k], -qs[k + 1]);
+            const uint64_t s = add2(p, y), t = sub2(s, p);
+            lo = add2(lo, add2(sub2(p, sub2(s, t)), sub2(y, t)));
+            hi = s;
+          }
+          const uint64_t n = add2(hi, lo);
+          lo = sub2(lo, sub2(n, hi));
+          float n0, n1, l0, l1;
+          unpair2(n, n0, n1);
+          unpair2(lo, l0, l1);
+          sum.lo = add2(sum.lo, pair2(n0 > 0.f ? l0 : 0.f, n1 > 0.f ? l1 : 0.f));
+          x = pair2(fmaxf(n0, 0.f), fmaxf(n1, 0.f));
+        } else {
+          const Two r0 = sp_residual(two_mul(inv, Two{w[k], 0.f}), qs[k], rz, nz, less), r1 = sp_residual(two_mul(inv, Two{w[k + 1], 0.f}), qs[k + 1], rz, nz, less);
+          sum.lo = add2(sum.lo, pair2(r0.lo, r1.lo));
+          x = pair2(r0.hi, r1.hi);
+        }
+      }
+      sum.add(x);
+    }
+  }
+};
+
 // One CTA for a sequence, with draft probabilities a cluster of eight whose CTAs all take the same walk.
 template <bool DRAFT>
 __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
@@ -367,20 +495,10 @@ __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
   // the sum of max(r - q, 0) over the vocabulary at the current node, the same in every CTA of the cluster
   auto residual_sum = [&] {
     const int node = sm.cur, nz = sm.nz;
-    const LogitRow row(a.logits + (n0 + node) * a.ld, a.V);
-    const float* q = a.draft + (n0 + node) * a.draft_ld;
-    const float top = sm.top[node];
-    const Two inv = two_of(1.0 / sm.total[node]);
-    Two part = {0.f, 0.f};
-    for (int g = rank * threads + tid; g < row.count; g += SP_CLUSTER * threads) {
-      const uint4 v = row.load(g);
-      const int e0 = g * 8 - row.skip;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e0 + e >= 0 && e0 + e < a.V)
-          two_add(part, sp_residual(two_mul(inv, Two{sp_weight(sp_logit(v, e), temp, top), 0.f}), __ldg(q + e0 + e), sm.rz, nz, true));
-    }
-    double mine = two_double(part);
+    const LeftRow<DRAFT> row(a, n0 + node, temp, sm.top[node], two_of(1.0 / sm.total[node]), sm.rz, nz, nullptr, 0);
+    TwoPair part = {0ull, 0ull};
+    for (int g = rank * threads + tid; g < row.row.count; g += SP_CLUSTER * threads) row.add(row.row.load(g), g, true, part);
+    double mine = two_double(part.sum());
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0) sm.warp_sum[warp] = mine;
@@ -514,64 +632,6 @@ __global__ void __cluster_dims__(SP_CLUSTER, 1, 1) __launch_bounds__(SP_THREADS)
   verify_walk<true>(a, sm);
 }
 
-// What is left of the tokens of the row in which a walk ended: weights (point-mass drafts) or probabilities.
-template <bool DRAFT>
-struct LastRow {
-  LogitRow row;
-  const float* q;
-  const WalkEnd* end;
-  float temp, top;
-  Two inv;
-  int nz, ngone;
-  bool q4;  // granules of q are 16-byte aligned
-  __device__ __forceinline__ LastRow(const VerifyArgs& a, const WalkEnd& e, float temperature)
-      : row(a.logits + e.node * a.ld, a.V), q(DRAFT ? a.draft + e.node * a.draft_ld : nullptr), end(&e), temp(temperature), top(e.top),
-        inv{e.inv_total.x, e.inv_total.y}, nz(e.nz), ngone(e.ngone) {
-    q4 = DRAFT && ((reinterpret_cast<uintptr_t>(q) - 4 * row.skip) & 15) == 0;
-  }
-  // f(k, what is left of it) for the tokens of granule g that have anything left, in their order
-  template <typename F>
-  __device__ __forceinline__ void left(const uint4& v, int g, bool less, F&& f) const {
-    const int e0 = g * 8 - row.skip;
-    uint32_t drop = 0;  // outside of the row, or rejected
-    if (g == 0 || g >= row.count - 1) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (e0 + k < 0 || e0 + k >= row.V) drop |= 1u << k;
-    }
-    if (!DRAFT)
-      for (int j = 0; j < ngone; ++j) {
-        const int d = end->gone[j] - e0;
-        if (d >= 0 && d < 8) drop |= 1u << d;
-      }
-    float qs[8];
-    if (DRAFT) {
-      if (q4 && !drop) {
-        const float4 lo = __ldg(reinterpret_cast<const float4*>(q + e0)), hi = __ldg(reinterpret_cast<const float4*>(q + e0) + 1);
-        qs[0] = lo.x, qs[1] = lo.y, qs[2] = lo.z, qs[3] = lo.w, qs[4] = hi.x, qs[5] = hi.y, qs[6] = hi.z, qs[7] = hi.w;
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) qs[k] = (drop >> k & 1u) ? 0.f : __ldg(q + e0 + k);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float w = sp_weight(sp_logit(v, k), temp, top);
-      Two r = {(drop >> k & 1u) ? 0.f : w, 0.f};
-      if (DRAFT) {
-        if (nz == 0) {  // the common case without the loop: w * inv - q, hi and lo
-          const float p = __fmul_rn(r.hi, inv.hi), lo = __fmaf_rn(r.hi, inv.lo, __fmaf_rn(r.hi, inv.hi, -p));
-          const Two d = two_sum(p, less ? -qs[k] : 0.f);
-          r = two_norm(d.hi, __fadd_rn(d.lo, lo));
-        } else {
-          r = sp_residual(two_mul(inv, r), qs[k], end->rz, nz, less);
-        }
-      }
-      if (r.hi > 0.f) f(k, r);
-    }
-  }
-};
-
 template <bool DRAFT>
 __global__ void __launch_bounds__(SP_SUM_THREADS) verify_sums_kernel(const __grid_constant__ VerifyArgs a) {
   constexpr int PER = SP_CHUNK / SP_SUM_THREADS;
@@ -583,15 +643,15 @@ __global__ void __launch_bounds__(SP_SUM_THREADS) verify_sums_kernel(const __gri
   const WalkEnd& e = a.end[b];
   if (e.node < 0) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const LastRow<DRAFT> last(a, e, a.temperature[b]);
+  const LeftRow<DRAFT> last(a, e.node, a.temperature[b], e.top, Two{e.inv_total.x, e.inv_total.y}, e.rz, e.nz, e.gone, e.ngone);
   // all loads first, the work on them in a loop (unrolled, it was ten times slower: it did not fit the instruction cache)
 #pragma unroll
   for (int i = 0; i < PER; ++i) held[i][tid] = last.row.load(c * SP_CHUNK + i * SP_SUM_THREADS + tid);
   const bool less = e.less != 0;
-  Two part = {0.f, 0.f};
+  TwoPair part = {0ull, 0ull};
 #pragma unroll 1
-  for (int i = 0; i < PER; ++i) last.left(held[i][tid], c * SP_CHUNK + i * SP_SUM_THREADS + tid, less, [&](int, const Two& r) { two_add(part, r); });
-  double sum = two_double(part);
+  for (int i = 0; i < PER; ++i) last.add(held[i][tid], c * SP_CHUNK + i * SP_SUM_THREADS + tid, less, part);
+  double sum = two_double(part.sum());
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) ssum[warp] = sum;
@@ -602,10 +662,13 @@ __global__ void __launch_bounds__(SP_SUM_THREADS) verify_sums_kernel(const __gri
   }
 }
 
-// One CTA per sequence, a thread for every granule of a chunk.
+// One CTA per sequence, a thread has consecutive granules of a chunk: two, so that two CTAs fit on an SM and 256 sequences are
+// one wave (16 -> 10 us), with draft probabilities one (two make the code too long for the instruction cache: 11 -> 20 us).
+constexpr int sp_pick_threads(bool draft) { return draft ? SP_CHUNK : SP_CHUNK / 2; }
 template <bool DRAFT>
-__global__ void __launch_bounds__(SP_CHUNK) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
-  __shared__ double ssum[SP_CHUNK / 32];
+__global__ void __launch_bounds__(sp_pick_threads(DRAFT), DRAFT ? 1 : 2) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
+  constexpr int THREADS = sp_pick_threads(DRAFT), PER = SP_CHUNK / THREADS;
+  __shared__ double ssum[THREADS / 32];
   __shared__ int pick, tail;
   griddep_launch_dependents();
   griddep_wait();
@@ -615,7 +678,7 @@ __global__ void __launch_bounds__(SP_CHUNK) verify_pick_kernel(const __grid_cons
   const float temp = a.temperature[b];
   const double u = static_cast<double>(a.u_sample[b]);
   const double* sums = a.sums + static_cast<long long>(b) * a.chunks;
-  const LastRow<DRAFT> last(a, e, temp);
+  const LeftRow<DRAFT> last(a, e.node, temp, e.top, Two{e.inv_total.x, e.inv_total.y}, e.rz, e.nz, e.gone, e.ngone);
   bool less = e.less != 0;
   if (tid == 0) {
     pick = a.V;
@@ -624,14 +687,18 @@ __global__ void __launch_bounds__(SP_CHUNK) verify_pick_kernel(const __grid_cons
   // One chunk: the token in which the cumulative sum (`before` at the chunk's beginning) passes `target`, if it does, to
   // `pick`, the last token with weight to `tail`.  Returns the cumulative sum at the chunk's end.
   auto look = [&](int chunk, double before, double target) {
-    const int g = chunk * SP_CHUNK + tid;
-    const uint4 v = last.row.load(g);
+    const int g = chunk * SP_CHUNK + tid * PER;
+    uint4 v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = last.row.load(g + i);
     Two part = {0.f, 0.f};
     int mine_last = -1;
-    last.left(v, g, less, [&](int k, const Two& r) {
-      two_add(part, r);
-      mine_last = g * 8 - last.row.skip + k;
-    });
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      last.left(v[i], g + i, less, [&](int k, const Two& r) {
+        two_add(part, r);
+        mine_last = (g + i) * 8 - last.row.skip + k;
+      });
     const double mine = two_double(part);
     double incl = mine;
 #pragma unroll
@@ -642,7 +709,7 @@ __global__ void __launch_bounds__(SP_CHUNK) verify_pick_kernel(const __grid_cons
     __syncthreads();
     if (lane == 31) ssum[warp] = incl;
     __syncthreads();
-    double warps = lane < SP_CHUNK / 32 ? ssum[lane] : 0.0, upto = warps;  // the warps' sums, added up by every warp
+    double warps = lane < THREADS / 32 ? ssum[lane] : 0.0, upto = warps;  // the warps' sums, added up by every warp
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double x = __shfl_up_sync(0xffffffffu, upto, o);
@@ -654,10 +721,12 @@ __global__ void __launch_bounds__(SP_CHUNK) verify_pick_kernel(const __grid_cons
     if (from <= target && from + mine > target) {
       int found = -1;
       double c = from;
-      last.left(v, g, less, [&](int k, const Two& r) {
-        if (c <= target) found = g * 8 - last.row.skip + k;
-        c += two_double(r);
-      });
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        last.left(v[i], g + i, less, [&](int k, const Two& r) {
+          if (c <= target) found = (g + i) * 8 - last.row.skip + k;
+          c += two_double(r);
+        });
       if (found >= 0) atomicMin(&pick, found);  // one thread, or two at a border that rounding moved
     }
     __syncthreads();
@@ -818,7 +887,7 @@ extern "C" int b200_verify_tree(const void* logits, long long ld, int V, const f
   const auto sums = draft ? verify_sums_kernel<true> : verify_sums_kernel<false>;
   const auto pick = draft ? verify_pick_kernel<true> : verify_pick_kernel<false>;
   if (e == cudaSuccess) e = launch_pdl(sums, dim3(static_cast<unsigned>(B) * a.chunks), dim3(SP_SUM_THREADS), 0, st, a);
-  if (e == cudaSuccess) e = launch_pdl(pick, dim3(B), dim3(SP_CHUNK), 0, st, a);
+  if (e == cudaSuccess) e = launch_pdl(pick, dim3(B), dim3(sp_pick_threads(draft != nullptr)), 0, st, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
