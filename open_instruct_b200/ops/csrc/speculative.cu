@@ -357,56 +357,40 @@ struct LeftRow {
         if (drop >> k & 1u) w[k] = 0.f;
     }
   }
-  // f(k, what is left of it) for the tokens of granule g that have anything left, in their order
-  template <typename F>
-  __device__ __forceinline__ void left(const uint4& v, int g, bool less, F&& f) const {
+  // what is left of the eight tokens of granule g
+  __device__ __forceinline__ void left(const uint4& v, int g, bool less, Two (&r)[8]) const {
     const uint32_t drop = dropped(g);
-    float qs[8];
+    float qs[8], w[8];
     if (DRAFT) draft(g, drop, qs);
-    float w[8];
     weights(v, drop, w);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      Two r = {w[k], 0.f};
-      if (DRAFT) r = sp_residual(two_mul(inv, r), qs[k], rz, nz, less);
-      if (r.hi > 0.f) f(k, r);
+    for (int k = 0; k < 8; ++k) r[k] = DRAFT ? two_mul(inv, Two{w[k], 0.f}) : Two{w[k], 0.f};
+    if (!DRAFT) return;
+    for (int j = 0; j <= nz; ++j) {  // the residuals so far, then one more if `less`: one body for all of them
+      if (j == nz && !less) break;
+      const Two z = j < nz ? Two{rz[j].x, rz[j].y} : Two{1.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const Two d = two_minus(r[k], qs[k]);
+        r[k] = d.hi > 0.f ? two_mul(d, z) : Two{0.f, 0.f};
+      }
     }
   }
   // the granule's share of a running sum
   __device__ __forceinline__ void add(const uint4& v, int g, bool less, TwoPair& sum) const {
-    const uint32_t drop = dropped(g);
-    float qs[8];
-    if (DRAFT) draft(g, drop, qs);
-    float w[8];
-    weights(v, drop, w);
+    if (DRAFT) {
+      Two r[8];
+      left(v, g, less, r);
 #pragma unroll
-    for (int k = 0; k < 8; k += 2) {
-      uint64_t x = pair2(w[k], w[k + 1]);
-      if (DRAFT) {
-        if (nz == 0) {  // the common case: w * inv (- q)
-          const uint64_t ih = pair2(inv.hi, inv.hi), il = pair2(inv.lo, inv.lo), p = mul2(x, ih);
-          uint64_t lo = fma2(x, il, fma2(x, ih, sub2(0ull, p)));
-          uint64_t hi = p;
-          if (less) {
-            const uint64_t y = pair2(-qs[k], -qs[k + 1]);
-            const uint64_t s = add2(p, y), t = sub2(s, p);
-            lo = add2(lo, add2(sub2(p, sub2(s, t)), sub2(y, t)));
-            hi = s;
-          }
-          const uint64_t n = add2(hi, lo);
-          lo = sub2(lo, sub2(n, hi));
-          float n0, n1, l0, l1;
-          unpair2(n, n0, n1);
-          unpair2(lo, l0, l1);
-          sum.lo = add2(sum.lo, pair2(n0 > 0.f ? l0 : 0.f, n1 > 0.f ? l1 : 0.f));
-          x = pair2(fmaxf(n0, 0.f), fmaxf(n1, 0.f));
-        } else {
-          const Two r0 = sp_residual(two_mul(inv, Two{w[k], 0.f}), qs[k], rz, nz, less), r1 = sp_residual(two_mul(inv, Two{w[k + 1], 0.f}), qs[k + 1], rz, nz, less);
-          sum.lo = add2(sum.lo, pair2(r0.lo, r1.lo));
-          x = pair2(r0.hi, r1.hi);
-        }
+      for (int k = 0; k < 8; k += 2) {
+        sum.lo = add2(sum.lo, pair2(r[k].lo, r[k + 1].lo));
+        sum.add(pair2(r[k].hi, r[k + 1].hi));
       }
-      sum.add(x);
+    } else {
+      float w[8];
+      weights(v, dropped(g), w);
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) sum.add(pair2(w[k], w[k + 1]));
     }
   }
 };
@@ -664,7 +648,7 @@ __global__ void __launch_bounds__(SP_SUM_THREADS) verify_sums_kernel(const __gri
 
 // One CTA per sequence, a thread has consecutive granules of a chunk: two, so that two CTAs fit on an SM and 256 sequences are
 // one wave (16 -> 10 us), with draft probabilities one (two make the code too long for the instruction cache: 11 -> 20 us).
-constexpr int sp_pick_threads(bool draft) { return draft ? SP_CHUNK : SP_CHUNK / 2; }
+__host__ __device__ constexpr int sp_pick_threads(bool draft) { return draft ? SP_CHUNK : SP_CHUNK / 2; }
 template <bool DRAFT>
 __global__ void __launch_bounds__(sp_pick_threads(DRAFT), DRAFT ? 1 : 2) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
   constexpr int THREADS = sp_pick_threads(DRAFT), PER = SP_CHUNK / THREADS;
@@ -688,17 +672,18 @@ __global__ void __launch_bounds__(sp_pick_threads(DRAFT), DRAFT ? 1 : 2) verify_
   // `pick`, the last token with weight to `tail`.  Returns the cumulative sum at the chunk's end.
   auto look = [&](int chunk, double before, double target) {
     const int g = chunk * SP_CHUNK + tid * PER;
-    uint4 v[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = last.row.load(g + i);
+    Two r[PER][8];
     Two part = {0.f, 0.f};
     int mine_last = -1;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      last.left(v[i], g + i, less, [&](int k, const Two& r) {
-        two_add(part, r);
-        mine_last = (g + i) * 8 - last.row.skip + k;
-      });
+    for (int i = 0; i < PER; ++i) {
+      last.left(last.row.load(g + i), g + i, less, r[i]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        two_add(part, r[i][k]);
+        if (r[i][k].hi > 0.f) mine_last = (g + i) * 8 - last.row.skip + k;
+      }
+    }
     const double mine = two_double(part);
     double incl = mine;
 #pragma unroll
@@ -720,13 +705,16 @@ __global__ void __launch_bounds__(sp_pick_threads(DRAFT), DRAFT ? 1 : 2) verify_
     if (mine_last >= 0) atomicMax(&tail, mine_last);
     if (from <= target && from + mine > target) {
       int found = -1;
-      double c = from;
+      const Two room = two_of(target - from);  // what the sum may grow by
+      Two c = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        last.left(v[i], g + i, less, [&](int k, const Two& r) {
-          if (c <= target) found = (g + i) * 8 - last.row.skip + k;
-          c += two_double(r);
-        });
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (r[i][k].hi > 0.f && __fadd_rn(__fsub_rn(c.hi, room.hi), __fsub_rn(c.lo, room.lo)) <= 0.f) found = (g + i) * 8 - last.row.skip + k;
+          two_add(c, r[i][k]);
+          c = two_norm(c.hi, c.lo);
+        }
       if (found >= 0) atomicMin(&pick, found);  // one thread, or two at a border that rounding moved
     }
     __syncthreads();
@@ -758,18 +746,21 @@ __global__ void __launch_bounds__(sp_pick_threads(DRAFT), DRAFT ? 1 : 2) verify_
     }
   }
   __syncthreads();
-  if (sum > 0.0 && chunk >= 0) look(chunk, before, target);
-  __syncthreads();
-  if (pick == a.V && (!(sum > 0.0) || chunk < 0 || tail < 0)) {
-    // Rare: nothing is left (then the residual before the last rejection), or a coin of the last share.  Chunk after chunk.
-    if (!(sum > 0.0)) less = false;
-    double total = 0.0;
-    for (int c = 0; c < a.chunks; ++c) total = look(c, total, INFINITY);
-    double upto = 0.0;
-    for (int c = 0; c < a.chunks; ++c) {
-      upto = look(c, upto, u * total);
+  // That chunk.  Rare, where it does not settle the matter (nothing is left: then the residual before the last rejection counts;
+  // a coin of the last share): all chunks for their sum, then one after the other.
+  const bool settled = sum > 0.0 && chunk >= 0;
+  double total = 0.0;
+  for (int round = settled ? 0 : 1; round < 3; ++round) {
+    if (round == 1 && !(sum > 0.0)) less = false;
+    double upto = round == 0 ? before : 0.0;
+    const double goal = round == 0 ? target : round == 1 ? INFINITY : u * total;
+    for (int c = round == 0 ? chunk : 0; c < (round == 0 ? chunk + 1 : a.chunks); ++c) {
+      upto = look(c, upto, goal);
       if (pick < a.V) break;
     }
+    if (pick < a.V || (round == 0 && tail >= 0)) break;
+    total = upto;
+    __syncthreads();
   }
   if (tid == 0) {
     const int x = pick < a.V ? pick : max(tail, 0);
