@@ -392,44 +392,47 @@ MAX_TREE_NODES = 64  # nodes of one sequence's draft tree (its newest token incl
 
 def _call_on(device: torch.device, name: str, *args) -> None:
     """``call`` with the current stream of ``device`` as the last argument, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, stream_ptr())
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)  # a tenth of the time that the stream object takes
+    if index == torch.cuda.current_device():
+        call(name, *args, stream)
     else:
         with torch.cuda.device(device):
-            call(name, *args, stream_ptr())
+            call(name, *args, stream)
 
 
 def _check_index(t: torch.Tensor, dtype, shape: tuple, device, name: str) -> None:
-    if t.dtype != dtype or t.device != device:
+    if t.dtype is not dtype or t.device != device:
         raise TypeError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous tensor of shape {shape}, got {tuple(t.shape)}")
 
 
 def _check_rows(t: torch.Tensor, dtype, width: int, device, name: str) -> None:
-    if t.dtype != dtype or t.device != device:
+    if t.dtype is not dtype or t.device != device:
         raise TypeError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
     if t.dim() != 2 or t.shape[1] != width or t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
         raise ValueError(f"{name}: expected [N, {width}], 16-byte aligned, contiguous rows with a stride that is a multiple of 8, got {tuple(t.shape)}")
 
 
 def _check_cache(k_cache, v_cache, block_table, ctx, n_kv: int, head_dim: int, dtype, device, lead: tuple = ()) -> None:
+    shape = k_cache.shape
+    if len(shape) != 4 + len(lead) or shape != (*lead, shape[-4], n_kv, KV_PAGE, head_dim) or shape[-4] < 1 or v_cache.shape != shape:
+        raise ValueError(f"k_cache, v_cache: expected caches of [{''.join(f'{n}, ' for n in lead)}blocks, {n_kv}, {KV_PAGE}, {head_dim}] with one block at least, "
+                         f"got {tuple(shape)} and {tuple(v_cache.shape)}")
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dtype != dtype or t.device != device:
+        if t.dtype is not dtype or t.device != device:
             raise TypeError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
-        if t.dim() != 4 + len(lead) or tuple(t.shape[:len(lead)]) != lead or tuple(t.shape[-3:]) != (n_kv, KV_PAGE, head_dim) or not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError(f"{name}: expected a contiguous [{''.join(f'{n}, ' for n in lead)}blocks, {n_kv}, {KV_PAGE}, {head_dim}] cache, got {tuple(t.shape)}")
-        if t.shape[len(lead)] < 1:
-            raise ValueError(f"{name}: a cache has one page at least")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError("k_cache and v_cache must have the same shape")
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{name}: expected a contiguous, 16-byte aligned cache")
     if ctx.dim() != 1:
         raise ValueError(f"ctx: expected [B], got {tuple(ctx.shape)}")
-    _check_index(ctx, torch.int32, (ctx.shape[0],), device, "ctx")
-    if block_table.dtype != torch.int32 or block_table.device != device:
+    batch = ctx.shape[0]
+    _check_index(ctx, torch.int32, (batch,), device, "ctx")
+    if block_table.dtype is not torch.int32 or block_table.device != device:
         raise TypeError(f"block_table: expected int32 on {device}, got {block_table.dtype} on {block_table.device}")
-    if block_table.dim() != 2 or block_table.shape[0] != ctx.shape[0] or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"block_table: expected [{ctx.shape[0]}, pages] with contiguous rows, got {tuple(block_table.shape)}")
+    if block_table.dim() != 2 or block_table.shape[0] != batch or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError(f"block_table: expected [{batch}, pages] with contiguous rows, got {tuple(block_table.shape)}")
 
 
 def _check_tree_attn(qkv, k_cache, v_cache, block_table, ctx, cu_nodes, parents, n_q: int, n_kv: int, head_dim: int, scale: float, max_nodes: int,
@@ -473,22 +476,28 @@ def _check_verify_tree(logits, tokens, parents, cu_nodes, temperature, u_accept,
             raise ValueError(f"draft_probs: expected {tuple(logits.shape)} with contiguous rows, got {tuple(draft_probs.shape)}")
 
 
-def _check_kv_commit(qkv_layers, k_cache, v_cache, block_table, ctx, path, n_q: int, n_kv: int, head_dim: int, dtype) -> None:
+def _check_kv_commit(qkv_layers, k_cache, v_cache, block_table, ctx, path, n_q: int, n_kv: int, head_dim: int, dtype) -> list:
+    """Checks the arguments and returns the layers' addresses."""
     L = len(qkv_layers)
     if L < 1 or k_cache.dim() < 1 or L != k_cache.shape[0]:
         raise ValueError(f"kv_commit_: {L} layers of qkv for a cache of shape {tuple(k_cache.shape)}")
     if head_dim != 128 or n_kv < 1 or n_q < 0:
         raise ValueError(f"kv_commit_: head_dim 128, got {n_q} / {n_kv} heads of {head_dim}")
     first = qkv_layers[0]
-    dev, shape, ld = first.device, first.shape, first.stride(0)
+    dev, shape, strides = first.device, first.shape, first.stride()
     _check_rows(first, dtype, (n_q + 2 * n_kv) * head_dim, dev, "qkv of layer 0")
-    for i, t in enumerate(qkv_layers):
-        if t.dtype != dtype or t.device != dev or t.shape != shape or t.stride(0) != ld or t.stride(1) != 1 or t.data_ptr() % 16:
-            raise ValueError(f"kv_commit_: the qkv rows of layer {i} are not laid out as those of layer 0")
+    pointers = []
+    dense = first.is_contiguous()  # then contiguous is all that has to be asked of the others' strides
+    for t in qkv_layers:
+        at = t.data_ptr()
+        if t.dtype is not dtype or t.shape != shape or not (t.is_contiguous() if dense else t.stride() == strides) or t.device != dev or at & 15:
+            raise ValueError(f"kv_commit_: the qkv rows of layer {len(pointers)} are not laid out as those of layer 0")
+        pointers.append(at)
     _check_cache(k_cache, v_cache, block_table, ctx, n_kv, head_dim, dtype, dev, (L,))
     if path.dim() != 2:
         raise ValueError(f"path: expected [B, P], got {tuple(path.shape)}")
     _check_index(path, torch.int32, (ctx.shape[0], path.shape[1]), dev, "path")
+    return pointers
 
 
 def _need_cuda(t: torch.Tensor, name: str) -> None:
@@ -570,9 +579,8 @@ def kv_commit_(qkv_layers, k_cache: torch.Tensor, v_cache: torch.Tensor, block_t
     L = len(qkv_layers)
     if L:
         _need_cuda(qkv_layers[0], "qkv")
-    _check_kv_commit(qkv_layers, k_cache, v_cache, block_table, ctx, path, n_q, n_kv, head_dim, torch.bfloat16)
-    first = qkv_layers[0]
-    pointers = (ctypes.c_void_p * L)(*[t.data_ptr() for t in qkv_layers])
+    pointers = _check_kv_commit(qkv_layers, k_cache, v_cache, block_table, ctx, path, n_q, n_kv, head_dim, torch.bfloat16)
+    first, pointers = qkv_layers[0], (ctypes.c_void_p * L)(*pointers)
     _call_on(first.device, "b200_kv_commit", ctypes.addressof(pointers), L, first.stride(0), first.shape[0], ptr(k_cache), ptr(v_cache),
              k_cache.stride(0), k_cache.shape[1], ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(ctx), ptr(path),
              ctx.shape[0], path.shape[1], n_q, n_kv, head_dim)
