@@ -145,6 +145,7 @@ def main(argv=None) -> dict:
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--csv", default="")
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
+    ap.add_argument("--speculative_tokens", type=int, default=0, help="drafted tokens per sequence and decode step (prompt lookup), 0 = none")
     ap.add_argument("--impl", default="ours", choices=["ours", "vllm"],
                     help="vllm: the same batches through vllm.LLM.generate (library bar on the same box; not this package's engine)")
     a = ap.parse_args(argv)
@@ -155,7 +156,8 @@ def main(argv=None) -> dict:
 
     spec = get_spec(a.model)
     engine = RolloutEngine(spec, device=a.device, gpu_memory_utilization=a.gpu_memory_utilization, max_running=a.max_running,
-                           max_model_len=a.prompt_length + a.response_length + 16, seed=a.seed, eos_token_ids=[])
+                           max_model_len=a.prompt_length + a.response_length + 16, seed=a.seed, eos_token_ids=[],
+                           speculative_tokens=a.speculative_tokens)
     learner_flat = engine.model.flat.detach().clone()
     dims = ModelDims.from_spec(spec)
     cfg = SamplingConfig(temperature=a.temperature, top_p=a.top_p, max_tokens=a.response_length, min_tokens=a.response_length,
@@ -181,6 +183,8 @@ def main(argv=None) -> dict:
         k = 1e3 / st["decode_steps"]
         summary["decode_step_ms"] = {"host_pack": st["host_pack_s"] * k, "device_wait": st["device_wait_s"] * k, "host_accept": st["host_accept_s"] * k,
                                      "host_schedule": st["host_sched_s"] * 1e3 / max(1, st["steps"]), "steps": st["decode_steps"]}
+    if a.speculative_tokens:
+        summary["drafts"] = {"drafted": st.get("drafted_tokens", 0), "accepted": st.get("accepted_tokens", 0)}
     print(json.dumps({"summary": summary}))
     if a.csv:
         new = not os.path.exists(a.csv)

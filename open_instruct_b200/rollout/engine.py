@@ -10,6 +10,9 @@ Scheduling and block management are native (``ops/csrc/host/host_runtime.cpp``);
 on this package's kernels: packed varlen attention for prefill, ``b200_paged_decode`` for decode
 steps, ``b200_kv_write`` to fill cache blocks, ``b200_sample`` (Philox Gumbel-max) for sampling.
 ``ops="ref"`` keeps everything in PyTorch (CPU-testable; same cache layout and scheduler).
+
+With ``speculative_tokens`` a decode step scores a tree of drafted tokens for every sequence (``rollout/speculative.py``) and emits as
+many of them as the target's distribution confirms, plus one: the same distribution in fewer steps.
 """
 
 from __future__ import annotations
@@ -153,6 +156,7 @@ class _Sequence:
     finish_reason: str | None = None
     seed: int = 0
     last_token: int = 0
+    lookup: object = None  # index of the sequence's n-grams (speculative decoding)
 
 
 @dataclass
@@ -172,7 +176,10 @@ class RolloutEngine:
     def __init__(self, spec: ModelSpec, device="cuda", ops: str = "auto", num_blocks: int | None = None,
                  gpu_memory_utilization: float = 0.85, max_running: int = 256, max_model_len: int = 8192, seed: int = 0,
                  flat: torch.Tensor | None = None, eos_token_ids: list[int] | None = None, tokenizer=None, tp=None,
-                 enable_prefix_caching: bool = False):
+                 enable_prefix_caching: bool = False, speculative_tokens: int = 0):
+        # ``speculative_tokens``: drafted tokens per sequence and decode step (0: one token per step, as before).  Steps whose
+        # sequences all sample without a nucleus (top_p = 1) and where any has a draft are verified steps; they run eagerly, so
+        # they pay where a step is bound by the GPU (large models, long contexts).
         # ``enable_prefix_caching``: full KV blocks outlive their request and serve later requests that start with the same
         # tokens (multi-turn conversations re-submit their history; the reference reaches this through vLLM's
         # ``enable_prefix_caching``, ``open_instruct/vllm_utils.py:1057-1070``).  Without it only the ``n`` samples of one
@@ -197,6 +204,13 @@ class RolloutEngine:
         if tp is not None and (spec.post_norm or spec.num_experts):
             raise NotImplementedError("tensor-parallel engines are built for dense pre-norm blocks (a norm or a router over all heads / "
                                       "experts does not split by rank)")
+        if speculative_tokens:
+            if not 0 < speculative_tokens < 64:
+                raise ValueError(f"speculative_tokens: 1 to 63 drafted tokens a sequence (trees have 64 nodes), got {speculative_tokens}")
+            if spec.head_dim != 128 or spec.has_gdn or tp is not None or (spec.min_window and max_model_len > spec.min_window):
+                raise NotImplementedError("speculative decoding is built for attention with head_dim 128 over the whole context, one GPU per engine "
+                                          "(no gated-DeltaNet layers, no tensor parallelism, no sliding window shorter than max_model_len)")
+        self.speculative_tokens = speculative_tokens
         dtype = torch.bfloat16 if self.device.type == "cuda" else torch.float32
         self.model = LlamaModel(spec, device=self.device, dtype=dtype, ops=ops, seed=seed, flat=flat)
         if ops == "ref":
@@ -769,10 +783,15 @@ class RolloutEngine:
         return results(buf)
 
     def _decode(self, seqs: list[_Sequence]) -> None:
-        """One token for every running sequence."""
+        """One token for every running sequence; with drafts, one and as many as the target confirms."""
         s = self.spec
         dev = self.device
         B = len(seqs)
+        if self.speculative_tokens and all(q.request.sampling.top_p >= 1.0 for q in seqs):
+            drafts = [self._draft(q) for q in seqs]
+            if any(len(tokens) > 1 for tokens, _, _ in drafts):
+                self._decode_drafts(seqs, drafts)
+                return
         if self.ops == "fused":
             t0 = time.perf_counter()
             self._t_launched = None
@@ -838,3 +857,67 @@ class RolloutEngine:
         toks, lps = self._sample(logits, seqs)
         for q, t, lp in zip(seqs, toks, lps):
             self._accept(q, int(t), float(lp))
+
+    # ---- speculative decode step
+    def _draft(self, seq: _Sequence):
+        """Draft tree of one sequence: no deeper than the tokens it may still emit and the pages it holds."""
+        from .speculative import PromptLookup, draft_tree
+
+        if seq.lookup is None:
+            seq.lookup = PromptLookup()
+        n = len(seq.tokens)
+        room = min(len(self.host.blocks(seq.sid)[0]) * KV_BLOCK - n, seq.request.sampling.max_tokens - (n - seq.prompt_len) - 1, self.speculative_tokens)
+        return draft_tree(seq.tokens[-1], seq.lookup.continuations(seq.tokens, room), self.speculative_tokens)
+
+    def _decode_drafts(self, seqs: list[_Sequence], drafts: list) -> None:
+        """One pass over the draft trees of all sequences: the layers with tree attention, verification of the trees, commit of the
+        confirmed nodes' keys and values, acceptance of their tokens."""
+        import numpy as np
+
+        from .speculative import uniforms
+
+        if self.ops == "fused":
+            from ..ops import fused as f
+        else:
+            from ..ops import emulated as f
+
+        s, dev, B = self.spec, self.device, len(seqs)
+        counts = [len(tokens) for tokens, _, _ in drafts]
+        cached = np.array([len(q.tokens) - 1 for q in seqs], dtype=np.int32)  # the newest token's K/V are not in the cache yet
+        tables = [self.host.blocks(q.sid)[0] for q in seqs]
+        bt = np.zeros((B, max(len(t) for t in tables)), dtype=np.int32)
+        for b, t in enumerate(tables):
+            bt[b, : len(t)] = t
+        cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        at = np.concatenate([np.arange(c) for c in counts])
+        seeds, step = np.array([q.seed for q in seqs]), np.array([len(q.tokens) - q.prompt_len for q in seqs])
+
+        def put(a, dtype):
+            return torch.from_numpy(np.ascontiguousarray(a, dtype=dtype)).to(dev, non_blocking=True)
+
+        ids = put([t for tokens, _, _ in drafts for t in tokens], np.int64)
+        parents = put([p for _, par, _ in drafts for p in par], np.int32)
+        pos = put(np.repeat(cached, counts) + np.concatenate([d for _, _, d in drafts]), np.int64)
+        ctx, bt, cu = put(cached, np.int32), put(bt, np.int32), put(cu, np.int32)
+        u_accept = put(uniforms(np.repeat(seeds, counts), np.repeat(step, counts), at + 0x80000000), np.float32)
+        u_sample = put(uniforms(seeds, step, np.full(B, 0xFFFFFFFF)), np.float32)
+        temp = put([q.request.sampling.temperature for q in seqs], np.float32)
+        nowhere = torch.full((len(at),), -1, dtype=torch.long, device=dev)  # nothing of a draft goes to the cache
+        most, layers = max(counts), []
+
+        def attn_fn(i, qkv):
+            layers.append(qkv)
+            return f.tree_attn(qkv, self.k_cache[i], self.v_cache[i], bt, ctx, cu, parents, s.num_heads, s.num_kv_heads, s.head_dim, s.attn_scale, most)
+
+        logits = self._logits(self._layer_stack(ids, pos, nowhere, attn_fn))
+        count, tokens, path, logprobs = f.verify_tree(logits, ids, parents, cu, temp, u_accept, u_sample, most)
+        f.kv_commit_(layers, self.k_cache, self.v_cache, bt, ctx, path, s.num_heads, s.num_kv_heads, s.head_dim)
+        count, tokens, logprobs = count.tolist(), tokens.tolist(), logprobs.tolist()
+        self.stats["drafted_tokens"] = self.stats.get("drafted_tokens", 0) + len(at) - B
+        self.stats["accepted_tokens"] = self.stats.get("accepted_tokens", 0) + sum(count) - B
+        for q, n, toks, lps in zip(seqs, count, tokens, logprobs):
+            for t, lp in zip(toks[:n], lps):
+                self._accept(q, t, lp)
+                self.stats["decode_tokens"] += 1
+                if q.finish_reason is not None:
+                    break

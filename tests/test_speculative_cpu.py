@@ -162,3 +162,101 @@ def test_refusals_of_commit():
     for kw in bad:
         with pytest.raises((TypeError, ValueError)):
             emulated.kv_commit_(**_change(a, **kw))
+
+
+# ------------------------------------------------------------------------------------------------ the rollout engine
+def _engine(speculative_tokens, **kw):
+    from open_instruct_b200.models import get_spec
+    from open_instruct_b200.rollout.engine import RolloutEngine
+
+    spec = get_spec("tiny128").replace(eos_token_id=3)
+    return RolloutEngine(spec, device="cpu", ops="ref", seed=1, speculative_tokens=speculative_tokens, **kw)
+
+
+def _prompts():
+    g = torch.Generator().manual_seed(0)
+    base = torch.randint(4, 512, (40,), generator=g).tolist()
+    return [base * 3, base + base[:20], torch.randint(4, 512, (7,), generator=g).tolist()]
+
+
+def test_draft_trees():
+    from open_instruct_b200.rollout.speculative import PromptLookup, draft_tree
+
+    look = PromptLookup(2)
+    toks = [1, 2, 3, 4, 1, 2, 5, 6, 1, 2]
+    assert look.continuations(toks, 3) == [[5, 6, 1], [3, 4, 1]]
+    assert look.continuations(toks + [3], 2) == [[4, 1]] and look.continuations([9], 4) == [] and look.continuations(toks, 0) == []
+    tokens, parents, depths = draft_tree(2, [[5, 6, 1], [5, 7, 8]], 5)
+    assert tokens == [2, 5, 6, 1, 7, 8] and parents == [-1, 0, 1, 2, 1, 4] and depths == [0, 1, 2, 3, 2, 3]
+    tokens, parents, _ = draft_tree(2, [[5, 6, 1, 1, 1], [3, 4]], 3)
+    assert len(tokens) == 4 and tokens[:3] == [2, 5, 6] and tokens[3] == 3 and parents[3] == 0
+    assert draft_tree(4, [], 3) == ([4], [-1], [0])
+
+
+def test_drafting_coins_are_the_samplers_numbers():
+    """The vectorised generator is the sampler's Philox: its numbers lie half a step above these."""
+    import numpy as np
+
+    from open_instruct_b200.rollout.sampler import philox_uniform
+    from open_instruct_b200.rollout.speculative import uniforms
+
+    seeds, ctr, idx = np.array([5, 1 << 40, 12345678901]), np.array([0, 7, 100]), np.array([0x80000000, 0x80000003, 0xFFFFFFFF])
+    got = uniforms(seeds, ctr, idx)
+    want = [philox_uniform(int(s), int(c), np.array([i], dtype=np.uint32))[0] for s, c, i in zip(seeds, ctr, idx)]
+    assert np.abs(got - (np.array(want) - 0.5 / 16777216.0)).max() == 0.0 and got.dtype == np.float32
+
+
+@pytest.mark.parametrize("drafts", [1, 4, 63])
+def test_engine_with_drafts_emits_the_same_greedy_text(drafts):
+    from open_instruct_b200.data_types import SamplingConfig
+
+    cfg = SamplingConfig(temperature=0.0, max_tokens=70, n=2)
+    plain, spec = _engine(0, num_blocks=64), _engine(drafts, num_blocks=64)
+    a, b = plain.generate(_prompts(), cfg), spec.generate(_prompts(), cfg)
+    assert [r.responses for r in a] == [r.responses for r in b] and [r.finish_reasons for r in a] == [r.finish_reasons for r in b]
+    for x, y in zip(a, b):   # fp32 on both sides, other summation orders
+        for p, q in zip(x.logprobs, y.logprobs):
+            assert len(p) == len(q) and max(abs(u - v) for u, v in zip(p, q)) < 1e-3
+    assert spec.stats["accepted_tokens"] > 0 and spec.stats["steps"] < plain.stats["steps"]
+    assert spec.host.free_blocks() == 64
+
+
+def test_engine_with_drafts_samples_reproducibly_and_reports_the_targets_logprobs():
+    from open_instruct_b200.data_types import SamplingConfig
+
+    cfg = SamplingConfig(temperature=0.7, max_tokens=20, n=3, seed=11)
+    eng = _engine(6, num_blocks=64)
+    a, b = eng.generate(_prompts(), cfg), eng.generate(_prompts(), cfg)
+    assert [r.responses for r in a] == [r.responses for r in b]
+    for prompt, r in zip(_prompts(), a):
+        for text, lps in zip(r.responses, r.logprobs):
+            ids = torch.tensor(prompt + text)
+            logits = eng.model.logits(ids, torch.arange(len(ids)), torch.tensor([0, len(ids)], dtype=torch.int32)).float() / 0.7
+            want = torch.log_softmax(logits, -1)[len(prompt) - 1:-1].gather(1, ids[len(prompt):, None]).squeeze(1)
+            assert (want - torch.tensor(lps)).abs().max() < 1e-3
+
+
+def test_engine_with_drafts_under_preemption_and_with_a_nucleus():
+    from open_instruct_b200.data_types import SamplingConfig
+
+    prompts = [list(range(5, 5 + n)) * 2 for n in (50, 55, 60)]
+    cfg = SamplingConfig(temperature=0.0, max_tokens=40, n=1)
+    big, small = _engine(5, num_blocks=64), _engine(5, num_blocks=7)
+    assert [r.responses for r in big.generate(prompts, cfg)] == [r.responses for r in small.generate(prompts, cfg)]
+    assert small.host.preemptions() > 0 and small.host.free_blocks() == 7
+    nucleus = SamplingConfig(temperature=1.0, top_p=0.9, max_tokens=8, n=1, seed=3)
+    eng = _engine(5, num_blocks=64)
+    assert [r.responses for r in eng.generate(prompts, nucleus)] == [r.responses for r in _engine(0, num_blocks=64).generate(prompts, nucleus)]
+    assert "drafted_tokens" not in eng.stats
+
+
+def test_engine_refuses_drafts_it_cannot_verify():
+    from open_instruct_b200.models import get_spec
+    from open_instruct_b200.rollout.engine import RolloutEngine
+
+    with pytest.raises(ValueError):
+        _engine(64)
+    with pytest.raises(ValueError):
+        _engine(-1)
+    with pytest.raises(NotImplementedError):
+        RolloutEngine(get_spec("tiny"), device="cpu", ops="ref", num_blocks=16, speculative_tokens=4)

@@ -339,3 +339,37 @@ def test_one_speculative_step():
             pos = ctx[b] + j
             row = a["qkv"][int(path[b, j])].view(heads + 2 * kv_heads, DIM)
             assert torch.equal(k[0, int(a["block_table"][b, pos // PAGE]), :, pos % PAGE], row[heads:heads + kv_heads])
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.05, 0.8])
+def test_engine_with_drafts(temperature):
+    """The fused engine with drafted tokens: every emitted token's log-probability is the model's own (fp32 PyTorch statement on the
+    same weights; the two-layer model's bf16 activations leave its logits off by less than 0.08, the bound of the engine tests
+    without drafts), greedy tokens are within that of the largest logit, and drafts are accepted."""
+    from open_instruct_b200.data_types import SamplingConfig
+    from open_instruct_b200.models import LlamaModel, get_spec
+    from open_instruct_b200.rollout.engine import RolloutEngine
+
+    spec = get_spec("tiny128")
+    eng = RolloutEngine(spec, device="cuda", ops="fused", num_blocks=128, max_model_len=1024, seed=3, eos_token_ids=[], speculative_tokens=7)
+    g = torch.Generator().manual_seed(1)
+    base = torch.randint(4, spec.vocab_size, (50,), generator=g).tolist()
+    prompts = [base * 4, base + base[:30], torch.randint(4, spec.vocab_size, (9,), generator=g).tolist(), base[:20] * 12]
+    res = eng.generate(prompts, SamplingConfig(temperature=temperature, max_tokens=60, min_tokens=60, n=2, seed=5))
+    # at 0.8 a random model's text hardly repeats three tokens, so there is nothing to look up and nothing is drafted
+    assert eng.stats.get("accepted_tokens", 0) > 0 or temperature == 0.8
+    assert eng.host.free_blocks() == 128
+    oracle = LlamaModel(spec, device="cuda", dtype=torch.float32, ops="ref", flat=eng.model.flat.detach().float().clone())
+    t = temperature or 1.0
+    for prompt, r in zip(prompts, res):
+        for text, lps in zip(r.responses, r.logprobs):
+            assert len(text) == 60
+            ids = torch.tensor(prompt + text, device="cuda")
+            with torch.no_grad():
+                logits = oracle.logits(ids, torch.arange(len(ids), device="cuda"), torch.tensor([0, len(ids)], dtype=torch.int32, device="cuda")).float() / t
+            rows = torch.log_softmax(logits, -1)[len(prompt) - 1:-1]
+            want = rows.gather(1, ids[len(prompt):, None]).squeeze(1)
+            # a log-probability is a difference of two numbers that are logits / t: what the logits are off by counts 1 / t times
+            assert (want.cpu() - torch.tensor(lps)).abs().max() < 0.08 / min(t, 1.0)
+            if not temperature:
+                assert (rows.amax(-1) - want).max() < 0.08
