@@ -37,15 +37,19 @@ constexpr int TA_DH = 128;
 constexpr int TA_PAGE = 64;
 constexpr int TA_MAX_NODES = 64;
 constexpr int TA_THREADS = 384;          // four warps for TMA, products and planning (one idle), two groups of four for the softmax
-// Registers: 12 warps at launch have 168 a thread.  The softmax holds a row of 128 scores and spills at that; the first group
-// gives back what the other two take (56 + 2 * 224 = 3 * 168, checked against the launch).
-constexpr int TA_REGS = 168, TA_REGS_ISSUE = 56, TA_REGS_SOFTMAX = 224;
-static_assert(TA_REGS_ISSUE + 2 * TA_REGS_SOFTMAX <= 3 * TA_REGS, "the groups' shares exceed what the block is launched with");
+// Registers: 12 warps at launch have 168 a thread.  The softmax wants more, the issuing warps less (the wide kernel's four cursors
+// more than the narrow one's loop): the first group gives back what the other two take.
+constexpr int TA_REGS = 168;
+template <bool narrow>
+struct TaRegs {
+  static constexpr int issue = narrow ? 56 : 72, softmax = narrow ? 224 : 216;
+  static_assert(issue + 2 * softmax <= 3 * TA_REGS, "the groups' shares exceed what the block is launched with");
+};
 constexpr int TA_SUB = 128 * 64 * 2;     // bytes of one [128 x 64] swizzled sub-tile
 constexpr int TA_TILE = 2 * TA_SUB;      // a [128 keys or rows x 128] bf16 tile
 constexpr int TA_RING = 4;               // two tiles of keys and values in flight (a fifth buffer was measured to change nothing)
 constexpr int TA_QSUB = 32 * 64 * 2;     // a narrow unit's queries: two [32 x 64] swizzled sub-tiles
-constexpr int TA_MIN_TILES = 2;          // key tiles a CTA takes at least: below that joining the parts costs more than it saves
+constexpr int TA_MIN_WORK = 2;           // products of a key and a row tile that a CTA takes at least: below that joining the parts costs more than it saves
 constexpr float TA_LOG2E = 1.4426950408889634f;
 
 struct TreeArgs {
@@ -69,25 +73,29 @@ struct TreeArgs {
 // A sequence as the kernel sees it.  Tiles of 128 cached keys, then one tile with the tree's own keys; an odd last page shares
 // that tile with the tree (page in rows 0 .. 63, tree in rows 64 .. 127; without such a page the tree is in rows 0 .. 63).
 struct TreeSeq {
-  int n0, T, C, nt, nru;
+  int n0, T, C, nt, rts;  // first row, nodes, cached keys, key tiles, row tiles
   __device__ __forceinline__ void load(const TreeArgs& a, int b) {
     n0 = min(max(a.cu[b], 0), a.N);
     T = min(min(max(a.cu[b + 1] - n0, 0), a.max_nodes), a.N - n0);
     C = min(max(a.ctx[b], 0), a.max_blocks * TA_PAGE);
     nt = (C + TA_PAGE - 1) / TA_PAGE / 2 + 1;
-    nru = (T + 2 * a.npt - 1) / (2 * a.npt);
+    rts = (T + a.npt - 1) / a.npt;
   }
-  __device__ __forceinline__ int tiles(const TreeArgs& a) const { return a.Hkv * nru * nt; }
+  // Work in products of a key tile with a row tile: what a unit costs goes with its row tiles (2560 cycles each a key tile of the
+  // wide kernel, with two of them or one).  Shares in key tiles alone left the busiest SM of an uneven batch with 1.3 times the mean.
+  __device__ __forceinline__ int work(const TreeArgs& a) const { return a.Hkv * rts * nt; }
+  __device__ __forceinline__ int pairs() const { return (rts + 1) >> 1; }  // of row tiles: units of a KV head
 };
 
-// Even shares of `total` tiles: the first `more` CTAs take one more than the others.
+// Even shares of `total` products: the first `more` CTAs take one more than the others.  Inside a unit of two row tiles a boundary
+// is rounded down to a whole key tile.
 struct TreeShares {
   int each, more;
   __device__ __forceinline__ TreeShares(int total, int ctas) : each(total / ctas), more(total % ctas) {}
   __device__ __forceinline__ int begin(int cta) const { return each * cta + min(cta, more); }
-  __device__ __forceinline__ int owner(int tile) const {
+  __device__ __forceinline__ int owner(int at) const {
     const int low = more * (each + 1);
-    return tile < low ? tile / (each + 1) : more + (tile - low) / each;
+    return at < low ? at / (each + 1) : more + (at - low) / each;
   }
 };
 
@@ -117,7 +125,8 @@ struct TreeSmem {
   float wt[8][2][32];    // narrow units: a warp's weights of the rows, on their way from one lane to all
   uint32_t flags[2];     // narrow units: a byte for each warp of a group
   TreeSegment seg[2];
-  uint64_t q_full[2], q_empty[2], r_full[RING], r_empty[RING], s_full[2], p_full[2], o_full[2], o_free[2], seg_full[2], seg_empty[2], ml_full[2], lx_full[2], flag_full[2], mx_full[2];
+  uint64_t q_full[2], q_empty[2], r_full[RING], r_empty[RING], s_full[2][2], p_full[2][2], o_full[2], o_free[2],
+      seg_full[2], seg_empty[2], ml_full[2], lx_full[2], flag_full[2], mx_full[2];
   int scan[TA_THREADS / 32];
   TreeSeq at;            // the sequence in which the CTA's share begins
   int at_seq, at_off;
@@ -181,9 +190,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.q_full[i], 1);
-      mbar_init(&sm.q_empty[i], 1);
-      mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i], 4);
+      mbar_init(&sm.q_empty[i], narrow ? 1 : 2);  // the threads that issue products: one, or one a group
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&sm.s_full[i][j], 1);
+        mbar_init(&sm.p_full[i][j], 4);
+      }
       mbar_init(&sm.o_full[i], 1);
       mbar_init(&sm.o_free[i], 8);
       mbar_init(&sm.ml_full[i], 4);
@@ -191,11 +202,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_init(&sm.flag_full[i], 4);
       mbar_init(&sm.mx_full[i], 4);
       mbar_init(&sm.seg_full[i], 1);
-      mbar_init(&sm.seg_empty[i], 10);  // the TMA and the product threads, eight softmax warps
+      mbar_init(&sm.seg_empty[i], narrow ? 10 : 11);  // the TMA and the product threads, eight softmax warps
     }
     for (int i = 0; i < RING; ++i) {
       mbar_init(&sm.r_full[i], 1);
-      mbar_init(&sm.r_empty[i], 1);
+      mbar_init(&sm.r_empty[i], narrow ? 1 : 2);
     }
     sm.abort_flag = 0;
     fence_barrier_init();
@@ -208,7 +219,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   griddep_launch_dependents();
   griddep_wait();
 
-  // ---- this CTA's share: total number of key tiles, then the sequence in which the share begins
+  // ---- this CTA's share: the batch's work, then the sequence in which the share begins
   auto block_scan = [&](int v, int& total) {  // inclusive prefix over the block's threads
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -228,18 +239,18 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     return v + before;
   };
   TreeSeq seq;
-  auto tiles_of = [&](int b) {
+  auto work_of = [&](int b) {
     if (b >= a.B) return 0;
     seq.load(a, b);
-    return seq.tiles(a);
+    return seq.work(a);
   };
   int total = 0, chunk, mine = 0, incl = 0;
   for (int b0 = 0; b0 < a.B; b0 += TA_THREADS) {
-    mine = tiles_of(b0 + tid);
+    mine = work_of(b0 + tid);
     incl = block_scan(mine, chunk);
     total += chunk;
   }
-  const int ctas = min(static_cast<int>(gridDim.x), max(total / TA_MIN_TILES, 1)), cta = blockIdx.x;
+  const int ctas = min(static_cast<int>(gridDim.x), max(total / TA_MIN_WORK, 1)), cta = blockIdx.x;
   const TreeShares share(total, ctas);
   const int begin = share.begin(cta), end = share.begin(cta + 1);
   if (cta >= ctas || begin >= end || (smem_u32(smem_raw) & 1023u)) {
@@ -251,7 +262,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   }
   for (int b0 = 0, base = 0; b0 < a.B; b0 += TA_THREADS, base += chunk) {
     if (a.B > TA_THREADS) {  // more than one chunk: the values of this one again
-      mine = tiles_of(b0 + tid);
+      mine = work_of(b0 + tid);
       incl = block_scan(mine, chunk);
     }
     const int lo = base + incl - mine;
@@ -271,20 +282,22 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const uint32_t tmem = sm.tmem_ptr;  // S (then P) of group g at column 128 g, O of group g at 256 + 128 g
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_REGS_ISSUE));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TaRegs<narrow>::issue));
     if (warp == 2) {
       // ---- planning: the CTA's segments one or two ahead of the others, so that their loads wait for no index
       TreeSeq q = sm.at;
-      int b = sm.at_seq, left = end - begin, unit = sm.at_off / q.nt, t0 = sm.at_off % q.nt, have = -1;
+      const int head = q.rts * q.nt, in_head = sm.at_off % head;  // work of a KV head
+      int b = sm.at_seq, left = end - begin, kvh = sm.at_off / head, pair = in_head / (2 * q.nt), p0 = in_head % (2 * q.nt), have = -1;
       unsigned long long s0 = 0, s1 = 0;  // what nodes `lane` and `lane + 32` see
       bool ok = true;
+      if (lane == 0) a.joins[cta] = make_int4(0, 0, 0, 0);
       for (uint32_t n = 0; ok; ++n) {
         TreeSegment& g = sm.seg[n & 1];
         if (n >= 2) ok = ta_warp_wait(&sm.seg_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag);
         if (!ok) break;
-        const int t1 = left > 0 ? min(q.nt, t0 + left) : t0;
-        if (left > 0) {
-          const int kvh = unit / q.nru, first = unit % q.nru * 2 * a.npt;
+        const int nrt = min(2, q.rts - 2 * pair), p1 = min(q.nt * nrt, p0 + left), t0 = p0 / nrt, t1 = p1 / nrt;
+        if (t0 < t1) {  // none: the share is done, or its last product is half a tile, which the next CTA has
+          const int first = pair * 2 * a.npt;
           int blk = -1;
           if (lane < 2 && (2 * t0 + lane) * TA_PAGE < q.C) blk = a.table[b * a.table_ld + 2 * t0 + lane];
           if (have != b) {
@@ -325,15 +338,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             g.nt = q.nt;
             g.kvh = kvh;
             g.first = first;
-            g.nrt = !narrow && q.T - first > a.npt ? 2 : 1;
+            g.nrt = nrt;
             g.b = b;
-            if (left <= t1 - t0) {  // the CTA's last: a unit that begins here and goes on elsewhere is joined from its parts
-              int4 join = make_int4(0, 0, 0, 0);
-              if (t0 == 0 && t1 < q.nt) {
-                const int c = share.owner(end - t1 + q.nt - 1);  // who has the unit's last tile
-                join = make_int4(c - cta + 1, q.n0 + first, min(2 * a.npt, q.T - first), kvh);
-              }
-              a.joins[cta] = join;
+            if (t0 == 0 && t1 < q.nt) {  // a unit that begins here and goes on in the next CTAs is joined from its parts
+              const int c = share.owner(end - p1 + q.nt * nrt - 1);  // who has the unit's last product
+              a.joins[cta] = make_int4(c - cta + 1, q.n0 + first, min(2 * a.npt, q.T - first), kvh);
             }
           }
         }
@@ -344,12 +353,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.seg_full[n & 1]);
         if (t1 == t0) break;
-        left -= t1 - t0;
-        t0 = 0;
-        if (left > 0 && ++unit == a.Hkv * q.nru) {
-          unit = 0;
-          do q.load(a, ++b);
-          while (q.T == 0);
+        left -= p1 - p0;
+        p0 = 0;
+        if (left > 0 && ++pair == q.pairs()) {
+          pair = 0;
+          if (++kvh == a.Hkv) {
+            kvh = 0;
+            do q.load(a, ++b);
+            while (q.T == 0);
+          }
         }
       }
       if (!ok && lane == 0) atomicCAS(a.status, 0, ST_TIMEOUT_EMPTY);
@@ -378,15 +390,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const int s = qc & 1;
             ok = mbar_wait(&sm.q_empty[s], ((qc >> 1) & 1) ^ 1, abort_flag);
             if (!ok) break;
-            if (narrow) {
-              mbar_expect_tx(&sm.q_full[s], a.G * a.npt * 256);
-              tma_load_3d(sm.q[s], &tm_q, &sm.q_full[s], 0, kvh * a.G, q0);
-              tma_load_3d(sm.q[s] + TA_QSUB, &tm_q, &sm.q_full[s], 64, kvh * a.G, q0);
-              continue;
-            }
             mbar_expect_tx(&sm.q_full[s], a.G * a.npt * 256);
+            constexpr int right = narrow ? TA_QSUB : TA_SUB;  // where the dimensions from 64 on start
             tma_load_3d(sm.q[s], &tm_q, &sm.q_full[s], 0, kvh * a.G, q0 + rt * a.npt);
-            tma_load_3d(sm.q[s] + TA_SUB, &tm_q, &sm.q_full[s], 64, kvh * a.G, q0 + rt * a.npt);
+            tma_load_3d(sm.q[s] + right, &tm_q, &sm.q_full[s], 64, kvh * a.G, q0 + rt * a.npt);
           }
           auto page = [&](int p) {  // a page outside the cache: rows past its end, which read as zeros
             if (p * TA_PAGE >= C) return -1;
@@ -426,160 +433,239 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         }
         if (!ok) atomicCAS(a.status, 0, ST_TIMEOUT_EMPTY);
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 || (!narrow && warp == 3)) {
       if (elect_one()) {
-        constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, false, false), idesc_s64 = umma_idesc_bf16(128, 64, false, false);
-        constexpr uint32_t idesc_o = umma_idesc_bf16(128, 128, false, true);
-        constexpr uint32_t idesc_sn = umma_idesc_bf16(128, 32, false, false), idesc_on = umma_idesc_bf16(128, 32, true, true);
-        struct Job {
-          int grp, vslot;
-          uint32_t vpar;
-          bool half, wait_v, free_v, first, last, alone;
-        };
-        uint32_t jc = 0, rbase = 0, qc = 0, pc = 0;  // pc: bit g is the parity of group g's next P
-        bool ok = true;
         auto give_up = [&](int code) {
           atomicCAS(a.status, 0, code);
           return false;
         };
-        auto issue_pv = [&](const Job& j, uint32_t seg) -> bool {
-          if (!mbar_wait(&sm.p_full[j.grp], (pc >> j.grp) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
-          pc ^= 1u << j.grp;
-          if (j.wait_v && !mbar_wait(&sm.r_full[j.vslot], j.vpar, abort_flag)) return give_up(ST_TIMEOUT_FULL);
-          // a group's first product of a unit overwrites its O: the last unit's must have been read
-          // (each barrier is waited for once a segment, so that a parity always means the phase before)
-          if (j.first && seg > 0 &&
-              !(mbar_wait(&sm.o_free[j.grp], (seg - 1) & 1, abort_flag) && (!j.alone || mbar_wait(&sm.o_free[j.grp ^ 1], (seg - 1) & 1, abort_flag))))
-            return give_up(ST_TIMEOUT_TMEM_EMPTY);
-          tc_fence_after();
-          const uint32_t v = smem_u32(sm.ring[j.vslot]), p = tmem + j.grp * 128, o = tmem + 256 + j.grp * 128;
-          const int steps = j.half ? 4 : 8;
-          if (narrow) {
-            const uint32_t ps = smem_u32(sm.p[j.grp]);
-            for (int k = 0; k < steps; ++k) umma_ss(o, ta_desc_mn(v, k), ta_desc_p(ps + k * 1024), idesc_on, !(j.first && k == 0));
-          } else {
-            for (int k = 0; k < steps; ++k) umma_ts(o, p + k * 8, ta_desc_mn(v, k), idesc_o, !(j.first && k == 0));
-          }
-          if (j.free_v) umma_commit(&sm.r_empty[j.vslot]);
-          if (j.last) umma_commit(&sm.o_full[j.grp]);
-          return true;
-        };
-        Job prev;
-        bool have = false;
-        uint32_t prev_seg = 0;
-        for (uint32_t n = 0; ok; ++n) {
-          const TreeSegment& g = sm.seg[n & 1];
-          if (!mbar_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag)) {
-            ok = give_up(ST_TIMEOUT_FULL);
-            break;
-          }
-          if (g.t0 == g.t1) break;
-          const int count = g.t1 - g.t0, nrt = g.nrt, jobs = count * nrt;
-          const int half_at = g.C <= (g.nt - 1) * 128 ? g.nt - 1 - g.t0 : -1;  // the tree's tile without a page: 64 keys
-          mbar_arrive(&sm.seg_empty[n & 1]);
-          for (int x = 0; x < jobs && ok; ++x, ++jc) {
-            const int i = nrt == 2 ? x >> 1 : x, rt = nrt == 2 ? x & 1 : 0;
-            Job j;
-            j.grp = jc & 1;
-            const uint32_t kn = rbase + ring_k(i), vn = rbase + ring_v(i, count);
-            const int ks = kn % RING, qs = (qc + rt) & 1;
-            j.vslot = vn % RING;
-            j.vpar = (vn / RING) & 1;
-            j.half = i == half_at;
-            j.wait_v = rt == 0;
-            j.free_v = rt == nrt - 1;
-            j.first = x < 2;
-            j.alone = jobs == 1;
-            j.last = x >= jobs - 2;
-            if ((i == 0 && !mbar_wait(&sm.q_full[qs], ((qc + rt) >> 1) & 1, abort_flag)) ||
-                (rt == 0 && !mbar_wait(&sm.r_full[ks], (kn / RING) & 1, abort_flag))) {
+        if constexpr (narrow) {
+          // Jobs (key tiles) alternate between the groups; S of a job is issued before P V of the one before.
+          constexpr uint32_t idesc_s = umma_idesc_bf16(128, 32, false, false), idesc_o = umma_idesc_bf16(128, 32, true, true);
+          struct Job {
+            int grp, vslot;
+            uint32_t vpar;
+            bool half, first, last, alone;
+          };
+          uint32_t jc = 0, rbase = 0, qc = 0, pc = 0;  // pc: bit g is the parity of group g's next P
+          bool ok = true;
+          auto issue_pv = [&](const Job& j, uint32_t seg) -> bool {
+            if (!mbar_wait(&sm.p_full[j.grp][0], (pc >> j.grp) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
+            pc ^= 1u << j.grp;
+            if (!mbar_wait(&sm.r_full[j.vslot], j.vpar, abort_flag)) return give_up(ST_TIMEOUT_FULL);
+            // a group's first product of a unit overwrites its O: the last unit's must have been read
+            // (each barrier is waited for once a segment, so that a parity always means the phase before)
+            if (j.first && seg > 0 &&
+                !(mbar_wait(&sm.o_free[j.grp], (seg - 1) & 1, abort_flag) && (!j.alone || mbar_wait(&sm.o_free[j.grp ^ 1], (seg - 1) & 1, abort_flag))))
+              return give_up(ST_TIMEOUT_TMEM_EMPTY);
+            tc_fence_after();
+            const uint32_t v = smem_u32(sm.ring[j.vslot]), p = smem_u32(sm.p[j.grp]), o = tmem + 256 + j.grp * 128;
+            const int steps = j.half ? 4 : 8;
+            for (int k = 0; k < steps; ++k) umma_ss(o, ta_desc_mn(v, k), ta_desc_p(p + k * 1024), idesc_o, !(j.first && k == 0));
+            umma_commit(&sm.r_empty[j.vslot]);
+            if (j.last) umma_commit(&sm.o_full[j.grp]);
+            return true;
+          };
+          Job prev;
+          bool have = false;
+          uint32_t prev_seg = 0;
+          for (uint32_t n = 0; ok; ++n) {
+            const TreeSegment& g = sm.seg[n & 1];
+            if (!mbar_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag)) {
               ok = give_up(ST_TIMEOUT_FULL);
               break;
             }
-            tc_fence_after();
-            const uint32_t q = smem_u32(sm.q[qs]), kt = smem_u32(sm.ring[ks]);
-            if (narrow) {
+            if (g.t0 == g.t1) break;
+            const int count = g.t1 - g.t0;
+            const int half_at = g.C <= (g.nt - 1) * 128 ? g.nt - 1 - g.t0 : -1;  // the tree's tile without a page: 64 keys
+            mbar_arrive(&sm.seg_empty[n & 1]);
+            const int qs = qc & 1;
+            for (int x = 0; x < count && ok; ++x, ++jc) {
+              Job j;
+              j.grp = jc & 1;
+              const uint32_t kn = rbase + ring_k(x), vn = rbase + ring_v(x, count);
+              const int ks = kn % RING;
+              j.vslot = vn % RING;
+              j.vpar = (vn / RING) & 1;
+              j.half = x == half_at;
+              j.first = x < 2;
+              j.alone = count == 1;
+              j.last = x >= count - 2;
+              if ((x == 0 && !mbar_wait(&sm.q_full[qs], (qc >> 1) & 1, abort_flag)) || !mbar_wait(&sm.r_full[ks], (kn / RING) & 1, abort_flag)) {
+                ok = give_up(ST_TIMEOUT_FULL);
+                break;
+              }
+              tc_fence_after();
+              const uint32_t q = smem_u32(sm.q[qs]), kt = smem_u32(sm.ring[ks]);
               for (int k = 0; k < 8; ++k)
-                umma_ss(tmem + j.grp * 128, ta_desc_k(kt, k), umma_desc_sw128(q + (k >> 2) * TA_QSUB + (k & 3) * 32, 16, 1024), idesc_sn, k != 0);
-            } else {
-              for (int k = 0; k < 8; ++k) umma_ss(tmem + j.grp * 128, ta_desc_k(q, k), ta_desc_k(kt, k), j.half ? idesc_s64 : idesc_s, k != 0);
+                umma_ss(tmem + j.grp * 128, ta_desc_k(kt, k), umma_desc_sw128(q + (k >> 2) * TA_QSUB + (k & 3) * 32, 16, 1024), idesc_s, k != 0);
+              umma_commit(&sm.r_empty[ks]);
+              if (x == count - 1) umma_commit(&sm.q_empty[qs]);
+              umma_commit(&sm.s_full[j.grp][0]);
+              if (have) ok = issue_pv(prev, prev_seg);
+              prev = j;
+              prev_seg = n;
+              have = true;
             }
-            if (rt == nrt - 1) umma_commit(&sm.r_empty[ks]);
-            if (i == count - 1) umma_commit(&sm.q_empty[qs]);
-            umma_commit(&sm.s_full[j.grp]);
-            if (have) ok = issue_pv(prev, prev_seg);
-            prev = j;
-            prev_seg = n;
-            have = true;
+            rbase += 2 * count;
+            ++qc;
           }
-          rbase += 2 * count;
-          qc += nrt;
+          if (ok && have) issue_pv(prev, prev_seg);
+        } else {
+          // Each group has a thread of its own here and steps of 64 keys: with two row tiles the halves of all key tiles in turn, with
+          // one row tile its half of each.  S has two buffers of 64 columns, so S of a step is issued while the softmax still works
+          // on the step before, and the groups do not wait for one another.  Both threads give back every load, used or not.
+          constexpr uint32_t idesc_s = umma_idesc_bf16(128, 64, false, false), idesc_o = umma_idesc_bf16(128, 128, false, true);
+          const int grp = warp >> 1;
+          const uint32_t t_s = tmem + grp * 128, t_o = tmem + 256 + grp * 128;
+          uint32_t rbase = 0, qc = 0, steps_s = 0, steps_o = 0;  // loads and row tiles so far; S and P V issued
+          struct Step {
+            uint32_t v;  // load
+            int h;
+            bool first, last;  // of the segment; of this V
+          } prev{0u, 0, false, false};
+          bool have = false, ok = true;
+          uint32_t prev_seg = 0;
+          auto loaded = [&](uint32_t load) { return mbar_wait(&sm.r_full[load % RING], (load / RING) & 1, abort_flag) || give_up(ST_TIMEOUT_FULL); };
+          auto issue_pv = [&]() -> bool {
+            const int b = steps_o & 1;
+            if (!mbar_wait(&sm.p_full[grp][b], (steps_o >> 1) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
+            if (!loaded(prev.v)) return false;
+            // the first product of a unit overwrites O: the last unit's must have been read
+            if (prev.first && prev_seg > 0 && !mbar_wait(&sm.o_free[grp], (prev_seg - 1) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
+            tc_fence_after();
+            const uint32_t v = smem_u32(sm.ring[prev.v % RING]) + prev.h * (TA_SUB / 2), p = t_s + b * 64;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_ts(t_o, p + k * 8, ta_desc_mn(v, k), idesc_o, !(prev.first && k == 0));
+            if (prev.last) umma_commit(&sm.r_empty[prev.v % RING]);
+            umma_commit(&sm.o_full[grp]);  // of every step: the softmax rescales O between them
+            ++steps_o;
+            have = false;
+            return true;
+          };
+          for (uint32_t n = 0; ok; ++n) {
+            const TreeSegment& g = sm.seg[n & 1];
+            if (!mbar_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag)) {
+              ok = give_up(ST_TIMEOUT_FULL);
+              break;
+            }
+            if (g.t0 == g.t1) break;
+            const int count = g.t1 - g.t0, tail = (g.C >> 7) - g.t0;  // from tile `tail` on the softmax may clear rows of V
+            const bool two = g.nrt == 2, half_last = g.t1 == g.nt && g.C <= (g.nt - 1) * 128;
+            mbar_arrive(&sm.seg_empty[n & 1]);
+            const bool skips = !two && grp == 1 && half_last;  // the last tile has no half for this group
+            const int steps = two ? 2 * count - half_last : count - skips;
+            for (int rt = 0; rt <= two && ok; ++rt)
+              if (!mbar_wait(&sm.q_full[(qc + rt) & 1], ((qc + rt) >> 1) & 1, abort_flag)) ok = give_up(ST_TIMEOUT_FULL);
+            const int qs = (qc + (two ? grp : 0)) & 1;
+            const uint32_t q = smem_u32(sm.q[qs]);
+            for (int u = 0; u < steps && ok; ++u) {
+              const int i = two ? u >> 1 : u, h = two ? u & 1 : grp;
+              const uint32_t kn = rbase + ring_k(i), vn = rbase + ring_v(i, count);
+              ok = loaded(kn) && (i < tail || loaded(vn));  // the softmax's own wait for V then cannot mean an older load
+              if (!ok) break;
+              const bool last = !two || h == 1 || (half_last && i == count - 1);
+              tc_fence_after();
+              const uint32_t kt = smem_u32(sm.ring[kn % RING]) + h * (TA_SUB / 2);
+              const int b = steps_s++ & 1;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) umma_ss(t_s + b * 64, ta_desc_k(q, k), ta_desc_k(kt, k), idesc_s, k != 0);
+              umma_commit(&sm.s_full[grp][b]);
+              if (last) umma_commit(&sm.r_empty[kn % RING]);
+              if (u == steps - 1) umma_commit(&sm.q_empty[qs]);
+              if (have) ok = issue_pv();
+              prev = Step{vn, h, u == 0, last};
+              prev_seg = n;
+              have = true;
+            }
+            if (!ok) break;
+            if (two) mbar_arrive(&sm.q_empty[qs ^ 1]);  // filled, and not used here
+            if (skips) {
+              if (have) ok = issue_pv();
+              if (steps == 0) mbar_arrive(&sm.q_empty[qs]);
+              const uint32_t kn = rbase + ring_k(count - 1), vn = rbase + ring_v(count - 1, count);
+              ok = ok && loaded(kn);
+              if (ok) mbar_arrive(&sm.r_empty[kn % RING]);
+              ok = ok && loaded(vn);
+              if (ok) mbar_arrive(&sm.r_empty[vn % RING]);
+            }
+            rbase += 2 * count;
+            qc += two ? 2 : 1;
+          }
+          if (ok && have) issue_pv();
         }
-        if (ok && have) issue_pv(prev, prev_seg);
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TA_REGS_SOFTMAX));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TaRegs<narrow>::softmax));
     const int grp = (warp - 4) >> 2, lg = warp & 3, r = lg * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(lg * 32) << 16;
     const uint32_t t_s = tmem + grp * 128 + lane_off, t_o = tmem + 256 + lane_off;
     const float c = a.scale * TA_LOG2E;
-    uint32_t jc = 0, rbase = 0;
-    uint32_t par_s = 0, par_o = 0, par_ml = 0, par_flag = 0, par_mx = 0, par_lx = 0;  // parities of the next S, of either group's O (bits 0, 1), of exchanges
-    bool late = false;                            // this group's last O was somebody else's to wait for
-    const int rn = r / a.G, rg = r - rn * a.G;                // node of the row tile and head of the group
-    const int rn32 = lane / a.G, rg32 = lane - rn32 * a.G;  // the same in a narrow unit
+    uint32_t rbase = 0;
     bool ok = true;
-    for (uint32_t n = 0; ok; ++n) {
-      const TreeSegment& g = sm.seg[n & 1];
-      ok = ta_warp_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
-      if (!ok || g.t0 == g.t1) break;
-      const int t0 = g.t0, count = g.t1 - t0, nt = g.nt, nrt = narrow ? 1 : g.nrt, T = g.T, C = g.C, jobs = count * nrt;
-      const int x0 = (grp ^ jc) & 1;           // my first job of this segment; then every second one
-      const int rt = nrt == 2 ? x0 : 0, node = narrow ? rn32 : g.first + rt * a.npt + rn;  // of this thread's row (narrow: of row `lane`)
-      const bool valid = (narrow || rn < a.npt) && node < T;
-      const unsigned long long sees = valid ? g.sees[node] : 0ull;
-      const long long seg_at = (static_cast<long long>(g.n0) * a.Hq + g.kvh * a.G) * TA_DH;  // the sequence's first row in the result
-      const long long out_at = seg_at + (static_cast<long long>(node) * a.Hq + (narrow ? rg32 : rg)) * TA_DH;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.seg_empty[n & 1]);
-      const bool busy = __any_sync(0xffffffffu, valid);
-      float m = narrow ? 0.f : -INFINITY, l = 0.f;
-      // The scores of tile i are there: its keys (as many as 128, fewer in the last tiles) and whether it is the tree's without a
-      // page.  Rows of V that hold no key are cleared: 0 * NaN must not reach the output.
-      auto begin_job = [&](int i, int& keys, bool& half) -> bool {
-        if (!ta_warp_wait(&sm.s_full[grp], par_s, abort_flag)) return false;
-        par_s ^= 1;
-        if (late) {  // complete since this S was issued behind it: keeps the parity in step
-          if (!ta_warp_wait(&sm.o_full[grp], (par_o >> grp & 1) ^ 1, abort_flag)) return false;
-          late = false;
-        }
-        tc_fence_after();
-        const int t = t0 + i;
-        keys = min(128, C - t * 128);
-        half = t == nt - 1 && keys <= 0;
-        if (rt > 0 || (t < nt - 1 && keys == 128)) return true;
-        int z0 = keys, z1 = 128, z2 = 128, z3 = 128;  // rows [z0, z1) and [z2, z3) of V are empty
-        if (t == nt - 1) {
-          z0 = max(keys, 0);
-          z1 = half ? 0 : 64;
-          z2 = z1 + T;
-          z3 = z1 + 64;
-        }
-        const uint32_t vn = rbase + ring_v(i, count);
-        if (!ta_warp_wait(&sm.r_full[vn % RING], (vn / RING) & 1, abort_flag)) return false;
-        if ((r >= z0 && r < z1) || (r >= z2 && r < z3)) {
-          uint4* row = reinterpret_cast<uint4*>(sm.ring[vn % RING] + r * 128);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int at = (q + lane) & 7;  // neighbouring rows start in different banks
-            row[at] = row[at + TA_SUB / 16] = make_uint4(0u, 0u, 0u, 0u);
+    // the last segment's end is over on both sides, what it left behind has been read.  Every warp waits for that in every
+    // segment and says when it is through with this one, so no barrier is more than one phase away from a parity that is waited for.
+    auto last_end = [&](uint32_t n) {
+      return n == 0 || (ta_warp_wait(&sm.o_free[0], (n - 1) & 1, abort_flag) && ta_warp_wait(&sm.o_free[1], (n - 1) & 1, abort_flag));
+    };
+    auto through = [&] {
+      if (lane == 0) {
+        mbar_arrive(&sm.o_free[0]);
+        mbar_arrive(&sm.o_free[1]);
+      }
+    };
+    if constexpr (narrow) {
+      uint32_t jc = 0;
+      uint32_t par_s = 0, par_o = 0, par_ml = 0, par_flag = 0, par_mx = 0, par_lx = 0;  // parities of the next S, of either group's O (bits 0, 1), of exchanges
+      bool late = false;                            // this group's last O was somebody else's to wait for
+      const int rn = lane / a.G, rg = lane - rn * a.G;  // node and head of row `lane`
+      for (uint32_t n = 0; ok; ++n) {
+        const TreeSegment& g = sm.seg[n & 1];
+        ok = ta_warp_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
+        if (!ok || g.t0 == g.t1) break;
+        const int t0 = g.t0, count = g.t1 - t0, nt = g.nt, T = g.T, C = g.C, jobs = count;
+        const int x0 = (grp ^ jc) & 1;           // my first job of this segment; then every second one
+        const bool valid = rn < T;
+        const unsigned long long sees = valid ? g.sees[rn] : 0ull;
+        const long long seg_at = (static_cast<long long>(g.n0) * a.Hq + g.kvh * a.G) * TA_DH;  // the sequence's first row in the result
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.seg_empty[n & 1]);
+        float m = 0.f, l = 0.f;
+        // The scores of tile x are there: its keys (as many as 128, fewer in the last tiles) and whether it is the tree's without a
+        // page.  Rows of V that hold no key are cleared: 0 * NaN must not reach the output.
+        auto begin_job = [&](int x, int& keys, bool& half) -> bool {
+          if (!ta_warp_wait(&sm.s_full[grp][0], par_s, abort_flag)) return false;
+          par_s ^= 1;
+          if (late) {  // complete since this S was issued behind it: keeps the parity in step
+            if (!ta_warp_wait(&sm.o_full[grp], (par_o >> grp & 1) ^ 1, abort_flag)) return false;
+            late = false;
           }
-        }
-        fence_proxy_async();
-        return true;
-      };
-      if constexpr (narrow) {
+          tc_fence_after();
+          const int t = t0 + x;
+          keys = min(128, C - t * 128);
+          half = t == nt - 1 && keys <= 0;
+          if (t < nt - 1 && keys == 128) return true;
+          int z0 = keys, z1 = 128, z2 = 128, z3 = 128;  // rows [z0, z1) and [z2, z3) of V are empty
+          if (t == nt - 1) {
+            z0 = max(keys, 0);
+            z1 = half ? 0 : 64;
+            z2 = z1 + T;
+            z3 = z1 + 64;
+          }
+          const uint32_t vn = rbase + ring_v(x, count);
+          if (!ta_warp_wait(&sm.r_full[vn % RING], (vn / RING) & 1, abort_flag)) return false;
+          if ((r >= z0 && r < z1) || (r >= z2 && r < z3)) {
+            uint4* row = reinterpret_cast<uint4*>(sm.ring[vn % RING] + r * 128);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const int at = (q + lane) & 7;  // neighbouring rows start in different banks
+              row[at] = row[at + TA_SUB / 16] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async();
+          return true;
+        };
         uint64_t nm[16], ln[16];  // reference points (negated) and sums of the 32 rows, this thread's keys
 #pragma unroll
         for (int e = 0; e < 16; ++e) nm[e] = ln[e] = 0ull;
@@ -704,7 +790,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           fence_proxy_async();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.p_full[grp]);
+          if (lane == 0) mbar_arrive(&sm.p_full[grp][0]);
         }
         if (!ok) break;
         // 32 sums over the warp's keys: halve the rows and the lanes that share them, until lane i has row i
@@ -721,170 +807,41 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           }
         }
         l = sees ? v[0] : 0.f;
-      } else {
-        for (int x = x0; x < jobs; x += 2) {
-          const int i = nrt == 2 ? x >> 1 : x, t = t0 + i;
-          int keys;
-          bool half;
-          ok = begin_job(i, keys, half);
-          if (!ok) break;
-          unsigned long long lo = ~0ull, hi = ~0ull;  // keys of this tile that the row sees
-          if (t == nt - 1) {
-            lo = half ? sees : low_bits(keys);
-            hi = half ? 0ull : sees;
-          } else if (keys < 128) {
-            lo = low_bits(keys);
-            hi = low_bits(max(keys - 64, 0));
-          }
-          if (busy) {
-            uint32_t sv[4][32];
-            tmem_ld32(t_s, sv[0]);
-            tmem_ld32(t_s + 32, sv[1]);
-            if (!half) {
-              tmem_ld32(t_s + 64, sv[2]);
-              tmem_ld32(t_s + 96, sv[3]);
-            }
-            tmem_ld_wait();
-            const bool masked = (lo & hi) != ~0ull;
-            if (masked) {
-              const uint32_t words[4] = {static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
-                                         static_cast<uint32_t>(hi >> 32)};
-#pragma unroll
-              for (int cc = 0; cc < 4; ++cc)
-                if (cc < 2 || !half) {
-#pragma unroll
-                  for (int e = 0; e < 32; ++e)
-                    if (!((words[cc] >> e) & 1u)) sv[cc][e] = 0xff800000u;
-                }
-            }
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int cc = 0; cc < 4; ++cc)
-              if (cc < 2 || !half) {
-#pragma unroll
-                for (int e = 0; e < 32; e += 2)
-                  mx4[e / 2 & 3] = max3(mx4[e / 2 & 3], __uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1]));
-              }
-            const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
-            float alpha = 1.f;
-            const bool grow = (mx - m) * c > 8.f;
-            if (grow) {
-              alpha = ex2_approx((m - mx) * c);
-              m = mx;
-              l *= alpha;
-            }
-            const uint64_t c2 = pair2(c, c), mc2 = pair2(-m * c, -m * c);
-            uint64_t sum[2] = {0ull, 0ull};  // two pairs of zeros
-#pragma unroll
-            for (int cc = 0; cc < 4; ++cc) {
-              if (cc < 2 || !half) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                  const uint64_t x = fma2(pair2(__uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1])), c2, mc2);
-                  float p0, p1;
-                  unpair2(x, p0, p1);
-                  p0 = ex2_approx(p0);
-                  p1 = ex2_approx(p1);
-                  sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair2(p0, p1));
-                  pk[e >> 1] = pack_bf16x2(p0, p1);
-                }
-                tmem_st16(t_s + cc * 16, pk);
-              }
-            }
-            {
-              float s0, s1;
-              unpair2(add2(sum[0], sum[1]), s0, s1);
-              l += s0 + s1;
-            }
-            // S of this job was issued after every earlier P V of this group, so O is at rest here
-            if (x >= 2 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll
-              for (int cc = 0; cc < 4; ++cc) {
-                uint32_t o[32];
-                tmem_ld32(t_o + grp * 128 + cc * 32, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                tmem_st32(t_o + grp * 128 + cc * 32, o);
-              }
-            }
-            tmem_st_wait();
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.p_full[grp]);
-        }
-        if (!ok) break;
-        if (!sees) {
-          m = -INFINITY;
-          l = 0.f;
-        }
-        m *= c;  // base-2 scale from here on
-      }
 
-      // ---- end of the segment: the result or a part of it.  Two row tiles: each group writes its own.  One: the group of the last
-      // job joins both, the other hands over its maxima and sums and goes on with the next unit.
-      const int last = (jc + jobs - 1) & 1;
-      const bool both = nrt == 1 && jobs > 1;
-      jc += jobs;
-      rbase += 2 * count;
-      float a0 = 1.f, a1 = 0.f;  // weights of my own O and of the other group's
-      // Every warp waits for the end of the last segment and says when it is through with this one, so no barrier is ever more than
-      // one phase away from a parity that somebody waits for.
-      if (n > 0) {
-        ok = ta_warp_wait(&sm.o_free[0], (n - 1) & 1, abort_flag) && ta_warp_wait(&sm.o_free[1], (n - 1) & 1, abort_flag);
+        // ---- end of the segment: the group of the last job joins both and writes, the other hands over its maxima and sums and goes on
+        const int last = (jc + jobs - 1) & 1;
+        const bool both = jobs > 1;
+        jc += jobs;
+        rbase += 2 * count;
+        ok = last_end(n);
         if (!ok) break;
-      }
-      if (nrt == 2) {
-        if (lane == 0) mbar_arrive(&sm.o_free[grp ^ 1]);
-        ok = ta_warp_wait(&sm.o_full[grp], par_o >> grp & 1, abort_flag);
-        par_o ^= 3;
-        if (!ok) break;
-      } else if (grp != last) {
-        if (both) {
-          if (narrow) {
+        if (grp != last) {
+          if (both) {
             sm.ls[grp][lg][lane] = l;
             sm.lm[grp][lane] = m;
-          } else {
-            sm.ml[r] = l;
-            sm.ml[128 + r] = m;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.ml_full[grp]);
+            late = true;
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.ml_full[grp]);
-          late = true;
+          through();
+          par_o ^= both ? 3 : 1 << last;
+          continue;
         }
-        if (lane == 0) {
-          mbar_arrive(&sm.o_free[0]);
-          mbar_arrive(&sm.o_free[1]);
-        }
-        par_o ^= both ? 3 : 1 << last;
-        continue;
-      } else {
-        float m_other = 0.f, l_other = 0.f;
-        if (narrow) {
-          sm.ls[grp][lg][lane] = l;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.lx_full[grp]);
-          ok = ta_warp_wait(&sm.lx_full[grp], par_lx, abort_flag);
-          par_lx ^= 1;
-          if (!ok) break;
-          l = (sm.ls[grp][0][lane] + sm.ls[grp][1][lane]) + (sm.ls[grp][2][lane] + sm.ls[grp][3][lane]);
-        }
+        float a0 = 1.f, a1 = 0.f;  // weights of my own O and of the other group's
+        sm.ls[grp][lg][lane] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.lx_full[grp]);
+        ok = ta_warp_wait(&sm.lx_full[grp], par_lx, abort_flag);
+        par_lx ^= 1;
+        if (!ok) break;
+        l = (sm.ls[grp][0][lane] + sm.ls[grp][1][lane]) + (sm.ls[grp][2][lane] + sm.ls[grp][3][lane]);
         if (both) {
           ok = ta_warp_wait(&sm.ml_full[grp ^ 1], par_ml, abort_flag);
           par_ml ^= 1;
           if (ok) ok = ta_warp_wait(&sm.o_full[grp ^ 1], par_o >> (grp ^ 1) & 1, abort_flag);
           if (!ok) break;
-          if (narrow) {
-            const float* o = &sm.ls[grp ^ 1][0][lane];
-            l_other = (o[0] + o[32]) + (o[64] + o[96]);
-            m_other = sm.lm[grp ^ 1][lane];
-          } else {
-            l_other = sm.ml[r];
-            m_other = sm.ml[128 + r];
-          }
-          const float top = fmaxf(m, m_other);
+          const float* o = &sm.ls[grp ^ 1][0][lane];
+          const float l_other = (o[0] + o[32]) + (o[64] + o[96]), m_other = sm.lm[grp ^ 1][lane], top = fmaxf(m, m_other);
           a0 = l != 0.f ? ex2_approx(m - top) : 0.f;
           a1 = l_other != 0.f ? ex2_approx(m_other - top) : 0.f;
           l = a0 * l + a1 * l_other;
@@ -893,20 +850,18 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         ok = ta_warp_wait(&sm.o_full[grp], par_o >> grp & 1, abort_flag);
         par_o ^= both ? 3 : 1 << grp;
         if (!ok) break;
-      }
-      tc_fence_after();
-      const bool whole = t0 == 0 && count == nt;
-      const long long part = (static_cast<long long>(cta) * 2 + (t0 == 0 ? 1 : 0)) * a.part_rows + rt * 128 + (narrow ? lane : r);
-      if constexpr (narrow) {
+        tc_fence_after();
+        const bool whole = t0 == 0 && count == nt;
+        const long long part = (static_cast<long long>(cta) * 2 + (t0 == 0 ? 1 : 0)) * a.part_rows + lane;
         // O^T: a thread has one dimension (r) of all 32 rows; the rows' weights come from the lanes that hold them
         const float inv = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;  // an empty row gives zeros, a NaN stays one
         sm.wt[warp - 4][0][lane] = a0 * inv;
         sm.wt[warp - 4][1][lane] = a1 * inv;
         if (!whole && valid && lg == 0) a.part_ml[part] = make_float2(m, l);
-        const int to = valid ? static_cast<int>(out_at - seg_at) : -1;
-        uint32_t v[32], u[32];
-        tmem_ld32(t_o + grp * 128, v);
-        if (both) tmem_ld32(t_o + (grp ^ 1) * 128, u);
+        const int to = valid ? (rn * a.Hq + rg) * TA_DH : -1;
+        uint32_t o0[32], o1[32];
+        tmem_ld32(t_o + grp * 128, o0);
+        if (both) tmem_ld32(t_o + (grp ^ 1) * 128, o1);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
@@ -914,22 +869,19 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 w = *reinterpret_cast<const float4*>(&sm.wt[warp - 4][0][e]), z = *reinterpret_cast<const float4*>(&sm.wt[warp - 4][1][e]);
-          f[e] = w.x * __uint_as_float(v[e]);
-          f[e + 1] = w.y * __uint_as_float(v[e + 1]);
-          f[e + 2] = w.z * __uint_as_float(v[e + 2]);
-          f[e + 3] = w.w * __uint_as_float(v[e + 3]);
+          f[e] = w.x * __uint_as_float(o0[e]);
+          f[e + 1] = w.y * __uint_as_float(o0[e + 1]);
+          f[e + 2] = w.z * __uint_as_float(o0[e + 2]);
+          f[e + 3] = w.w * __uint_as_float(o0[e + 3]);
           if (both) {
-            f[e] = fmaf(z.x, __uint_as_float(u[e]), f[e]);
-            f[e + 1] = fmaf(z.y, __uint_as_float(u[e + 1]), f[e + 1]);
-            f[e + 2] = fmaf(z.z, __uint_as_float(u[e + 2]), f[e + 2]);
-            f[e + 3] = fmaf(z.w, __uint_as_float(u[e + 3]), f[e + 3]);
+            f[e] = fmaf(z.x, __uint_as_float(o1[e]), f[e]);
+            f[e + 1] = fmaf(z.y, __uint_as_float(o1[e + 1]), f[e + 1]);
+            f[e + 2] = fmaf(z.z, __uint_as_float(o1[e + 2]), f[e + 2]);
+            f[e + 3] = fmaf(z.w, __uint_as_float(o1[e + 3]), f[e + 3]);
           }
         }
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sm.o_free[0]);
-          mbar_arrive(&sm.o_free[1]);
-        }
+        through();
         const int rows = T * a.G;
         if (whole) {
           __nv_bfloat16* dst = a.out + seg_at + (r & ~1);  // two neighbouring dimensions of every second row
@@ -947,52 +899,209 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           for (int e = 0; e < 32; ++e)
             if (e < rows) dst[e * TA_DH] = f[e];
         }
-        continue;
       }
-      if (whole) {  // a row that sees nothing gives zeros (below), a NaN stays one
-        a0 *= 1.f / l;
-        a1 *= 1.f / l;
-      }
-      const uint64_t w0 = pair2(a0, a0), w1 = pair2(a1, a1);
-      if (busy) {
+    } else {
+      uint32_t mine = 0, other = 0, par_ml = 0;  // steps of this group and of the other one before this segment
+      const int rn = r / a.G, rg = r - rn * a.G;  // node of the row tile and head of the group
+      for (uint32_t n = 0; ok; ++n) {
+        const TreeSegment& g = sm.seg[n & 1];
+        ok = ta_warp_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
+        if (!ok || g.t0 == g.t1) break;
+        const int t0 = g.t0, count = g.t1 - t0, nt = g.nt, T = g.T, C = g.C;
+        const bool two = g.nrt == 2, half_last = t0 + count == nt && C <= (nt - 1) * 128;
+        const int all = two ? 2 * count - half_last : count;                  // steps of group 0 in this segment
+        const int steps = two || grp == 0 ? all : all - half_last, others = two || grp == 1 ? all : all - half_last;
+        const int rt = two ? grp : 0, node = g.first + rt * a.npt + rn;
+        const bool valid = rn < a.npt && node < T;
+        const unsigned long long sees = valid ? g.sees[node] : 0ull;
+        const long long out_at = ((static_cast<long long>(g.n0) + node) * a.Hq + g.kvh * a.G + rg) * TA_DH;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.seg_empty[n & 1]);
+        const bool busy = __any_sync(0xffffffffu, valid);
+        float m = -INFINITY, l = 0.f;
+        for (int u = 0; u < steps; ++u) {
+          const uint32_t U = mine + u;
+          const int b = U & 1, i = two ? u >> 1 : u, h = two ? u & 1 : grp, t = t0 + i;
+          ok = ta_warp_wait(&sm.s_full[grp][b], (U >> 1) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          // the keys of this half: as many as 64 cached ones, or the tree's
+          const int keys = min(64, C - t * 128 - h * 64);
+          const bool tree = t == nt - 1 && (h == 1 || keys <= 0);
+          const unsigned long long live = tree ? sees : low_bits(max(keys, 0));
+          const int filled = tree ? T : keys;
+          if (filled < 64) {  // rows of V that hold no key are cleared (by either group: the same zeros): 0 * NaN must not reach the output
+            const uint32_t vn = rbase + ring_v(i, count);
+            ok = ta_warp_wait(&sm.r_full[vn % RING], (vn / RING) & 1, abort_flag);
+            if (!ok) break;
+            if ((r & 63) >= filled) {
+              uint4* row = reinterpret_cast<uint4*>(sm.ring[vn % RING] + (r >> 6) * TA_SUB + (h * 64 + (r & 63)) * 128);
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-          uint32_t v[32], u[32];
-          tmem_ld32(t_o + grp * 128 + cc * 32, v);
-          if (both) tmem_ld32(t_o + (grp ^ 1) * 128 + cc * 32, u);
-          tmem_ld_wait();
-          float f[32];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            uint64_t y = mul2(pair2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), w0);
-            if (both) y = fma2(pair2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), w1, y);
-            unpair2(y, f[e], f[e + 1]);
-          }
-          if (whole) {
-            if (valid) {
-              uint4* dst = reinterpret_cast<uint4*>(a.out + out_at + cc * 32);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint4 y = make_uint4(pack_bf16x2(f[8 * e], f[8 * e + 1]), pack_bf16x2(f[8 * e + 2], f[8 * e + 3]),
-                                           pack_bf16x2(f[8 * e + 4], f[8 * e + 5]), pack_bf16x2(f[8 * e + 6], f[8 * e + 7]));
-                dst[e] = sees ? y : make_uint4(0u, 0u, 0u, 0u);
-              }
+              for (int q = 0; q < 8; ++q) row[(q + lane) & 7] = make_uint4(0u, 0u, 0u, 0u);  // neighbouring rows start in different banks
             }
-          } else if (valid) {
-            float4* dst = reinterpret_cast<float4*>(a.part_o + part * TA_DH + cc * 32);
+            fence_proxy_async();
+          }
+          float alpha = 1.f;
+          bool grow = false;
+          if (busy) {
+            const uint32_t ts = t_s + b * 64;
+            uint32_t sv[2][32];
+            tmem_ld32(ts, sv[0]);
+            tmem_ld32(ts + 32, sv[1]);
+            tmem_ld_wait();
+            if (__any_sync(0xffffffffu, live != ~0ull)) {
+              const uint32_t words[2] = {static_cast<uint32_t>(live), static_cast<uint32_t>(live >> 32)};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+              for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (!((words[cc] >> e) & 1u)) sv[cc][e] = 0xff800000u;
+            }
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) mx4[e / 2 & 3] = max3(mx4[e / 2 & 3], __uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1]));
+            const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
+            grow = (mx - m) * c > 8.f;
+            if (grow) {
+              alpha = ex2_approx((m - mx) * c);
+              m = mx;
+              l *= alpha;
+            }
+            const uint64_t c2 = pair2(c, c), mc2 = pair2(-m * c, -m * c);
+            uint64_t sum[2] = {0ull, 0ull};  // two pairs of zeros
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                float p0, p1;
+                unpair2(fma2(pair2(__uint_as_float(sv[cc][e]), __uint_as_float(sv[cc][e + 1])), c2, mc2), p0, p1);
+                p0 = ex2_approx(p0);
+                p1 = ex2_approx(p1);
+                sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair2(p0, p1));
+                pk[e >> 1] = pack_bf16x2(p0, p1);
+              }
+              tmem_st16(ts + cc * 16, pk);
+            }
+            float s0, s1;
+            unpair2(add2(sum[0], sum[1]), s0, s1);
+            l += s0 + s1;
+          }
+          // The product of the step before is waited for where O is to be rescaled, and in the last step: from there on the parity of
+          // the last product's phase can only mean that one.
+          const bool rescale = u > 0 && __any_sync(0xffffffffu, grow);
+          if (U > 0 && (rescale || u == steps - 1)) {
+            ok = ta_warp_wait(&sm.o_full[grp], (U - 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          if (rescale) {
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) {
+              uint32_t o[32];
+              tmem_ld32(t_o + grp * 128 + cc * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st32(t_o + grp * 128 + cc * 32, o);
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full[grp][b]);
+        }
+        if (!ok) break;
+        if (!sees) {
+          m = -INFINITY;
+          l = 0.f;
+        }
+        m *= c;  // base-2 scale from here on
+
+        // ---- end of the segment: the result or a part of it.  Two row tiles: each group writes its own.  One: the group of the last
+        // step joins both, the other hands over its maxima and sums and goes on with the next unit.
+        const uint32_t my_last = mine + steps - 1, their_last = other + others - 1;
+        const bool both = !two && steps > 0 && others > 0;
+        const int last = both ? !half_last : 0;
+        mine += steps;
+        other += others;
+        rbase += 2 * count;
+        ok = last_end(n);
+        if (!ok) break;
+        float a0 = 1.f, a1 = 0.f;  // weights of my own O and of the other group's
+        if (two) {
+          if (lane == 0) mbar_arrive(&sm.o_free[grp ^ 1]);
+        } else if (grp != last) {
+          if (both) {
+            sm.ml[r] = l;
+            sm.ml[128 + r] = m;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.ml_full[grp]);
+          }
+          through();
+          continue;
+        } else if (both) {
+          ok = ta_warp_wait(&sm.ml_full[grp ^ 1], par_ml >> (grp ^ 1) & 1, abort_flag) && ta_warp_wait(&sm.o_full[grp ^ 1], their_last & 1, abort_flag);
+          par_ml ^= 1u << (grp ^ 1);
+          if (!ok) break;
+          const float l_other = sm.ml[r], m_other = sm.ml[128 + r], top = fmaxf(m, m_other);
+          a0 = l != 0.f ? ex2_approx(m - top) : 0.f;
+          a1 = l_other != 0.f ? ex2_approx(m_other - top) : 0.f;
+          l = a0 * l + a1 * l_other;
+          m = top;
+        }
+        ok = steps == 0 || ta_warp_wait(&sm.o_full[grp], my_last & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const bool whole = t0 == 0 && count == nt;
+        const long long part = (static_cast<long long>(cta) * 2 + (t0 == 0 ? 1 : 0)) * a.part_rows + rt * 128 + r;
+        if (whole) {  // a row that sees nothing gives zeros (below), a NaN stays one
+          a0 *= 1.f / l;
+          a1 *= 1.f / l;
+        }
+        const uint64_t w0 = pair2(a0, a0), w1 = pair2(a1, a1);
+        if (busy) {
+#pragma unroll
+          for (int cc = 0; cc < 4; ++cc) {
+            uint32_t v[32], u[32];
+            tmem_ld32(t_o + grp * 128 + cc * 32, v);
+            if (both) tmem_ld32(t_o + (grp ^ 1) * 128 + cc * 32, u);
+            tmem_ld_wait();
+            float f[32];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              uint64_t y = mul2(pair2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), w0);
+              if (both) y = fma2(pair2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), w1, y);
+              unpair2(y, f[e], f[e + 1]);
+            }
+            if (whole) {
+              if (valid) {
+                uint4* dst = reinterpret_cast<uint4*>(a.out + out_at + cc * 32);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint4 y = make_uint4(pack_bf16x2(f[8 * e], f[8 * e + 1]), pack_bf16x2(f[8 * e + 2], f[8 * e + 3]),
+                                             pack_bf16x2(f[8 * e + 4], f[8 * e + 5]), pack_bf16x2(f[8 * e + 6], f[8 * e + 7]));
+                  dst[e] = sees ? y : make_uint4(0u, 0u, 0u, 0u);
+                }
+              }
+            } else if (valid) {
+              float4* dst = reinterpret_cast<float4*>(a.part_o + part * TA_DH + cc * 32);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+            }
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.o_free[grp]);
+          if (!two) mbar_arrive(&sm.o_free[grp ^ 1]);
+        }
+        if (valid && !whole) a.part_ml[part] = make_float2(m, l);
+        __syncwarp();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.o_free[grp]);
-        if (nrt == 1) mbar_arrive(&sm.o_free[grp ^ 1]);
-      }
-      if (valid && !whole) a.part_ml[part] = make_float2(m, l);
-      __syncwarp();
     }
     if (!ok && lane == 0) atomicCAS(a.status, 0, ST_TIMEOUT_TMEM_FULL);
   }
@@ -1114,9 +1223,9 @@ extern "C" int b200_tree_attn(const void* qkv, long long ld, const void* k_cache
   if (B <= 0 || N <= 0) return 0;
   const int need = b200_tree_attn_scratch(max_nodes, Hq, Hkv);
   if (Dh != TA_DH || need < 0 || num_blocks < 1 || max_blocks > (1 << 24)) return -1;
-  // rows of the cache are 32-bit TMA coordinates, tiles are counted in 32 bits
+  // rows of the cache are 32-bit TMA coordinates, work is counted in 32 bits
   if ((static_cast<long long>(num_blocks) + 1) * Hkv * TA_PAGE >= (1ll << 31)) return -3;
-  if (static_cast<double>(B) * Hkv * ((max_nodes + 2 * (128 / (Hq / Hkv)) - 1) / (2 * (128 / (Hq / Hkv)))) * (max_blocks / 2 + 2) >= 2147483648.0) return -3;
+  if (static_cast<double>(B) * Hkv * ((max_nodes + 128 / (Hq / Hkv) - 1) / (128 / (Hq / Hkv))) * (max_blocks / 2 + 2) >= 2147483648.0) return -3;
   TreeArgs a;
   a.G = Hq / Hkv;
   // the narrow kernel where every tree fits into 32 rows
