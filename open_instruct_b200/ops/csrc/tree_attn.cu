@@ -969,7 +969,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
               m = mx;
               l *= alpha;
             }
-            const uint64_t c2 = pair2(c, c), mc2 = pair2(-m * c, -m * c);
+            const float at0 = m == -INFINITY ? 0.f : -m * c;  // no score above -inf yet: weights of zero, not -inf + inf
+            const uint64_t c2 = pair2(c, c), mc2 = pair2(at0, at0);
             uint64_t sum[2] = {0ull, 0ull};  // two pairs of zeros
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc) {

@@ -411,8 +411,9 @@ def _check_index(t: torch.Tensor, dtype, shape: tuple, device, name: str) -> Non
 def _check_rows(t: torch.Tensor, dtype, width: int, device, name: str) -> None:
     if t.dtype is not dtype or t.device != device:
         raise TypeError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
-    if t.dim() != 2 or t.shape[1] != width or t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
-        raise ValueError(f"{name}: expected [N, {width}], 16-byte aligned, contiguous rows with a stride that is a multiple of 8, got {tuple(t.shape)}")
+    if t.dim() != 2 or t.shape[1] != width or t.stride(1) != 1 or t.stride(0) % 8 or (t.stride(0) < width and t.shape[0] > 1) or t.data_ptr() % 16:
+        raise ValueError(f"{name}: expected [N, {width}], 16-byte aligned, contiguous rows with a stride that is a multiple of 8 and no overlap, "
+                         f"got {tuple(t.shape)} with strides {t.stride()}")
 
 
 def _check_cache(k_cache, v_cache, block_table, ctx, n_kv: int, head_dim: int, dtype, device, lead: tuple = ()) -> None:

@@ -260,3 +260,13 @@ def test_engine_refuses_drafts_it_cannot_verify():
         _engine(-1)
     with pytest.raises(NotImplementedError):
         RolloutEngine(get_spec("tiny"), device="cpu", ops="ref", num_blocks=16, speculative_tokens=4)
+
+
+def test_rows_that_overlap_are_refused():
+    a = make_attn(2, 1, [5], [3])
+    for qkv in (a["qkv"][:1].expand(3, -1), torch.empty(4096, dtype=torch.bfloat16).as_strided((3, 512), (256, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            fused._check_tree_attn(**{**a, "qkv": qkv}, out=None, dtype=torch.bfloat16)
+    a["qkv"] = a["qkv"][:1].expand(1, -1)   # one row alone has no stride
+    a["parents"] = a["parents"][:1]
+    fused._check_tree_attn(**a, out=None, dtype=torch.bfloat16)

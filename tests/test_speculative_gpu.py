@@ -60,6 +60,39 @@ def test_tree_attention_ragged(seed):
     _check_attn(make_attn(heads, kv_heads, ctx, counts, device="cuda", seed=seed, extra_rows=seed))
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(7, 1), (8, 2), (16, 1), (64, 1), (3, 3)])
+@pytest.mark.parametrize("seed", range(3))
+def test_tree_attention_uneven_trees(heads, kv_heads, seed):
+    """Trees of one to many row tiles next to each other: shares of the work that end inside a unit of two row tiles."""
+    g = torch.Generator().manual_seed(100 + seed)
+    counts = torch.randint(0, 65, (9,), generator=g).tolist()
+    ctx = [int(1500 * float(r) ** 2) for r in torch.rand(9, generator=g)]
+    _check_attn(make_attn(heads, kv_heads, ctx, counts, device="cuda", seed=seed, extra_rows=seed))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (8, 1)])
+def test_tree_attention_many_sequences(heads, kv_heads):
+    """More sequences than a CTA has threads, the first 500 of them empty."""
+    counts = [0] * 500 + [i % 6 for i in range(500)]
+    _check_attn(make_attn(heads, kv_heads, [(37 * i) % 150 for i in range(1000)], counts, device="cuda"))
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_tree_attention_scores_below_the_range(most):
+    """A whole tile of keys whose scores are -inf in fp32 (narrow and wide kernel): no weight, and nothing else is disturbed."""
+    a = make_attn(1, 1, [200, 5], [1, most], device="cuda")
+    far = -3.0e38 * torch.sign(a["qkv"][0, :DIM].float())
+    a["k_cache"][a["block_table"][0, :2].long(), 0] = far.bfloat16()
+    _check_attn(a)
+
+
+def test_tree_attention_shared_pages():
+    """Two sequences on the same pages and one table row for both."""
+    a = make_attn(8, 2, [150, 150], [5, 9], device="cuda", garbage=False)
+    a["block_table"] = a["block_table"][:1].expand(2, -1)
+    _check_attn(a)
+
+
 def test_tree_attention_peaked_and_large_scores():
     """Scores of a few tens and more: the running maximum moves far.  A query has a standard deviation of 18, the 128 products of
     a score add up to less than 2^12 in magnitude, so fp32 sums leave it off by at most 128 * 2^-24 * 2^12 = 2^-5, times the scale
@@ -198,6 +231,23 @@ def test_verification_large_vocabulary(likely, drafted):
 
 def test_verification_many_sequences():
     _check_verify(make_verify([1 + i % 5 for i in range(300)], 512, "tree", False, temps=(1.0, 0.0, 0.7), seed=6, device="cuda"))
+
+
+def test_verification_of_nothing():
+    from open_instruct_b200.ops import fused
+
+    for counts in ([], [0, 0, 0]):
+        for drafted in (False, True):
+            a = make_verify(counts, 50, "chain", drafted, device="cuda")
+            count, tokens, path, logprobs = fused.verify_tree(**a)
+            assert count.tolist() == counts and (tokens == -1).all() and (path == -1).all() and (logprobs == 0).all()
+
+
+def test_verification_broadcast_rows():
+    """One row of logits and one drafter's row for all nodes (stride 0)."""
+    a = make_verify([4, 1, 6], 1003, "tree", True, temps=(1.0, 0.7), seed=3, device="cuda")
+    a["logits"], a["draft_probs"] = a["logits"][:1].expand(11, -1), a["draft_probs"][2:3].expand(11, -1)
+    _check_verify(a)
 
 
 @pytest.mark.parametrize("drafted", [False, True])
