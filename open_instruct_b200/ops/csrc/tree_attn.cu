@@ -125,7 +125,7 @@ struct TreeSmem {
   float wt[8][2][32];    // narrow units: a warp's weights of the rows, on their way from one lane to all
   uint32_t flags[2];     // narrow units: a byte for each warp of a group
   TreeSegment seg[2];
-  uint64_t q_full[2], q_empty[2], r_full[RING], r_empty[RING], s_full[2][2], p_full[2][2], o_full[2], o_free[2],
+  uint64_t q_full[2], q_empty[2], r_full[RING], r_empty[RING], s_full[2][2], p_full[2][2], o_full[2][2], o_free[2][2],
       seg_full[2], seg_empty[2], ml_full[2], lx_full[2], flag_full[2], mx_full[2];
   int scan[TA_THREADS / 32];
   TreeSeq at;            // the sequence in which the CTA's share begins
@@ -194,9 +194,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       for (int j = 0; j < 2; ++j) {
         mbar_init(&sm.s_full[i][j], 1);
         mbar_init(&sm.p_full[i][j], 4);
+        mbar_init(&sm.o_full[i][j], 1);
+        mbar_init(&sm.o_free[i][j], 8);
       }
-      mbar_init(&sm.o_full[i], 1);
-      mbar_init(&sm.o_free[i], 8);
       mbar_init(&sm.ml_full[i], 4);
       mbar_init(&sm.lx_full[i], 4);
       mbar_init(&sm.flag_full[i], 4);
@@ -453,17 +453,20 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             if (!mbar_wait(&sm.p_full[j.grp][0], (pc >> j.grp) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
             pc ^= 1u << j.grp;
             if (!mbar_wait(&sm.r_full[j.vslot], j.vpar, abort_flag)) return give_up(ST_TIMEOUT_FULL);
-            // a group's first product of a unit overwrites its O: the last unit's must have been read
-            // (each barrier is waited for once a segment, so that a parity always means the phase before)
-            if (j.first && seg > 0 &&
-                !(mbar_wait(&sm.o_free[j.grp], (seg - 1) & 1, abort_flag) && (!j.alone || mbar_wait(&sm.o_free[j.grp ^ 1], (seg - 1) & 1, abort_flag))))
+            // A group's first product of a segment overwrites its O of the segment before the last, which must have been read: two O
+            // for each group, so that a unit's result is written while the next unit's products go on.
+            // (Each barrier is waited for once in two segments, so that a parity always means the phase before.)
+            const int ob = seg & 1;
+            if (j.first && seg > 1 &&
+                !(mbar_wait(&sm.o_free[j.grp][ob], ((seg >> 1) - 1) & 1, abort_flag) &&
+                  (!j.alone || mbar_wait(&sm.o_free[j.grp ^ 1][ob], ((seg >> 1) - 1) & 1, abort_flag))))
               return give_up(ST_TIMEOUT_TMEM_EMPTY);
             tc_fence_after();
-            const uint32_t v = smem_u32(sm.ring[j.vslot]), p = smem_u32(sm.p[j.grp]), o = tmem + 256 + j.grp * 128;
+            const uint32_t v = smem_u32(sm.ring[j.vslot]), p = smem_u32(sm.p[j.grp]), o = tmem + 256 + j.grp * 128 + ob * 32;
             const int steps = j.half ? 4 : 8;
             for (int k = 0; k < steps; ++k) umma_ss(o, ta_desc_mn(v, k), ta_desc_p(p + k * 1024), idesc_o, !(j.first && k == 0));
             umma_commit(&sm.r_empty[j.vslot]);
-            if (j.last) umma_commit(&sm.o_full[j.grp]);
+            if (j.last) umma_commit(&sm.o_full[j.grp][ob]);
             return true;
           };
           Job prev;
@@ -532,13 +535,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             if (!mbar_wait(&sm.p_full[grp][b], (steps_o >> 1) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
             if (!loaded(prev.v)) return false;
             // the first product of a unit overwrites O: the last unit's must have been read
-            if (prev.first && prev_seg > 0 && !mbar_wait(&sm.o_free[grp], (prev_seg - 1) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
+            if (prev.first && prev_seg > 0 && !mbar_wait(&sm.o_free[grp][0], (prev_seg - 1) & 1, abort_flag)) return give_up(ST_TIMEOUT_TMEM_EMPTY);
             tc_fence_after();
             const uint32_t v = smem_u32(sm.ring[prev.v % RING]) + prev.h * (TA_SUB / 2), p = t_s + b * 64;
 #pragma unroll
             for (int k = 0; k < 4; ++k) umma_ts(t_o, p + k * 8, ta_desc_mn(v, k), idesc_o, !(prev.first && k == 0));
             if (prev.last) umma_commit(&sm.r_empty[prev.v % RING]);
-            umma_commit(&sm.o_full[grp]);  // of every step: the softmax rescales O between them
+            umma_commit(&sm.o_full[grp][0]);  // of every step: the softmax rescales O between them
             ++steps_o;
             have = false;
             return true;
@@ -607,24 +610,26 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     // the last segment's end is over on both sides, what it left behind has been read.  Every warp waits for that in every
     // segment and says when it is through with this one, so no barrier is more than one phase away from a parity that is waited for.
     auto last_end = [&](uint32_t n) {
-      return n == 0 || (ta_warp_wait(&sm.o_free[0], (n - 1) & 1, abort_flag) && ta_warp_wait(&sm.o_free[1], (n - 1) & 1, abort_flag));
+      const int ob = narrow ? (n - 1) & 1 : 0, par = (narrow ? (n - 1) >> 1 : n - 1) & 1;
+      return n == 0 || (ta_warp_wait(&sm.o_free[0][ob], par, abort_flag) && ta_warp_wait(&sm.o_free[1][ob], par, abort_flag));
     };
-    auto through = [&] {
+    auto through = [&](uint32_t n) {
+      const int ob = narrow ? n & 1 : 0;
       if (lane == 0) {
-        mbar_arrive(&sm.o_free[0]);
-        mbar_arrive(&sm.o_free[1]);
+        mbar_arrive(&sm.o_free[0][ob]);
+        mbar_arrive(&sm.o_free[1][ob]);
       }
     };
     if constexpr (narrow) {
       uint32_t jc = 0;
-      uint32_t par_s = 0, par_o = 0, par_ml = 0, par_flag = 0, par_mx = 0, par_lx = 0;  // parities of the next S, of either group's O (bits 0, 1), of exchanges
-      bool late = false;                            // this group's last O was somebody else's to wait for
+      uint32_t par_s = 0, par_o = 0, par_ml = 0, par_flag = 0, par_mx = 0, par_lx = 0;  // parities of the next S, of either group's O (bit: group, and 2 more in odd segments), of exchanges
       const int rn = lane / a.G, rg = lane - rn * a.G;  // node and head of row `lane`
       for (uint32_t n = 0; ok; ++n) {
         const TreeSegment& g = sm.seg[n & 1];
         ok = ta_warp_wait(&sm.seg_full[n & 1], (n >> 1) & 1, abort_flag);
         if (!ok || g.t0 == g.t1) break;
-        const int t0 = g.t0, count = g.t1 - t0, nt = g.nt, T = g.T, C = g.C, jobs = count;
+        const int t0 = g.t0, count = g.t1 - t0, nt = g.nt, T = g.T, C = g.C, jobs = count, ob = n & 1;
+        const uint32_t t_on = t_o + ob * 32;
         const int x0 = (grp ^ jc) & 1;           // my first job of this segment; then every second one
         const bool valid = rn < T;
         const unsigned long long sees = valid ? g.sees[rn] : 0ull;
@@ -637,10 +642,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         auto begin_job = [&](int x, int& keys, bool& half) -> bool {
           if (!ta_warp_wait(&sm.s_full[grp][0], par_s, abort_flag)) return false;
           par_s ^= 1;
-          if (late) {  // complete since this S was issued behind it: keeps the parity in step
-            if (!ta_warp_wait(&sm.o_full[grp], (par_o >> grp & 1) ^ 1, abort_flag)) return false;
-            late = false;
-          }
           tc_fence_after();
           const int t = t0 + x;
           keys = min(128, C - t * 128);
@@ -759,7 +760,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             }
             if (x >= 2) {
               uint32_t o[32];
-              tmem_ld32(t_o + grp * 128, o);
+              tmem_ld32(t_on + grp * 128, o);
               tmem_ld_wait();
 #pragma unroll
               for (int e = 0; e < 32; e += 4) {
@@ -769,7 +770,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 o[e + 2] = __float_as_uint(__uint_as_float(o[e + 2]) * w.z);
                 o[e + 3] = __float_as_uint(__uint_as_float(o[e + 3]) * w.w);
               }
-              tmem_st32(t_o + grp * 128, o);
+              tmem_st32(t_on + grp * 128, o);
               tmem_st_wait();
             }
             __syncwarp();
@@ -821,10 +822,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             sm.lm[grp][lane] = m;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.ml_full[grp]);
-            late = true;
           }
-          through();
-          par_o ^= both ? 3 : 1 << last;
+          through(n);
+          par_o ^= (both ? 3 : 1 << last) << 2 * ob;
           continue;
         }
         float a0 = 1.f, a1 = 0.f;  // weights of my own O and of the other group's
@@ -838,7 +838,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (both) {
           ok = ta_warp_wait(&sm.ml_full[grp ^ 1], par_ml, abort_flag);
           par_ml ^= 1;
-          if (ok) ok = ta_warp_wait(&sm.o_full[grp ^ 1], par_o >> (grp ^ 1) & 1, abort_flag);
+          if (ok) ok = ta_warp_wait(&sm.o_full[grp ^ 1][ob], par_o >> (2 * ob + (grp ^ 1)) & 1, abort_flag);
           if (!ok) break;
           const float* o = &sm.ls[grp ^ 1][0][lane];
           const float l_other = (o[0] + o[32]) + (o[64] + o[96]), m_other = sm.lm[grp ^ 1][lane], top = fmaxf(m, m_other);
@@ -847,8 +847,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           l = a0 * l + a1 * l_other;
           m = top;
         }
-        ok = ta_warp_wait(&sm.o_full[grp], par_o >> grp & 1, abort_flag);
-        par_o ^= both ? 3 : 1 << grp;
+        ok = ta_warp_wait(&sm.o_full[grp][ob], par_o >> (2 * ob + grp) & 1, abort_flag);
+        par_o ^= (both ? 3 : 1 << grp) << 2 * ob;
         if (!ok) break;
         tc_fence_after();
         const bool whole = t0 == 0 && count == nt;
@@ -860,8 +860,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (!whole && valid && lg == 0) a.part_ml[part] = make_float2(m, l);
         const int to = valid ? (rn * a.Hq + rg) * TA_DH : -1;
         uint32_t o0[32], o1[32];
-        tmem_ld32(t_o + grp * 128, o0);
-        if (both) tmem_ld32(t_o + (grp ^ 1) * 128, o1);
+        tmem_ld32(t_on + grp * 128, o0);
+        if (both) tmem_ld32(t_on + (grp ^ 1) * 128, o1);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
@@ -881,7 +881,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           }
         }
         __syncwarp();
-        through();
+        through(n);
         const int rows = T * a.G;
         if (whole) {
           __nv_bfloat16* dst = a.out + seg_at + (r & ~1);  // two neighbouring dimensions of every second row
@@ -994,7 +994,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           // the last product's phase can only mean that one.
           const bool rescale = u > 0 && __any_sync(0xffffffffu, grow);
           if (U > 0 && (rescale || u == steps - 1)) {
-            ok = ta_warp_wait(&sm.o_full[grp], (U - 1) & 1, abort_flag);
+            ok = ta_warp_wait(&sm.o_full[grp][0], (U - 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
           }
@@ -1033,7 +1033,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (!ok) break;
         float a0 = 1.f, a1 = 0.f;  // weights of my own O and of the other group's
         if (two) {
-          if (lane == 0) mbar_arrive(&sm.o_free[grp ^ 1]);
+          if (lane == 0) mbar_arrive(&sm.o_free[grp ^ 1][0]);
         } else if (grp != last) {
           if (both) {
             sm.ml[r] = l;
@@ -1041,10 +1041,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.ml_full[grp]);
           }
-          through();
+          through(n);
           continue;
         } else if (both) {
-          ok = ta_warp_wait(&sm.ml_full[grp ^ 1], par_ml >> (grp ^ 1) & 1, abort_flag) && ta_warp_wait(&sm.o_full[grp ^ 1], their_last & 1, abort_flag);
+          ok = ta_warp_wait(&sm.ml_full[grp ^ 1], par_ml >> (grp ^ 1) & 1, abort_flag) && ta_warp_wait(&sm.o_full[grp ^ 1][0], their_last & 1, abort_flag);
           par_ml ^= 1u << (grp ^ 1);
           if (!ok) break;
           const float l_other = sm.ml[r], m_other = sm.ml[128 + r], top = fmaxf(m, m_other);
@@ -1053,7 +1053,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           l = a0 * l + a1 * l_other;
           m = top;
         }
-        ok = steps == 0 || ta_warp_wait(&sm.o_full[grp], my_last & 1, abort_flag);
+        ok = steps == 0 || ta_warp_wait(&sm.o_full[grp][0], my_last & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
         const bool whole = t0 == 0 && count == nt;
@@ -1097,8 +1097,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&sm.o_free[grp]);
-          if (!two) mbar_arrive(&sm.o_free[grp ^ 1]);
+          mbar_arrive(&sm.o_free[grp][0]);
+          if (!two) mbar_arrive(&sm.o_free[grp ^ 1][0]);
         }
         if (valid && !whole) a.part_ml[part] = make_float2(m, l);
         __syncwarp();
