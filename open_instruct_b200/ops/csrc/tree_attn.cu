@@ -9,26 +9,36 @@
 //
 // Work.  All nodes of a sequence and all G query heads of a KV head read the same keys, so they are the rows of one matrix
 // product: a row tile holds floor(128 / G) nodes x G heads, a UNIT is up to two row tiles of one (sequence, KV head), its keys
-// come in tiles of 128 (two cache pages), the tree's own keys are one last tile of 64.  Per tile of keys the cache delivers
-// 64 KB; the tensor cores need about 1000 cycles for the two products of a row tile and HBM about 2700 cycles of one SM's share for
-// the 64 KB, so up to 256 rows are bound by the cache's bytes.
+// come in tiles of 128 (two cache pages), the tree's own keys are the last 64 (beside an odd last page, or a half tile of their
+// own).  HBM gives one SM's share of the 64 KB of a key tile in about 2700 cycles.  A row tile's products take the tensor cores
+// 1300 cycles a key tile and its exponentials the special-function units 1024; what the softmax warps really need for them,
+// with loads, maxima and packing, is 2560.  So units of one row tile run at the cache's bytes, two row tiles at the softmax.
 //
-// Split.  The key tiles of all units, laid end to end, are shared out evenly over the CTAs (one per SM), whatever the
-// sequences' lengths; a unit that crosses a border is finished in parts (unnormalised output, maximum and sum in fp32), which
-// a second kernel joins in the order of the keys.  The shares are computed from ctx and cu on the device, so one captured graph
-// serves every step.
+// Split.  The work of all units - key tiles times row tiles, laid end to end - is shared out evenly over the CTAs (one per SM),
+// whatever the sequences' lengths; a unit that crosses a border is finished in parts (unnormalised output, maximum and sum in
+// fp32), which a second kernel joins in the order of the keys.  The shares are computed from ctx and cu on the device, so one
+// captured graph serves every step.
 //
-// One CTA: warp 0 streams pages with TMA through a ring of four 32 KB buffers, warp 1 issues S = Q K^T and O += P V, two groups
-// of four warps own the softmax (warps 4 to 7 and 8 to 11), warp 2 plans the segments ahead.  A unit of two row tiles gives each group one of them (the keys are loaded once for both); a
-// unit of one row tile gives the groups alternate key tiles, merged at the end, so that one group's exponentials always run
-// beside the other group's products.  P replaces S in tensor memory (bf16), O stays there for the whole unit and is rescaled
-// only when the row maximum has grown by more than 2^8.
+// One CTA: warp 0 streams pages with TMA through a ring of 32 KB buffers, warp 2 plans the segments ahead, warps 1 and 3 issue
+// S = Q K^T and O += P V, two groups of four warps own the softmax (warps 4 to 7 and 8 to 11).
 //
-// A second kernel serves batches whose units have at most 32 rows (single tokens and short drafts).  As rows of a 128-row tile they would leave three quarters
-// of the tensor work and most of the softmax warps to padding - and the padding is paid for in power: at 8 rows a unit the GPU
-// ran at its 1000 W limit with the clock down to 1.5 GHz.  So the products are turned round, S^T = K Q^T and O^T = V^T P^T, with
-// the 128 keys (the 128 dimensions) as the tile's rows and 32 columns: a quarter of the tensor work, every thread of a group
-// has one key and 32 rows, and the result's rows are written by all of its warps.
+// Wide kernel (more than 32 rows a unit): 128 rows by 64 keys a step.  A unit of two row tiles gives each group one of them (the
+// keys are loaded once for both); a unit of one row tile gives each group its half of every key tile, merged at the end.  Each
+// group has its own product thread and two buffers for S, so the next scores are there when a step's softmax is through.  P
+// replaces S in tensor memory (bf16), O stays there for the whole unit and is rescaled only when the row maximum has grown by
+// more than 2^8.  Measured: 16 trees of 64 nodes, 8 heads a KV head, contexts of 8192 to 32768: 697 GFLOP in 815 to 900 us = 775
+// to 855 TFLOP/s; the GPU is at its 1000 W limit by then and holds the SM clock at 1.5 GHz, where steps of 128 keys with one
+// product thread (4 % behind), a later start of the second group, and scores fetched a step ahead (12 % behind) make no gain.
+// 32 trees of 1 to 27 nodes, 7 heads a KV head: 88 to 97 us, 102 with shares in key tiles alone.
+//
+// Narrow kernel (at most 32 rows a unit: single tokens and short drafts).  As rows of a 128-row tile they would leave three
+// quarters of the tensor work and most of the softmax warps to padding - and the padding is paid for in power: at 8 rows a unit
+// the GPU ran at its 1000 W limit with the clock down to 1.5 GHz.  So the products are turned round, S^T = K Q^T and O^T = V^T P^T,
+// with the 128 keys (the 128 dimensions) as the tile's rows and 32 columns: a quarter of the tensor work, every thread of a
+// group has one key and 32 rows, and the result's rows are written by all of its warps.  The groups take alternate key tiles and
+// have two O each, so that a unit is written while the next one runs (298 -> 289 us at one head a group).  Measured: 32 sequences
+// of 4 nodes at 16384 tokens, 8 KV heads: 326 us, 6.6 TB/s; 128 trees of 8 nodes, 32 KV heads, contexts of 256 to 1024: 289 us,
+// 4.8 TB/s (6 key tiles a unit: a sixth of the tiles are the trees' own, and a unit's end costs about 4000 cycles).
 #include "common.cuh"
 
 namespace b200 {
@@ -36,9 +46,9 @@ namespace b200 {
 constexpr int TA_DH = 128;
 constexpr int TA_PAGE = 64;
 constexpr int TA_MAX_NODES = 64;
-constexpr int TA_THREADS = 384;          // four warps for TMA, products and planning (one idle), two groups of four for the softmax
-// Registers: 12 warps at launch have 168 a thread.  The softmax wants more, the issuing warps less (the wide kernel's four cursors
-// more than the narrow one's loop): the first group gives back what the other two take.
+constexpr int TA_THREADS = 384;          // four warps for TMA, products and planning, two groups of four for the softmax
+// Registers: 12 warps at launch have 168 a thread.  The softmax wants more, the issuing warps less: the first group gives back what
+// the other two take.  No kernel spills with these splits (a few spilled words in the softmax loop had cost 10 %).
 constexpr int TA_REGS = 168;
 template <bool narrow>
 struct TaRegs {
@@ -47,7 +57,7 @@ struct TaRegs {
 };
 constexpr int TA_SUB = 128 * 64 * 2;     // bytes of one [128 x 64] swizzled sub-tile
 constexpr int TA_TILE = 2 * TA_SUB;      // a [128 keys or rows x 128] bf16 tile
-constexpr int TA_RING = 4;               // two tiles of keys and values in flight (a fifth buffer was measured to change nothing)
+constexpr int TA_RING = 4;               // two tiles of keys and values in flight; the narrow kernel has room for a fifth (no difference measured)
 constexpr int TA_QSUB = 32 * 64 * 2;     // a narrow unit's queries: two [32 x 64] swizzled sub-tiles
 constexpr int TA_MIN_WORK = 2;           // products of a key and a row tile that a CTA takes at least: below that joining the parts costs more than it saves
 constexpr float TA_LOG2E = 1.4426950408889634f;
@@ -81,8 +91,8 @@ struct TreeSeq {
     nt = (C + TA_PAGE - 1) / TA_PAGE / 2 + 1;
     rts = (T + a.npt - 1) / a.npt;
   }
-  // Work in products of a key tile with a row tile: what a unit costs goes with its row tiles (2560 cycles each a key tile of the
-  // wide kernel, with two of them or one).  Shares in key tiles alone left the busiest SM of an uneven batch with 1.3 times the mean.
+  // Work in products of a key tile with a row tile: what a unit of the wide kernel costs goes with its row tiles.  Shares in key
+  // tiles alone left the busiest SM of an uneven batch with 1.33 times the mean (1.20 now), 102 us against 91.
   __device__ __forceinline__ int work(const TreeArgs& a) const { return a.Hkv * rts * nt; }
   __device__ __forceinline__ int pairs() const { return (rts + 1) >> 1; }  // of row tiles: units of a KV head
 };
@@ -1229,7 +1239,8 @@ extern "C" int b200_tree_attn(const void* qkv, long long ld, const void* k_cache
   if (static_cast<double>(B) * Hkv * ((max_nodes + 128 / (Hq / Hkv) - 1) / (128 / (Hq / Hkv))) * (max_blocks / 2 + 2) >= 2147483648.0) return -3;
   TreeArgs a;
   a.G = Hq / Hkv;
-  // the narrow kernel where every tree fits into 32 rows
+  // The narrow kernel where every tree fits into 32 rows.  Narrow against wide: 32 rows at contexts of 16384, 345 against 368 us, of
+  // 1024, 68 against 75; 20 rows, 69 against 81; 8 rows, 290 against 350; single tokens, 12.0 against 15.0.
   const bool narrow = max_nodes * a.G <= 32;
   a.npt = (narrow ? 32 : 128) / a.G;
   CUtensorMap tq, tn, tk, tv;
