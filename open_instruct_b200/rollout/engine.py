@@ -28,6 +28,7 @@ import torch
 from ..data_types import GenerationResult, RequestInfo, SamplingConfig, TokenStatistics
 from ..models import LlamaModel, ModelSpec
 from ..ops import lib, ref
+from .speculative import PromptLookup, draft_tree, uniforms
 
 KV_BLOCK = 64
 
@@ -861,20 +862,19 @@ class RolloutEngine:
     # ---- speculative decode step
     def _draft(self, seq: _Sequence):
         """Draft tree of one sequence: no deeper than the tokens it may still emit and the pages it holds."""
-        from .speculative import PromptLookup, draft_tree
-
         if seq.lookup is None:
             seq.lookup = PromptLookup()
-        n = len(seq.tokens)
-        room = min(len(self.host.blocks(seq.sid)[0]) * KV_BLOCK - n, seq.request.sampling.max_tokens - (n - seq.prompt_len) - 1, self.speculative_tokens)
-        return draft_tree(seq.tokens[-1], seq.lookup.continuations(seq.tokens, room), self.speculative_tokens)
+        ahead = seq.lookup.continuations(seq.tokens, self.speculative_tokens)
+        if ahead:
+            n = len(seq.tokens)
+            room = min(len(self.host.blocks(seq.sid)[0]) * KV_BLOCK - n, seq.request.sampling.max_tokens - (n - seq.prompt_len) - 1)
+            ahead = [chain[:max(room, 0)] for chain in ahead]
+        return draft_tree(seq.tokens[-1], ahead, self.speculative_tokens)
 
     def _decode_drafts(self, seqs: list[_Sequence], drafts: list) -> None:
         """One pass over the draft trees of all sequences: the layers with tree attention, verification of the trees, commit of the
         confirmed nodes' keys and values, acceptance of their tokens."""
         import numpy as np
-
-        from .speculative import uniforms
 
         if self.ops == "fused":
             from ..ops import fused as f
