@@ -1141,37 +1141,64 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
   const int4 join = a.joins[cta];
   const int parts = join.x;
   if (parts == 0) return;
-  const int lane = threadIdx.x & 31;
-  for (int i = 0; i < 4; ++i) {
-    const int row = blockIdx.y * 32 + i * 8 + (threadIdx.x >> 5), rt = row >> 7, r = row & 127;
-    const int rn = r / a.G, node = rt * a.npt + rn;
-    if (row >= a.part_rows || rn >= a.npt || node >= join.z) continue;
-    auto at = [&](int p) { return (static_cast<long long>(cta + p) * 2 + (p == 0 ? 1 : 0)) * a.part_rows + row; };
-    float top = -INFINITY;
-    for (int p = lane; p < parts; p += 32) {
-      const float2 ml = a.part_ml[at(p)];
-      if (ml.y != 0.f) top = fmaxf(top, ml.x);
+  // A warp joins four rows at a time, all their loads in flight together: one row after the other took 15.5 us for parts of 256
+  // rows (75 MB of parts), this 9.6; with four rows in all it is 0.5 us slower (12.7 against 12.2 us for the whole call).
+  constexpr int ROWS = 4;
+  const int lane = threadIdx.x & 31, row0 = blockIdx.y * 32 + (threadIdx.x >> 5);  // and every eighth row from there
+  int node[ROWS];  // -1: no row
+  float top[ROWS], l[ROWS];
+  float4 acc[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int row = row0 + 8 * i, rn = (row & 127) / a.G;
+    node[i] = (row >> 7) * a.npt + rn;
+    if (row >= a.part_rows || rn >= a.npt || node[i] >= join.z) node[i] = -1;
+    top[i] = -INFINITY;
+    l[i] = 0.f;
+    acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  auto at = [&](int p, int i) { return (static_cast<long long>(cta + p) * 2 + (p == 0 ? 1 : 0)) * a.part_rows + row0 + 8 * i; };
+  for (int p = lane; p < parts; p += 32) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if (node[i] < 0) continue;
+      const float2 ml = a.part_ml[at(p, i)];
+      if (ml.y != 0.f) top[i] = fmaxf(top[i], ml.x);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+  for (int p = 0; p < parts; ++p) {
+    float2 ml[ROWS];
+    float4 v[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      ml[i] = make_float2(0.f, 0.f);
+      if (node[i] < 0) continue;
+      ml[i] = a.part_ml[at(p, i)];
+      v[i] = reinterpret_cast<const float4*>(a.part_o + at(p, i) * TA_DH)[lane];
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < parts; ++p) {
-      const float2 ml = a.part_ml[at(p)];
-      if (ml.y == 0.f) continue;
-      const float w = ex2_approx(ml.x - top);
-      const float4 v = reinterpret_cast<const float4*>(a.part_o + at(p) * TA_DH)[lane];
-      l += w * ml.y;
-      acc.x += w * v.x;
-      acc.y += w * v.y;
-      acc.z += w * v.z;
-      acc.w += w * v.w;
+    for (int i = 0; i < ROWS; ++i) {
+      if (ml[i].y == 0.f) continue;
+      const float w = ex2_approx(ml[i].x - top[i]);
+      l[i] += w * ml[i].y;
+      acc[i].x += w * v[i].x;
+      acc[i].y += w * v[i].y;
+      acc[i].z += w * v[i].z;
+      acc[i].w += w * v[i].w;
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;  // an empty row gives zeros, a NaN stays one
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    if (node[i] < 0) continue;
+    const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;  // an empty row gives zeros, a NaN stays one
     uint2 res;
-    res.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-    res.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-    __nv_bfloat16* dst = a.out + ((static_cast<long long>(join.y) + node) * a.Hq + join.w * a.G + r % a.G) * TA_DH;
+    res.x = pack_bf16x2(acc[i].x * inv, acc[i].y * inv);
+    res.y = pack_bf16x2(acc[i].z * inv, acc[i].w * inv);
+    __nv_bfloat16* dst = a.out + ((static_cast<long long>(join.y) + node[i]) * a.Hq + join.w * a.G + ((row0 + 8 * i) & 127) % a.G) * TA_DH;
     reinterpret_cast<uint2*>(dst)[lane] = res;
   }
 }
