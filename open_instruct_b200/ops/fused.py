@@ -7,9 +7,9 @@ call fails in Python instead of on the device.
 
 from __future__ import annotations
 
-import ctypes
 import functools
 import math
+from array import array
 
 import torch
 
@@ -581,7 +581,7 @@ def kv_commit_(qkv_layers, k_cache: torch.Tensor, v_cache: torch.Tensor, block_t
     if L:
         _need_cuda(qkv_layers[0], "qkv")
     pointers = _check_kv_commit(qkv_layers, k_cache, v_cache, block_table, ctx, path, n_q, n_kv, head_dim, torch.bfloat16)
-    first, pointers = qkv_layers[0], (ctypes.c_void_p * L)(*pointers)
-    _call_on(first.device, "b200_kv_commit", ctypes.addressof(pointers), L, first.stride(0), first.shape[0], ptr(k_cache), ptr(v_cache),
+    first, pointers = qkv_layers[0], array("Q", pointers)  # a ctypes array takes seven times as long
+    _call_on(first.device, "b200_kv_commit", pointers.buffer_info()[0], L, first.stride(0), first.shape[0], ptr(k_cache), ptr(v_cache),
              k_cache.stride(0), k_cache.shape[1], ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(ctx), ptr(path),
              ctx.shape[0], path.shape[1], n_q, n_kv, head_dim)
