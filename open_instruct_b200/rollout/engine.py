@@ -789,9 +789,9 @@ class RolloutEngine:
         dev = self.device
         B = len(seqs)
         if self.speculative_tokens and all(q.request.sampling.top_p >= 1.0 for q in seqs):
-            drafts = [self._draft(q) for q in seqs]
-            if any(len(tokens) > 1 for tokens, _, _ in drafts):
-                self._decode_drafts(seqs, drafts)
+            ahead = [self._ahead(q) for q in seqs]
+            if any(ahead):
+                self._decode_drafts(seqs, [draft_tree(q.tokens[-1], chains, self.speculative_tokens) for q, chains in zip(seqs, ahead)])
                 return
         if self.ops == "fused":
             t0 = time.perf_counter()
@@ -860,16 +860,16 @@ class RolloutEngine:
             self._accept(q, int(t), float(lp))
 
     # ---- speculative decode step
-    def _draft(self, seq: _Sequence):
-        """Draft tree of one sequence: no deeper than the tokens it may still emit and the pages it holds."""
+    def _ahead(self, seq: _Sequence) -> list:
+        """What may come next in one sequence, no longer than the tokens it may still emit and the pages it holds."""
         if seq.lookup is None:
             seq.lookup = PromptLookup()
         ahead = seq.lookup.continuations(seq.tokens, self.speculative_tokens)
         if ahead:
             n = len(seq.tokens)
             room = min(len(self.host.blocks(seq.sid)[0]) * KV_BLOCK - n, seq.request.sampling.max_tokens - (n - seq.prompt_len) - 1)
-            ahead = [chain[:max(room, 0)] for chain in ahead]
-        return draft_tree(seq.tokens[-1], ahead, self.speculative_tokens)
+            ahead = [chain[:room] for chain in ahead] if room > 0 else []
+        return ahead
 
     def _decode_drafts(self, seqs: list[_Sequence], drafts: list) -> None:
         """One pass over the draft trees of all sequences: the layers with tree attention, verification of the trees, commit of the

@@ -26,14 +26,14 @@ class PromptLookup:
         for p in range(max(self.seen, n), len(tokens)):
             key = tuple(tokens[p - n:p])
             old = self.behind.get(key)
-            self.behind[key] = (p, old[0] if old else -1)
+            self.behind[key] = (p, old[0]) if old else (p,)
         self.seen = len(tokens)
 
     def continuations(self, tokens: list, length: int) -> list:
         """What followed the last n-gram before, latest first: lists of at most ``length`` tokens."""
         self.update(tokens)
         at = self.behind.get(tuple(tokens[-self.ngram:])) if len(tokens) >= self.ngram and length > 0 else None
-        return [tokens[p:p + length] for p in at or () if 0 <= p]
+        return [tokens[p:p + length] for p in at] if at else []
 
 
 def draft_tree(last_token: int, continuations: list, most: int):
