@@ -1133,9 +1133,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 }
 
 // Joins the parts of the units that cross a border between CTAs: block (x, y) rows 32 y .. of the unit that begins in CTA x.
-// A warp takes a row, parts in the order of the keys.
+// Parts in the order of the keys.
+//
+// Nothing is launched early behind this kernel, so whatever follows the attention starts when all of its CTAs have left and their
+// tensor memory is free.  Launched early, the pairs of a decode GEMM two kernels further took over SMs the moment the attention's
+// last CTAs left them, and their allocation of tensor memory for a pair, right behind the release by a single CTA, never returned
+// (5 rows at 8B, within 60 decode steps; the bounded waits cannot end that one).
 __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a) {
-  griddep_launch_dependents();
   griddep_wait();
   const int cta = blockIdx.x;
   const int4 join = a.joins[cta];

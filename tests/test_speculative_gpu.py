@@ -86,6 +86,38 @@ def test_tree_attention_scores_below_the_range(most):
     _check_attn(a)
 
 
+def test_tree_attention_between_decode_gemms():
+    """As in the engine's layers: the decode GEMMs around it allocate tensor memory for CTA pairs and are launched early."""
+    from open_instruct_b200.ops import fused
+
+    a = make_attn(32, 8, [300], [5], device="cuda", garbage=False)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = [(torch.randn(n, k, device="cuda", generator=g) / k ** 0.5).bfloat16() for n, k in ((4096, 4096), (28672, 4096), (4096, 14336), (6144, 4096))]
+    norm = torch.ones(4096, device="cuda", dtype=torch.bfloat16)
+    x = a.pop("qkv")
+
+    def layer(x, sync):
+        o = fused.tree_attn(x, **a)
+        if sync:
+            torch.cuda.synchronize()
+        y = fused.rmsnorm_fwd(fused.gemm_decode(o, w[0]), norm, 1e-6)[0]
+        y = fused.gemm_decode(fused.swiglu_fwd(fused.gemm_decode(y, w[1])), w[2])
+        y = fused.gemm_decode(fused.rmsnorm_fwd(y, norm, 1e-6)[0], w[3])
+        if sync:
+            torch.cuda.synchronize()
+        return y
+
+    want = x
+    for _ in range(8):
+        want = layer(want, True)
+    for _ in range(60):
+        got = x
+        for _ in range(8):
+            got = layer(got, False)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_tree_attention_shared_pages():
     """Two sequences on the same pages and one table row for both."""
     a = make_attn(8, 2, [150, 150], [5, 9], device="cuda", garbage=False)
