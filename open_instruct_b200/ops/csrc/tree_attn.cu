@@ -37,8 +37,8 @@
 // with the 128 keys (the 128 dimensions) as the tile's rows and 32 columns: a quarter of the tensor work, every thread of a
 // group has one key and 32 rows, and the result's rows are written by all of its warps.  The groups take alternate key tiles and
 // have two O each, so that a unit is written while the next one runs (298 -> 289 us at one head a group).  Measured: 32 sequences
-// of 4 nodes at 16384 tokens, 8 KV heads: 326 us, 6.6 TB/s; 128 trees of 8 nodes, 32 KV heads, contexts of 256 to 1024: 289 us,
-// 4.8 TB/s (6 key tiles a unit: a sixth of the tiles are the trees' own, and a unit's end costs about 4000 cycles).
+// of 4 nodes at 16384 tokens, 8 KV heads: 326 us, 6.6 TB/s; 128 trees of 8 nodes, 32 KV heads, contexts of 256 to 1024: 289 to 295 us,
+// 4.7 TB/s (6 key tiles a unit: a sixth of the tiles are the trees' own, and a unit's end costs about 4000 cycles).
 #include "common.cuh"
 
 namespace b200 {

@@ -180,7 +180,7 @@ class RolloutEngine:
                  enable_prefix_caching: bool = False, speculative_tokens: int = 0):
         # ``speculative_tokens``: drafted tokens per sequence and decode step (0: one token per step, as before).  Steps whose
         # sequences all sample without a nucleus (top_p = 1) and where any has a draft are verified steps; they run eagerly, so
-        # they pay where a step is bound by the GPU (large models, long contexts).
+        # they pay where enough is accepted: at 8B with 4 drafts each from 0.8 tokens a step at 64 sequences, 1.8 at 256 on.
         # ``enable_prefix_caching``: full KV blocks outlive their request and serve later requests that start with the same
         # tokens (multi-turn conversations re-submit their history; the reference reaches this through vLLM's
         # ``enable_prefix_caching``, ``open_instruct/vllm_utils.py:1057-1070``).  Without it only the ``n`` samples of one
