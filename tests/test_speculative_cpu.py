@@ -250,6 +250,20 @@ def test_engine_with_drafts_under_preemption_and_with_a_nucleus():
     assert "drafted_tokens" not in eng.stats
 
 
+def test_engine_with_drafts_and_prefix_caching():
+    """Pages filled by verified steps are found again by a follow-up turn."""
+    from open_instruct_b200.data_types import SamplingConfig
+
+    cfg = SamplingConfig(temperature=0.0, max_tokens=90, n=1)
+    plain, spec = _engine(0, num_blocks=64), _engine(4, num_blocks=64, enable_prefix_caching=True)
+    prompts = _prompts()
+    for _ in range(2):
+        a, b = plain.generate(prompts, cfg), spec.generate(prompts, cfg)
+        assert [r.responses for r in a] == [r.responses for r in b]
+        prompts = [p + r.responses[0] + [7, 8, 9] for p, r in zip(prompts, a)]
+    assert spec.stats["prefix_cached_tokens"] > 0 and spec.stats["accepted_tokens"] > 0
+
+
 def test_engine_refuses_drafts_it_cannot_verify():
     from open_instruct_b200.models import get_spec
     from open_instruct_b200.rollout.engine import RolloutEngine
