@@ -18,10 +18,17 @@
 // token in the chunk where the sum passes the coin's share.
 //
 // A sum that decides a token needs more than fp32, though its terms exp(z / temperature - max) are fp32: a vocabulary of 10^5
-// tokens has bins of 10^-5 and less, and fp32 partial sums would move their borders by a share of that.  Every thread adds up
-// its terms as an unevaluated sum of two fp32 numbers (about 48 bits, six additions a term), threads and chunks are joined
-// in fp64.  The statistics' exponentials come from the special-function unit (2^-22 of themselves, like the log-probabilities that
-// leave through fp32).
+// tokens has bins of 10^-5 and less, and fp32 partial sums would move their borders by a share of that.  The last draw's and the
+// residuals' sums are held as unevaluated sums of two fp32 numbers in every thread (about 48 bits, six additions a term), threads
+// and chunks are joined in fp64.
+//
+// The rows' totals from the statistics are sums of fp32 numbers with exponentials from the special-function unit, off by less
+// than 2^-17 of themselves: an exponential 2^x by 2^-22 and by 2^-22 |x| for its argument (|x| <= 18 where it counts, since a row
+// has less than 2^18 terms), the additions by 2^-20.  Probabilities, acceptances with draft probabilities and log-probabilities
+// carry that error.  With certain drafts it would land in full in the mass that rejections leave (1 minus the rejected ones),
+// however small that is, and a token that is all that is left could be rejected.  So an acceptance whose two sides lie closer
+// together than SP_CLOSE is settled by the row's own weights: what is left of the row is summed as for the last draw.  With
+// ordinary coins that is one test in 2^14, at the cost of one CTA reading a row.
 #include "common.cuh"
 
 #include <cooperative_groups.h>
@@ -40,6 +47,8 @@ constexpr int SP_CHUNK = 1024;                       // granules of a chunk of t
 constexpr int SP_CLUSTER = 8;
 constexpr int SP_THREADS = 512;                      // of a walking CTA with draft probabilities; 256 without
 constexpr float SP_LOG2E = 1.4426950408889634f;
+// Certain drafts: u rest and r are each off by less than 2^-17 (the totals' error); this is twice what that adds up to.
+constexpr double SP_CLOSE = 1.0 / 32768;
 
 // A row of logits as aligned 16-byte granules of eight: rows of an odd vocabulary start anywhere, so a row begins `skip` elements
 // into its first granule.  Granules are read whole; what lies outside of the row is replaced by -inf.
@@ -278,6 +287,7 @@ struct WalkSmem {
   float2 rz[SP_MAX_NODES];             // reciprocals of the residuals' sums so far (draft probabilities given), as two fp32 numbers
   double warp_sum[SP_THREADS / 32];
   double cta_sum[2][SP_CLUSTER];       // partial sums of the cluster's CTAs, two passes in turn
+  double rest;                         // mass that rejected point-mass drafts have left of the current node's row
   float top[SP_MAX_NODES];             // largest z / temperature of a node's row
   float u[SP_MAX_NODES];
   int best[SP_MAX_NODES];
@@ -285,6 +295,7 @@ struct WalkSmem {
   int token[SP_MAX_NODES];             // -1: not in the vocabulary
   int gone[SP_MAX_NODES];              // rejected tokens of the current node (point-mass drafts)
   int ngone, nz, cur, k, next, step, pending;
+  int settled;                         // rest is what the row's weights add up to, not what a subtraction left
   int accepted[SP_MAX_NODES];          // positions of the accepted nodes
 };
 
@@ -474,16 +485,18 @@ __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
     sm.p[tid] = p;
     sm.q[tid] = q;
   }
-  if (tid == 0) sm.cur = sm.k = sm.ngone = sm.nz = sm.pending = 0, sm.next = 1;
+  if (tid == 0) sm.cur = sm.k = sm.ngone = sm.nz = sm.pending = sm.settled = 0, sm.next = 1, sm.rest = 1.0;
   __syncthreads();
 
   int pass = 0;
-  // the sum of max(r - q, 0) over the vocabulary at the current node, the same in every CTA of the cluster
+  // What is left at the current node.  Draft probabilities: the sum of max(r - q, 0) over the vocabulary, the same in every CTA of
+  // the cluster.  Certain drafts: the sum of the weights of all tokens that were not rejected.
   auto residual_sum = [&] {
-    const int node = sm.cur, nz = sm.nz;
-    const LeftRow<DRAFT> row(a, n0 + node, temp, sm.top[node], two_of(1.0 / sm.total[node]), sm.rz, nz, nullptr, 0);
+    constexpr int CTAS = DRAFT ? SP_CLUSTER : 1;
+    const int node = sm.cur;
+    const LeftRow<DRAFT> row(a, n0 + node, temp, sm.top[node], two_of(1.0 / sm.total[node]), sm.rz, DRAFT ? sm.nz : 0, sm.gone, DRAFT ? 0 : sm.ngone);
     TwoPair part = {0ull, 0ull};
-    for (int g = rank * threads + tid; g < row.row.count; g += SP_CLUSTER * threads) row.add(row.row.load(g), g, true, part);
+    for (int g = rank * threads + tid; g < row.row.count; g += CTAS * threads) row.add(row.row.load(g), g, DRAFT, part);
     double mine = two_double(part.sum());
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -491,6 +504,7 @@ __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
     __syncthreads();
     double all = 0.0;
     for (int w = 0; w < threads / 32; ++w) all += sm.warp_sum[w];
+    if constexpr (!DRAFT) return all;
     cg::cluster_group cluster = cg::this_cluster();
     if (pass == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (tid < SP_CLUSTER) cluster.map_shared_rank(&sm, tid)->cta_sum[pass & 1][rank] = all;
@@ -502,12 +516,12 @@ __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
     return sum;
   };
 
-  // ---- the walk: one warp, until the nodes run out or a residual has to be summed
+  // ---- the walk: one warp, until the nodes run out or something has to be summed
   while (true) {
     if (warp == 0) {
       int cur = sm.cur, k = sm.k, ngone = sm.ngone, next = sm.next, pending = sm.pending;
-      double rest = 1.0;  // mass that rejected point-mass drafts have left
-      bool sum_first = false;
+      double rest = sm.rest;
+      bool settled = sm.settled, sum_first = false;
       while (next < T) {
         // the next child of the current node
         const bool lo = lane >= next && lane < T && sm.parent[lane] == cur;
@@ -532,6 +546,11 @@ __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
             if (sm.gone[i] == x) r = 0.0;
         }
         const double need = static_cast<double>(sm.u[j]) * (DRAFT ? sm.q[j] : rest);
+        if (!DRAFT && !greedy && !settled && r > 0.0 && fabs(need - r) < SP_CLOSE) {  // too close for these sums
+          sum_first = true;
+          next = j;
+          break;
+        }
         next = j + 1;
         __syncwarp();
         if (x >= 0 && need < r) {
@@ -543,12 +562,14 @@ __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
           cur = j;
           ngone = 0;
           rest = 1.0;
+          settled = false;
         } else if (DRAFT) {
           pending = 1;
         } else if (x >= 0 && r > 0.0) {
           if (lane == 0) sm.gone[ngone] = x;
           ++ngone;
           rest -= r;
+          settled = false;
         }
         __syncwarp();
       }
@@ -558,16 +579,21 @@ __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
         sm.ngone = ngone;
         sm.next = next;
         sm.pending = pending;
+        sm.rest = rest;
+        sm.settled = settled;
         sm.step = sum_first;
       }
     }
     __syncthreads();
-    if (!DRAFT || !sm.step) break;
+    if (!sm.step) break;
     // at temperature 0 all mass is on one token and stays there, whatever is taken off
     const double sum = greedy ? 0.0 : residual_sum();
     __syncthreads();
     if (tid == 0) {
-      if (sum > 0.0) {  // else nothing is left: the residual stays what it was
+      if (!DRAFT) {
+        sm.rest = sum / sm.total[sm.cur];
+        sm.settled = 1;
+      } else if (sum > 0.0) {  // else nothing is left: the residual stays what it was
         const Two r = two_of(1.0 / sum);
         sm.rz[sm.nz++] = make_float2(r.hi, r.lo);
       }
@@ -666,7 +692,7 @@ __global__ void __launch_bounds__(sp_pick_threads(DRAFT), DRAFT ? 1 : 2) verify_
   const float temp = a.temperature[b];
   const double u = static_cast<double>(a.u_sample[b]);
   const double* sums = a.sums + static_cast<long long>(b) * a.chunks;
-  const LeftRow<DRAFT> last(a, e.node, temp, e.top, Two{e.inv_total.x, e.inv_total.y}, e.rz, e.nz, e.gone, e.ngone);
+  LeftRow<DRAFT> last(a, e.node, temp, e.top, Two{e.inv_total.x, e.inv_total.y}, e.rz, e.nz, e.gone, e.ngone);
   bool less = e.less != 0;
   if (tid == 0) {
     pick = a.V;
@@ -750,12 +776,15 @@ __global__ void __launch_bounds__(sp_pick_threads(DRAFT), DRAFT ? 1 : 2) verify_
     }
   }
   __syncthreads();
-  // That chunk.  Rare, where it does not settle the matter (nothing is left: then the residual before the last rejection counts;
-  // a coin of the last share): all chunks for their sum, then one after the other.
+  // That chunk.  Rare, where it does not settle the matter (nothing is left: then what was there before the last rejection
+  // counts, the residual or the rejected token itself; a coin of the last share): all chunks for their sum, then one after the other.
   const bool settled = sum > 0.0 && chunk >= 0;
   double total = 0.0;
   for (int round = settled ? 0 : 1; round < 3; ++round) {
-    if (round == 1 && !(sum > 0.0)) less = false;
+    if (round == 1 && !(sum > 0.0)) {
+      less = false;
+      if (!DRAFT && last.ngone > 0) --last.ngone;
+    }
     double upto = round == 0 ? before : 0.0;
     const double goal = round == 0 ? target : round == 1 ? INFINITY : u * total;
     for (int c = round == 0 ? chunk : 0; c < (round == 0 ? chunk + 1 : a.chunks); ++c) {

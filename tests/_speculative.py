@@ -192,3 +192,35 @@ def logprob_bound(vocab):
     """A log-probability is z - max - log(sum): one fp32 rounding of the argument (|z| <= 64: 2^-18), a sum of fp32 weights (each
     off by 2^-22 of itself, so the sum is), one logarithm and one rounding of the result (below 2^-18 for results up to 32)."""
     return 2.0 ** -16
+
+
+ALMOST_ONE = 1.0 - 2.0 ** -24
+
+
+def make_covered(vocab=64, device="cpu"):
+    """Certain drafts whose siblings take up all, or nearly all, that a row allows: (inputs, expected first tokens, expected counts).
+    A case is the finite logits of a row, the children, their coins and what has to come out."""
+    lone = 1.0 / (1.0 + math.exp(-1.0))          # share of the heavier of two tokens that lie 1 apart
+    cases = [
+        ([(5, 0.0), (9, -12.0)], [5, 9], [ALMOST_ONE, 0.995], 9, 2),     # the first is rejected, so the second is certain
+        ([(5, 0.0), (9, -12.0)], [5, 9], [ALMOST_ONE, ALMOST_ONE], 9, 2),
+        ([(1, 0.3), (2, -0.7), (3, 0.9)], [1, 2, 3], [ALMOST_ONE] * 3, 3, 2),
+        ([(1, 2.5), (2, -3.0), (3, -9.0)], [3, 1, 2], [ALMOST_ONE] * 3, 2, 2),
+        ([(7, 0.0), (8, 0.0), (9, 0.0)], [8, 9, 7], [ALMOST_ONE] * 3, 7, 2),
+        ([(7, 1.0), (8, 0.0)], [7, 7, 8], [ALMOST_ONE] * 3, 8, 2),       # the same token twice: rejected once and for all
+        ([(4, -2.0)], [6, 4], [0.0, ALMOST_ONE], 4, 2),                  # the only token that is left
+    ]
+    for low in (-8.0, -10.0, -12.0, -13.0):      # a heavy token rejected, then one of two light ones with a coin beside its share
+        for off in (-1e-3, -2e-4, 2e-4, 1e-3):
+            cases.append(([(5, 0.0), (9, low), (30, low - 1.0)], [5, 9], [ALMOST_ONE, lone + off], 9 if off < 0 else 30, 2 if off < 0 else 1))
+    counts = [1 + len(c[1]) for c in cases]
+    a = make_verify(counts, vocab, "star", seed=4, device=device)
+    at = 0
+    for finite, kids, coins, _, _ in cases:
+        a["logits"][at] = float("-inf")
+        for x, z in finite:
+            a["logits"][at, x] = z
+        a["tokens"][at + 1:at + 1 + len(kids)] = torch.tensor(kids, device=device)
+        a["u_accept"][at + 1:at + 1 + len(kids)] = torch.tensor(coins, device=device)
+        at += 1 + len(kids)
+    return a, [c[3] for c in cases], [c[4] for c in cases]

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from _speculative import DIM, PAGE, attn_bound, attn_oracle, logprob_bound, make_attn, make_verify, verify_oracle
+from _speculative import DIM, PAGE, attn_bound, attn_oracle, logprob_bound, make_attn, make_covered, make_verify, verify_oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -455,3 +455,24 @@ def test_engine_with_drafts(temperature):
             assert (want.cpu() - torch.tensor(lps)).abs().max() < 0.08 / min(t, 1.0)
             if not temperature:
                 assert (rows.amax(-1) - want).max() < 0.08
+
+
+@pytest.mark.parametrize("vocab", [64, 20011])
+def test_drafts_that_cover_all_that_a_row_allows(vocab):
+    """Certain drafts: a last sibling that is all that is left is accepted, whatever its coin, and what is left beside rejected heavy
+    tokens is shared out by its own weights, not by what a subtraction from 1 leaves of them."""
+    a, first, counts = make_covered(vocab, "cuda")
+    got = _check_verify(a)
+    assert got[1][:, 0].tolist() == first and got[0].tolist() == counts
+
+
+@pytest.mark.parametrize("vocab", [64, 9001])
+def test_coins_of_one_leave_the_last_rejected_draft(vocab):
+    """Coins outside of [0, 1) reject what is certain.  Then nothing is left, the last rejected token stays and is drawn."""
+    from open_instruct_b200.ops import fused
+
+    a, first, _ = make_covered(vocab, "cuda")
+    a["u_accept"].fill_(1.0)
+    want = verify_oracle(a)
+    got = fused.verify_tree(**a)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1]) and torch.isfinite(got[3]).all()
