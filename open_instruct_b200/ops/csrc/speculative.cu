@@ -17,7 +17,7 @@
 // verify_sums_kernel sums what is left in every 8192-column chunk of the row in which a walk ended, verify_pick_kernel finds the
 // token in the chunk where the sum passes the coin's share.
 //
-// A sum that decides a token needs more than fp32, though its terms exp(z / temperature - max) are fp32: a vocabulary of 10^5
+// A sum that decides a token needs more than fp32, though its terms exp((z - max) / temperature) are fp32: a vocabulary of 10^5
 // tokens has bins of 10^-5 and less, and fp32 partial sums would move their borders by a share of that.  The last draw's and the
 // residuals' sums are held as unevaluated sums of two fp32 numbers in every thread (about 48 bits, six additions a term), threads
 // and chunks are joined in fp64.
@@ -81,11 +81,11 @@ struct LogitRow {
 
 // What verify_walk_kernel leaves for the last draw of a sequence.
 struct WalkEnd {
-  double total;              // sum of exp(z / temperature - top) over the row
+  double total;              // sum of exp((z - top) / temperature) over the row
   float2 inv_total;          // its reciprocal, as two fp32 numbers
   float2 rz[SP_MAX_NODES];   // reciprocals of the residuals' sums (draft probabilities given)
   int gone[SP_MAX_NODES];    // rejected tokens (point-mass drafts)
-  float top;                 // largest z / temperature of the row
+  float top;                 // largest z of the row
   int node;                  // batch row in which the walk ended, -1: nothing is left to draw
   int k, nz, ngone, less;    // tokens emitted so far; residuals, rejected tokens; whether one more rejection has to be taken off
 };
@@ -169,7 +169,13 @@ __device__ __forceinline__ double sp_log(double x) {
   return static_cast<double>(e) * 0.69314718055994530942 + (static_cast<double>(logf(m)) + (x - static_cast<double>(f)) / static_cast<double>(f));
 }
 
-__device__ __forceinline__ float sp_weight(float z, float temp, float top) { return expf(__fsub_rn(temp == 1.f ? z : __fdiv_rn(z, temp), top)); }
+// A token's exponent.  The difference first: of two bf16 numbers near one another it is exact, where z / temp and top / temp would
+// each be rounded at their own size (logits of 20 at temperature 0.05: 400, off by 2^-16, and so would the weight be).
+__device__ __forceinline__ float sp_exponent(float z, float temp, float top) {
+  const float d = __fsub_rn(z, top);
+  return temp == 1.f ? d : __fdiv_rn(d, temp);
+}
+__device__ __forceinline__ float sp_weight(float z, float temp, float top) { return expf(sp_exponent(z, temp, top)); }
 __device__ __forceinline__ float sp_logit(const uint4& v, int e) {
   const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
   return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
@@ -281,14 +287,14 @@ __global__ void __launch_bounds__(SP_STAT_THREADS, SP_STAT_CTAS) verify_stats_ke
 }
 
 struct WalkSmem {
-  double total[SP_MAX_NODES];          // sum of exp(z / temperature - top) over a node's row
+  double total[SP_MAX_NODES];          // sum of exp((z - top) / temperature) over a node's row
   double p[SP_MAX_NODES];              // probability of a node's token in its parent's row
   double q[SP_MAX_NODES];              // draft probability of the same
   float2 rz[SP_MAX_NODES];             // reciprocals of the residuals' sums so far (draft probabilities given), as two fp32 numbers
   double warp_sum[SP_THREADS / 32];
   double cta_sum[2][SP_CLUSTER];       // partial sums of the cluster's CTAs, two passes in turn
   double rest;                         // mass that rejected point-mass drafts have left of the current node's row
-  float top[SP_MAX_NODES];             // largest z / temperature of a node's row
+  float top[SP_MAX_NODES];             // largest z of a node's row
   float u[SP_MAX_NODES];
   int best[SP_MAX_NODES];
   int parent[SP_MAX_NODES];
@@ -361,7 +367,7 @@ struct LeftRow {
       for (int k = 0; k < 8; ++k) w[k] = expf(__fsub_rn(sp_logit(v, k), top));
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = expf(__fsub_rn(__fdiv_rn(sp_logit(v, k), temp), top));
+      for (int k = 0; k < 8; ++k) w[k] = expf(__fdiv_rn(__fsub_rn(sp_logit(v, k), top), temp));
     }
     if (drop) {
 #pragma unroll
@@ -468,7 +474,7 @@ __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
       for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
     }
     if (lane == 0) {
-      sm.top[j] = __fdiv_rn(all, temp);
+      sm.top[j] = all;
       sm.total[j] = d;
       sm.best[j] = first >= 0 && first < a.V ? first : 0;
     }
@@ -607,7 +613,7 @@ __device__ __forceinline__ void verify_walk(const VerifyArgs& a, WalkSmem& sm) {
   const int node = sm.cur, k = sm.k;
   auto logprob = [&](int at, int x) {
     const float z = __bfloat162float(a.logits[(n0 + at) * a.ld + x]);
-    return static_cast<float>(static_cast<double>(__fsub_rn(__fdiv_rn(z, temp), sm.top[at])) - sp_log(sm.total[at]));
+    return static_cast<float>(static_cast<double>(sp_exponent(z, temp, sm.top[at])) - sp_log(sm.total[at]));
   };
   for (int i = tid; i < a.max_nodes; i += threads) {
     const bool last = greedy && i == k;  // an accepted draft, or at temperature 0 the last token
@@ -800,7 +806,7 @@ __global__ void __launch_bounds__(sp_pick_threads(DRAFT), DRAFT ? 1 : 2) verify_
     const float z = __bfloat162float(a.logits[e.node * a.ld + x]);
     const long long o = static_cast<long long>(b) * a.max_nodes + e.k;
     a.out_tokens[o] = x;
-    a.logprobs[o] = static_cast<float>(static_cast<double>(__fsub_rn(__fdiv_rn(z, temp), e.top)) - sp_log(e.total));
+    a.logprobs[o] = static_cast<float>(static_cast<double>(sp_exponent(z, temp, e.top)) - sp_log(e.total));
   }
 }
 

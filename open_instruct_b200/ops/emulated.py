@@ -252,8 +252,7 @@ def verify_tree(logits, tokens, parents, cu_nodes, temperature, u_accept, u_samp
         t = float(temperature[b])
 
         def arrive(node):
-            z = logits[node].float() / (t if t > 0 else 1.0)
-            lp = torch.log_softmax(z.double(), -1)
+            lp = torch.log_softmax(logits[node].double() / (t if t > 0 else 1.0), -1)
             if t > 0:
                 return lp, lp.exp()
             p = torch.zeros_like(lp)

@@ -224,3 +224,10 @@ def make_covered(vocab=64, device="cpu"):
         a["u_accept"][at + 1:at + 1 + len(kids)] = torch.tensor(coins, device=device)
         at += 1 + len(kids)
     return a, [c[3] for c in cases], [c[4] for c in cases]
+
+
+def make_cold(vocab=2000, drafted=False, device="cpu", seed=21):
+    """Logits around 20 at temperatures down to 0.05, so that logits / temperature reach several hundreds."""
+    a = make_verify([3, 1, 7, 5, 12, 2, 4, 6], vocab, "tree", drafted, temps=(0.05, 0.1, 0.3, 0.07), seed=seed, device=device)
+    a["logits"] = (0.5 * a["logits"].float() + 20.0).bfloat16()
+    return a

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from open_instruct_b200.ops import emulated, fused
-from _speculative import DIM, PAGE, attn_oracle, logprob_bound, make_attn, make_covered, make_verify, verify_oracle
+from _speculative import DIM, PAGE, attn_oracle, logprob_bound, make_attn, make_cold, make_covered, make_verify, verify_oracle
 
 
 @pytest.mark.parametrize("heads,kv_heads", [(4, 2), (7, 1), (2, 2)])
@@ -293,3 +293,12 @@ def test_drafts_that_cover_all_that_a_row_allows():
         assert torch.equal(x, y.to(x.dtype))
     assert got[1][:, 0].tolist() == first and got[0].tolist() == counts
     assert torch.isfinite(got[3]).all()
+
+
+@pytest.mark.parametrize("drafted", [False, True])
+def test_verification_at_low_temperatures(drafted):
+    a = make_cold(drafted=drafted)
+    got, want = emulated.verify_tree(**a), verify_oracle(a)
+    for x, y in zip(got[:3], want[:3]):
+        assert torch.equal(x, y.to(x.dtype))
+    assert (got[3].double() - want[3]).abs().max() <= logprob_bound(2000)

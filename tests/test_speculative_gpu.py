@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from _speculative import DIM, PAGE, attn_bound, attn_oracle, logprob_bound, make_attn, make_covered, make_verify, verify_oracle
+from _speculative import DIM, PAGE, attn_bound, attn_oracle, logprob_bound, make_attn, make_cold, make_covered, make_verify, verify_oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -476,3 +476,9 @@ def test_coins_of_one_leave_the_last_rejected_draft(vocab):
     want = verify_oracle(a)
     got = fused.verify_tree(**a)
     assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1]) and torch.isfinite(got[3]).all()
+
+
+@pytest.mark.parametrize("drafted", [False, True])
+@pytest.mark.parametrize("vocab", [2000, 40013])
+def test_verification_at_low_temperatures(vocab, drafted):
+    _check_verify(make_cold(vocab, drafted, "cuda"))
