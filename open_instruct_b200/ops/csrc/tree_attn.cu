@@ -5,7 +5,8 @@
 //     o[n, h] = sum_j softmax_j(scale * q[n, h] . k[j]) v[j],   j in {0 .. ctx[b] - 1} and {n, parent(n), parent(parent(n)), ...}.
 // Keys and values of the nodes come from their qkv rows, so nothing of a draft is in the cache before it is accepted.
 // parents[n] is the parent's position inside the sequence (smaller than the node's own), -1 for a root, -2 for padding (a
-// padding row gives zeros).
+// padding row gives zeros, and may hold anything: its scores are replaced, its row of V is cleared in shared memory, since a
+// product takes every row of V and 0 * NaN is NaN).
 //
 // Work.  All nodes of a sequence and all G query heads of a KV head read the same keys, so they are the rows of one matrix
 // product: a row tile holds floor(128 / G) nodes x G heads, a UNIT is up to two row tiles of one (sequence, KV head), its keys
@@ -643,12 +644,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         const int x0 = (grp ^ jc) & 1;           // my first job of this segment; then every second one
         const bool valid = rn < T;
         const unsigned long long sees = valid ? g.sees[rn] : 0ull;
+        const int own = r - (C > (nt - 1) * 128 ? 64 : 0);  // the node whose key is in this thread's row of the tree's tile
+        const bool gap = own >= 0 && own < 64 && g.sees[own] == 0ull;  // there is none, or it is padding
+        // Rows that see cached keys: a padding node's do not, so that its products are zeros.  (Zeros put in when the result is written
+        // cost 4 to 8 us of 295 at one head a group.)
+        const uint32_t alive = ~__ballot_sync(0xffffffffu, valid && !sees);
         const long long seg_at = (static_cast<long long>(g.n0) * a.Hq + g.kvh * a.G) * TA_DH;  // the sequence's first row in the result
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.seg_empty[n & 1]);
         float m = 0.f, l = 0.f;
         // The scores of tile x are there: its keys (as many as 128, fewer in the last tiles) and whether it is the tree's without a
-        // page.  Rows of V that hold no key are cleared: 0 * NaN must not reach the output.
+        // page.  Rows of V that hold no key, or a padding node's, are cleared: 0 * NaN must not reach the output.
         auto begin_job = [&](int x, int& keys, bool& half) -> bool {
           if (!ta_warp_wait(&sm.s_full[grp][0], par_s, abort_flag)) return false;
           par_s ^= 1;
@@ -657,16 +663,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           keys = min(128, C - t * 128);
           half = t == nt - 1 && keys <= 0;
           if (t < nt - 1 && keys == 128) return true;
-          int z0 = keys, z1 = 128, z2 = 128, z3 = 128;  // rows [z0, z1) and [z2, z3) of V are empty
-          if (t == nt - 1) {
-            z0 = max(keys, 0);
-            z1 = half ? 0 : 64;
-            z2 = z1 + T;
-            z3 = z1 + 64;
-          }
+          const bool empty = t < nt - 1 ? r >= keys : gap || (r >= keys && r < 64 && !half);
           const uint32_t vn = rbase + ring_v(x, count);
           if (!ta_warp_wait(&sm.r_full[vn % RING], (vn / RING) & 1, abort_flag)) return false;
-          if ((r >= z0 && r < z1) || (r >= z2 && r < z3)) {
+          if (empty) {
             uint4* row = reinterpret_cast<uint4*>(sm.ring[vn % RING] + r * 128);
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
@@ -689,10 +689,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           // ---- a thread has one key and all 32 rows.  The exponentials are taken against a reference point that starts at 0 and moves
           // to the rows' maxima only if a score exceeds it by 2^40, or if none of a unit's first scores comes up to 2^-40 of it:
           // fp32 and bf16 hold 2^+-126, so in between only the sums' exponents differ.
-          uint32_t word = ~0u;  // the rows that see this key
+          uint32_t word = alive;  // the rows that see this key
           if (t == nt - 1) {
             const int node0 = (half ? lg : lg - 2) * 32;  // keys of the tree in this warp
-            word = r < keys ? ~0u : 0u;
+            word = r < keys ? alive : 0u;
             if (node0 == 0) {
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
@@ -924,6 +924,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         const int rt = two ? grp : 0, node = g.first + rt * a.npt + rn;
         const bool valid = rn < a.npt && node < T;
         const unsigned long long sees = valid ? g.sees[node] : 0ull;
+        const bool empty = g.sees[r & 63] == 0ull;  // the tree has no node, or padding, at this thread's key
+        const bool empties = __any_sync(0xffffffffu, empty);
         const long long out_at = ((static_cast<long long>(g.n0) + node) * a.Hq + g.kvh * a.G + rg) * TA_DH;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.seg_empty[n & 1]);
@@ -939,12 +941,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           const int keys = min(64, C - t * 128 - h * 64);
           const bool tree = t == nt - 1 && (h == 1 || keys <= 0);
           const unsigned long long live = tree ? sees : low_bits(max(keys, 0));
-          const int filled = tree ? T : keys;
-          if (filled < 64) {  // rows of V that hold no key are cleared (by either group: the same zeros): 0 * NaN must not reach the output
+          if (tree ? empties : keys < 64) {  // rows of V that hold no key are cleared (by either group: the same zeros): 0 * NaN must not reach the output
             const uint32_t vn = rbase + ring_v(i, count);
             ok = ta_warp_wait(&sm.r_full[vn % RING], (vn / RING) & 1, abort_flag);
             if (!ok) break;
-            if ((r & 63) >= filled) {
+            if (tree ? empty : (r & 63) >= keys) {
               uint4* row = reinterpret_cast<uint4*>(sm.ring[vn % RING] + (r >> 6) * TA_SUB + (h * 64 + (r & 63)) * 128);
 #pragma unroll
               for (int q = 0; q < 8; ++q) row[(q + lane) & 7] = make_uint4(0u, 0u, 0u, 0u);  // neighbouring rows start in different banks

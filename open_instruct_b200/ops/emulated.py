@@ -221,8 +221,9 @@ def tree_attn(qkv, k_cache, v_cache, block_table, ctx, cu_nodes, parents, n_q: i
         blk = torch.where(there.view(-1), blk, 0)
         old_k = k_cache[blk, :, at % page].float().masked_fill(~there, 0.0) if c else x[:0, :n_kv]
         old_v = v_cache[blk, :, at % page].float().masked_fill(~there, 0.0) if c else x[:0, :n_kv]
+        pad = torch.tensor([p < -1 for p in par[lo:lo + n]], device=qkv.device)
         k = torch.cat([old_k, x[:, n_q:n_q + n_kv]]).repeat_interleave(group, 1)
-        v = torch.cat([old_v, x[:, n_q + n_kv:]]).repeat_interleave(group, 1)
+        v = torch.cat([old_v, x[:, n_q + n_kv:].masked_fill(pad[:, None, None], 0.0)]).repeat_interleave(group, 1)  # 0 * NaN
         live = torch.ones(n, c + n, dtype=torch.bool)
         live[:, c:] = False
         for t in range(n):
@@ -230,7 +231,6 @@ def tree_attn(qkv, k_cache, v_cache, block_table, ctx, cu_nodes, parents, n_q: i
         s = torch.einsum("nhd,jhd->hnj", x[:, :n_q], k) * scale
         s = s.masked_fill(~live.to(s.device), float("-inf"))
         o = torch.einsum("hnj,jhd->nhd", torch.softmax(s, -1), v).reshape(n, -1)
-        pad = torch.tensor([p < -1 for p in par[lo:lo + n]], device=qkv.device)
         out[lo:lo + n] = o.masked_fill(pad[:, None], 0.0).to(qkv.dtype)
     return out
 

@@ -302,3 +302,15 @@ def test_verification_at_low_temperatures(drafted):
     for x, y in zip(got[:3], want[:3]):
         assert torch.equal(x, y.to(x.dtype))
     assert (got[3].double() - want[3]).abs().max() <= logprob_bound(2000)
+
+
+def test_padding_nodes_may_hold_anything():
+    """A padding node's row of qkv is never used: its result is zero and no other node's result is touched."""
+    a = make_attn(4, 2, [70, 0, 30], [6, 5, 3], dtype=torch.float32)
+    pads = [4, 5, 10, 12]
+    a["parents"][pads] = -2
+    a["parents"][[9, 13]] = 0
+    ref, mag = attn_oracle(a)
+    a["qkv"][pads] = float("nan")
+    out = emulated.tree_attn(**a)
+    assert (out[pads] == 0).all() and ((out.double() - ref).abs() <= 2.0 ** -13 * mag + 1e-30).all()

@@ -482,3 +482,29 @@ def test_coins_of_one_leave_the_last_rejected_draft(vocab):
 @pytest.mark.parametrize("vocab", [2000, 40013])
 def test_verification_at_low_temperatures(vocab, drafted):
     _check_verify(make_cold(vocab, drafted, "cuda"))
+
+
+@pytest.mark.parametrize("heads,kv_heads,ctx,counts", [
+    (4, 2, [20, 0, 63], [6, 5, 3]),        # narrow kernel, every unit in one piece
+    (4, 2, [70, 64, 129], [6, 5, 3]),      # the tree beside a page and alone
+    (4, 2, [9000, 0, 30], [6, 5, 3]),      # narrow kernel, joined from parts
+    (16, 1, [20, 0, 100], [6, 5, 3]),      # wide kernel, one row tile
+    (8, 1, [9000, 64, 20], [40, 5, 64]),   # wide kernel, several row tiles
+])
+@pytest.mark.parametrize("garbage", [float("nan"), float("inf")])
+def test_tree_attention_padding_nodes_may_hold_anything(heads, kv_heads, ctx, counts, garbage):
+    """A padding node's row of qkv is never used: its result is zero and no other node's result is touched."""
+    from open_instruct_b200.ops import fused
+
+    a = make_attn(heads, kv_heads, ctx, counts, device="cuda")
+    first = counts[0]
+    pads = [4, 5, first + 1, first + 4, first + counts[1] + 1]
+    at = torch.tensor(pads, device="cuda")
+    par = a["parents"]
+    lost = torch.isin(par, torch.tensor([1, 4, 5], device="cuda", dtype=par.dtype))   # children of padding hang on node 0 instead
+    par[lost] = 0
+    par[at] = -2
+    ref, mag = attn_oracle(a)
+    a["qkv"][at] = garbage
+    got = fused.tree_attn(**a)
+    assert (got[at] == 0).all() and ((got.double() - ref).abs() <= attn_bound(ref, mag)).all()
