@@ -188,7 +188,7 @@ def _ancestors(parents: list, t: int) -> list:
     if parents[t] < -1:
         return []
     seen = [t]
-    while 0 <= parents[t] < t:
+    while 0 <= parents[t] < t and parents[parents[t]] >= -1:   # padding has no descendants: its children are roots
         t = parents[t]
         seen.append(t)
     return sorted(seen)

@@ -521,8 +521,8 @@ def tree_attn(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     ``max_nodes`` <= 64 of them.  A node attends to the first ``ctx[b]`` (int32 [B]) cached tokens of its sequence, found
     through ``block_table`` (int32 [B, pages]) in the caches [blocks, n_kv, 64, head_dim], to its ancestors and to itself.
     ``parents`` (int32 [N]) gives a node's parent as a position inside its own sequence, smaller than the node's own; -1 is a
-    root, -2 padding (its row of the result is zero, its row of ``qkv`` may hold anything).  The nodes' keys and values are read
-    from ``qkv``: the cache does not hold them and is not written.  Cache rows at or past ``ctx`` may hold anything; a page that is
+    root, -2 padding (its row of the result is zero, its row of ``qkv`` may hold anything, a node that names it as its parent is a
+    root).  The nodes' keys and values are read from ``qkv``: the cache does not hold them and is not written.  Cache rows at or past ``ctx`` may hold anything; a page that is
     not in the cache reads as zeros.  Values that are used have to be finite: a NaN or an infinity in a cached value or in a node's
     reaches all nodes of its sequence, those that do not descend from that node too.  One node per sequence is an ordinary decode step.  With ``out`` the rows at and past ``cu_nodes[B]`` are left as they are.  head_dim 128, bf16 only."""
     _need_cuda(qkv, "qkv")

@@ -314,3 +314,14 @@ def test_padding_nodes_may_hold_anything():
     a["qkv"][pads] = float("nan")
     out = emulated.tree_attn(**a)
     assert (out[pads] == 0).all() and ((out.double() - ref).abs() <= 2.0 ** -13 * mag + 1e-30).all()
+
+
+def test_children_of_padding_are_roots():
+    a = make_attn(4, 2, [70, 0], [6, 3], "chain", dtype=torch.float32)
+    a["parents"][[2, 6, 7, 8]] = -2
+    roots = {**a, "parents": a["parents"].clone()}
+    roots["parents"][3] = -1
+    assert a["parents"][3] == 2
+    assert torch.equal(emulated.tree_attn(**a), emulated.tree_attn(**roots))
+    ref, mag = attn_oracle(roots)
+    assert ((emulated.tree_attn(**a).double() - ref).abs() <= 2.0 ** -13 * mag + 1e-30).all()

@@ -508,3 +508,17 @@ def test_tree_attention_padding_nodes_may_hold_anything(heads, kv_heads, ctx, co
     a["qkv"][at] = garbage
     got = fused.tree_attn(**a)
     assert (got[at] == 0).all() and ((got.double() - ref).abs() <= attn_bound(ref, mag)).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (16, 1)])
+def test_tree_attention_children_of_padding_are_roots(heads, kv_heads):
+    """In both kernels; the second sequence is padding alone."""
+    from open_instruct_b200.ops import fused
+
+    a = make_attn(heads, kv_heads, [70, 300, 5], [6, 3, 9], "chain", device="cuda")
+    a["parents"][[2, 6, 7, 8]] = -2
+    roots = {**a, "parents": a["parents"].clone()}
+    roots["parents"][3] = -1
+    got = fused.tree_attn(**a)
+    ref, mag = attn_oracle(roots)
+    assert ((got.double() - ref).abs() <= attn_bound(ref, mag)).all() and (got[6:9] == 0).all()
