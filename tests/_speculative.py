@@ -231,3 +231,24 @@ def make_cold(vocab=2000, drafted=False, device="cpu", seed=21):
     a = make_verify([3, 1, 7, 5, 12, 2, 4, 6], vocab, "tree", drafted, temps=(0.05, 0.1, 0.3, 0.07), seed=seed, device=device)
     a["logits"] = (0.5 * a["logits"].float() + 20.0).bfloat16()
     return a
+
+
+def make_borders(ctx, nodes, heads=4, device="cpu", seed=0):
+    """A long context in which every key at a page's border, the last one too, shows in the output: those keys answer the queries
+    with a score of 6 and have a value of 1 in one dimension each (the i-th in dimension i mod 128, the other keys' values are 0),
+    so an element of the output is the weight of at most ceil(keys / 128) border keys of the same weight, and losing one of them
+    changes it by that share or more.  Returns the inputs and the borders' positions."""
+    a = make_attn(heads, 1, [ctx], [nodes], "chain", seed=seed, device=device, garbage=False)
+    g = torch.Generator().manual_seed(seed + 1)
+    base = torch.randn(DIM, generator=g)
+    q = base + 0.05 * torch.randn(nodes, heads, DIM, generator=g)
+    a["qkv"][:, : heads * DIM] = q.view(nodes, -1).to(device, torch.bfloat16)
+    a["qkv"][:, (heads + 1) * DIM:] = 0.0
+    a["v_cache"].zero_()
+    borders = sorted({p for p in range(ctx) if p % PAGE in (0, PAGE - 1)} | {ctx - 1})
+    key = (base * (6.0 / a["scale"]) / float(base @ base)).to(device, torch.bfloat16)
+    for i, p in enumerate(borders):
+        blk = int(a["block_table"][0, p // PAGE])
+        a["k_cache"][blk, 0, p % PAGE] = key
+        a["v_cache"][blk, 0, p % PAGE, i % DIM] = 1.0
+    return a, borders

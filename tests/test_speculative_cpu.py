@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from open_instruct_b200.ops import emulated, fused
-from _speculative import DIM, PAGE, attn_oracle, logprob_bound, make_attn, make_cold, make_covered, make_verify, verify_oracle
+from _speculative import DIM, PAGE, attn_bound, attn_oracle, logprob_bound, make_attn, make_borders, make_cold, make_covered, make_verify, verify_oracle
 
 
 @pytest.mark.parametrize("heads,kv_heads", [(4, 2), (7, 1), (2, 2)])
@@ -325,3 +325,24 @@ def test_children_of_padding_are_roots():
     assert torch.equal(emulated.tree_attn(**a), emulated.tree_attn(**roots))
     ref, mag = attn_oracle(roots)
     assert ((emulated.tree_attn(**a).double() - ref).abs() <= 2.0 ** -13 * mag + 1e-30).all()
+
+
+@pytest.mark.parametrize("ctx", [383, 4097, 20011])
+def test_long_context_inputs_show_every_border_key(ctx):
+    """What the GPU test of long contexts relies on: leaving out any one key at a page's border moves the result by more than its
+    tolerance (every border key of the shorter contexts, every 37th and the last of the longest)."""
+    a, borders = make_borders(ctx, 1)
+    ref, mag = attn_oracle(a)
+    bound = attn_bound(ref, mag)
+    full = [a["block_table"][0].long(), torch.arange(ctx)]
+    k = a["k_cache"][full[0][full[1] // PAGE], 0, full[1] % PAGE].double()
+    v = a["v_cache"][full[0][full[1] // PAGE], 0, full[1] % PAGE].double()
+    x = a["qkv"][0].double().view(6, DIM)
+    s = torch.cat([x[:4] @ k.t(), x[:4] @ x[4:5].t()], 1) * a["scale"]
+    v = torch.cat([v, x[5:6]])
+    w = torch.exp(s - s.max())
+    top, total = w @ v, w.sum(1, keepdim=True)
+    assert torch.allclose((top / total).reshape(-1), ref[0], rtol=1e-9, atol=1e-15)
+    for p in borders if ctx < 10000 else borders[::37] + [ctx - 1]:
+        less = (top - w[:, p:p + 1] * v[p]) / (total - w[:, p:p + 1])
+        assert ((less.reshape(-1) - ref[0]).abs() > bound[0]).any(), p

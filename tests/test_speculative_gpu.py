@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from _speculative import DIM, PAGE, attn_bound, attn_oracle, logprob_bound, make_attn, make_cold, make_covered, make_verify, verify_oracle
+from _speculative import DIM, PAGE, attn_bound, attn_oracle, logprob_bound, make_attn, make_borders, make_cold, make_covered, make_verify, verify_oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -522,3 +522,10 @@ def test_tree_attention_children_of_padding_are_roots(heads, kv_heads):
     got = fused.tree_attn(**a)
     ref, mag = attn_oracle(roots)
     assert ((got.double() - ref).abs() <= attn_bound(ref, mag)).all() and (got[6:9] == 0).all()
+
+
+@pytest.mark.parametrize("nodes", [1, 5, 40])
+@pytest.mark.parametrize("ctx", [383, 4097, 20011])
+def test_tree_attention_loses_no_key_of_a_long_context(ctx, nodes):
+    """Every key at a page's border shows in the output (the CPU test of these inputs removes them one by one)."""
+    _check_attn(make_borders(ctx, nodes, device="cuda")[0])
