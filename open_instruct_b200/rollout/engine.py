@@ -28,7 +28,7 @@ import torch
 from ..data_types import GenerationResult, RequestInfo, SamplingConfig, TokenStatistics
 from ..models import LlamaModel, ModelSpec
 from ..ops import lib, ref
-from .speculative import PromptLookup, draft_tree, uniforms
+from .speculative import Acceptance, PromptLookup, draft_tree, plan_drafts, step_ms, uniforms
 
 KV_BLOCK = 64
 
@@ -158,6 +158,7 @@ class _Sequence:
     seed: int = 0
     last_token: int = 0
     lookup: object = None  # index of the sequence's n-grams (speculative decoding)
+    chance: object = None  # how often its drafts were right
 
 
 @dataclass
@@ -178,9 +179,10 @@ class RolloutEngine:
                  gpu_memory_utilization: float = 0.85, max_running: int = 256, max_model_len: int = 8192, seed: int = 0,
                  flat: torch.Tensor | None = None, eos_token_ids: list[int] | None = None, tokenizer=None, tp=None,
                  enable_prefix_caching: bool = False, speculative_tokens: int = 0):
-        # ``speculative_tokens``: drafted tokens per sequence and decode step (0: one token per step, as before).  Steps whose
-        # sequences all sample without a nucleus (top_p = 1) and where any has a draft are verified steps; they run eagerly, so
-        # they pay where enough is accepted: at 8B with 4 drafts each from 0.8 tokens a step at 64 sequences, 1.8 at 256 on.
+        # ``speculative_tokens``: drafted tokens per sequence and decode step, at most (0: one token per step, as before).  Steps whose
+        # sequences all sample without a nucleus (top_p = 1) and whose drafts are expected to pay are verified steps
+        # (``speculative.plan_drafts``).  They run eagerly and over more rows: at 8B with 4 drafts each they take 1.3 times an ordinary
+        # step at 32 sequences, 2.0 at 64, 3.2 at 256, so a sequence has to gain 0.3, 1.0 and 2.2 tokens by them.
         # ``enable_prefix_caching``: full KV blocks outlive their request and serve later requests that start with the same
         # tokens (multi-turn conversations re-submit their history; the reference reaches this through vLLM's
         # ``enable_prefix_caching``, ``open_instruct/vllm_utils.py:1057-1070``).  Without it only the ``n`` samples of one
@@ -212,6 +214,7 @@ class RolloutEngine:
                 raise NotImplementedError("speculative decoding is built for attention with head_dim 128 over the whole context, one GPU per engine "
                                           "(no gated-DeltaNet layers, no tensor parallelism, no sliding window shorter than max_model_len)")
         self.speculative_tokens = speculative_tokens
+        self.draft_rows = max_running * (1 + speculative_tokens)   # most rows of a verified step
         dtype = torch.bfloat16 if self.device.type == "cuda" else torch.float32
         self.model = LlamaModel(spec, device=self.device, dtype=dtype, ops=ops, seed=seed, flat=flat)
         if ops == "ref":
@@ -783,16 +786,31 @@ class RolloutEngine:
         self._t_launched = time.perf_counter()
         return results(buf)
 
+    def _step_ms(self, rows: int, drafts: bool) -> float:
+        """Modelled time of a decode step over ``rows`` tokens; ordinary steps of four sequences and more replay a graph."""
+        eager = drafts or self.ops != "fused" or not self.use_cuda_graphs or rows < 4
+        return step_ms(rows, self.spec.num_layers, self.model.flat.numel(), eager)
+
     def _decode(self, seqs: list[_Sequence]) -> None:
-        """One token for every running sequence; with drafts, one and as many as the target confirms."""
+        """One token for every running sequence; with drafts that are expected to pay, one and as many as the target confirms."""
+        if not self.speculative_tokens or any(q.request.sampling.top_p < 1.0 for q in seqs):
+            return self._decode_plain(seqs)
+        ahead = [self._ahead(q) for q in seqs]
+        if any(ahead):
+            most = plan_drafts(ahead, [q.chance for q in seqs], self.speculative_tokens, self.draft_rows, self._step_ms(len(seqs), False),
+                               lambda rows: self._step_ms(rows, True))
+            if most:
+                return self._decode_drafts(seqs, [draft_tree(q.tokens[-1], chains, most) for q, chains in zip(seqs, ahead)])
+        self._decode_plain(seqs)
+        for q, chains in zip(seqs, ahead):
+            if chains:  # what a draft would have gained
+                q.chance.record(q.tokens[-1] in [chain[0] for chain in chains], 1)
+
+    def _decode_plain(self, seqs: list[_Sequence]) -> None:
+        """One token for every running sequence."""
         s = self.spec
         dev = self.device
         B = len(seqs)
-        if self.speculative_tokens and all(q.request.sampling.top_p >= 1.0 for q in seqs):
-            ahead = [self._ahead(q) for q in seqs]
-            if any(ahead):
-                self._decode_drafts(seqs, [draft_tree(q.tokens[-1], chains, self.speculative_tokens) for q, chains in zip(seqs, ahead)])
-                return
         if self.ops == "fused":
             t0 = time.perf_counter()
             self._t_launched = None
@@ -863,7 +881,7 @@ class RolloutEngine:
     def _ahead(self, seq: _Sequence) -> list:
         """What may come next in one sequence, no longer than the tokens it may still emit and the pages it holds."""
         if seq.lookup is None:
-            seq.lookup = PromptLookup()
+            seq.lookup, seq.chance = PromptLookup(), Acceptance()
         ahead = seq.lookup.continuations(seq.tokens, self.speculative_tokens)
         if ahead:
             n = len(seq.tokens)
@@ -915,7 +933,9 @@ class RolloutEngine:
         count, tokens, logprobs = count.tolist(), tokens.tolist(), logprobs.tolist()
         self.stats["drafted_tokens"] = self.stats.get("drafted_tokens", 0) + len(at) - B
         self.stats["accepted_tokens"] = self.stats.get("accepted_tokens", 0) + sum(count) - B
-        for q, n, toks, lps in zip(seqs, count, tokens, logprobs):
+        for q, n, toks, lps, (_, _, depths) in zip(seqs, count, tokens, logprobs, drafts):
+            if len(depths) > 1:
+                q.chance.record(n - 1, min(n, max(depths)))
             for t, lp in zip(toks[:n], lps):
                 self._accept(q, t, lp)
                 self.stats["decode_tokens"] += 1

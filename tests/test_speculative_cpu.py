@@ -346,3 +346,62 @@ def test_long_context_inputs_show_every_border_key(ctx):
     for p in borders if ctx < 10000 else borders[::37] + [ctx - 1]:
         less = (top - w[:, p:p + 1] * v[p]) / (total - w[:, p:p + 1])
         assert ((less.reshape(-1) - ref[0]).abs() > bound[0]).any(), p
+
+
+def test_a_verified_step_has_to_pay():
+    """Which steps draft: the expected tokens against the steps' modelled times."""
+    from open_instruct_b200.rollout.speculative import DECODE_ROWS, Acceptance, plan_drafts, step_ms
+
+    def chance(hits, trials):
+        c = Acceptance()
+        for _ in range(30):
+            c.record(hits, trials)
+        return c
+
+    c = Acceptance()
+    assert c.expected(1) == 0.5 and c.expected(3) == 0.875 and c.expected(0) == 0.0
+    good, poor = chance(4, 4), chance(0, 1)
+    assert 3.5 < good.expected(4) < 4.0 and poor.expected(4) < 0.1
+
+    def plan(ahead, chances, most=4, rows=1 << 20, graphs=True):
+        model = lambda rows, eager: step_ms(rows, 32, 8_030_000_000, eager)
+        return plan_drafts(ahead, chances, most, rows, model(len(ahead), not graphs), lambda n: model(n, True))
+
+    draft, none = [[1, 2, 3, 4]], []
+    for batch, nodes in ((16, 4), (64, 3), (256, 4)):                                  # 64 of 1 + 3 nodes are the decode GEMMs' 256 rows
+        assert plan([draft] * batch, [good] * batch) == nodes                          # nearly all is accepted
+        assert plan([draft] * batch, [poor] * batch) == 0                              # nearly nothing is
+        assert plan([draft] + [none] * (batch - 1), [good] * batch) == 0               # one sequence of many
+    assert plan([draft], [poor], graphs=False) == 4                                    # a lone sequence has little to lose
+    # two tokens each would leave the decode GEMMs, one stays
+    fair = chance(3, 5)
+    assert plan([[[1, 2]]] * 120, [fair] * 120, most=2) in (0, 1)
+    assert plan([[[1, 2]]] * 120, [good] * 120, most=2, rows=240) == 1 and DECODE_ROWS == 256
+    assert plan([draft] * 8, [good] * 8, rows=8) == 0                                  # no room for a single node
+    assert plan([draft] * 8, [good] * 8, rows=16) == 1
+
+
+def test_one_drafting_sequence_does_not_move_a_batch_off_its_ordinary_steps():
+    from open_instruct_b200.data_types import SamplingConfig
+
+    prompts = [list(range(5 + 9 * i, 25 + 9 * i)) for i in range(8)]
+    cfg = SamplingConfig(temperature=0.0, max_tokens=12, min_tokens=12, n=1)
+    want = [r.responses for r in _engine(0, num_blocks=64).generate(prompts, cfg)]
+    right = {tuple(p): r[0] for p, r in zip(prompts, want)}
+
+    def run(drafting):
+        eng = _engine(3, num_blocks=64)
+        eng._step_ms = lambda rows, drafts: 1.5 if drafts else 1.0
+        ahead = eng._ahead
+
+        def foresee(q):   # the right tokens for the drafting sequences
+            ahead(q)
+            prompt, n = tuple(q.tokens[: q.prompt_len]), len(q.tokens) - q.prompt_len
+            chain = right[prompt][n:n + 3][: q.request.sampling.max_tokens - n - 1]
+            return [chain] if chain and prompts.index(list(prompt)) < drafting else []
+
+        eng._ahead = foresee
+        assert [r.responses for r in eng.generate(prompts, cfg)] == want
+        return eng.stats
+
+    assert "drafted_tokens" not in run(1) and run(8)["accepted_tokens"] > 20
