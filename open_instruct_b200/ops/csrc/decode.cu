@@ -444,7 +444,7 @@ decode_combine_kernel(const float* __restrict__ part_o, const float* __restrict_
 }
 
 // ------------------------------------------------------------------ sampling
-// Philox4x32-10 counter RNG: (seed, row counter, token index) -> uniform in (0, 1).
+// Philox4x32-10 counter RNG: (seed, row counter, token index) -> n in 0 .. 2^24 - 1, for the uniform number (n + 1/2) / 2^24.
 __device__ __forceinline__ void philox_round(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
   const uint64_t p0 = static_cast<uint64_t>(0xD2511F53u) * c[0];
   const uint64_t p1 = static_cast<uint64_t>(0xCD9E8D57u) * c[2];
@@ -455,7 +455,7 @@ __device__ __forceinline__ void philox_round(uint32_t (&c)[4], uint32_t k0, uint
   c[0] = n0;
   c[2] = n2;
 }
-__device__ __forceinline__ float philox_uniform(uint64_t seed, uint32_t ctr_hi, uint32_t ctr_lo, uint32_t idx) {
+__device__ __forceinline__ uint32_t philox_uniform(uint64_t seed, uint32_t ctr_hi, uint32_t ctr_lo, uint32_t idx) {
   uint32_t c[4] = {idx, ctr_lo, ctr_hi, 0u};
   uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
 #pragma unroll
@@ -464,7 +464,18 @@ __device__ __forceinline__ float philox_uniform(uint64_t seed, uint32_t ctr_hi, 
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  return (static_cast<float>(c[0] >> 8) + 0.5f) * (1.0f / 16777216.0f);
+  return c[0] >> 8;
+}
+// -log of the uniform number.  Near 1 its fp32 form would not do: n = 2^24 - 1 rounds to 1, whose Gumbel number is infinite, so any
+// token with that n was drawn, however unlikely (one draw in 130 from 128256 tokens); and the fast logarithm is off by 2^-23 of 1, as
+// much as the last few numbers' own logarithms.  So below w = 1 - u = 2^-8, where w is exact and the logarithm's error would pass
+// 2^-15 of itself, the series of -log(1 - w) takes over (off by w^3 / 4 < 2^-26 of itself; one warp in nine has such a number).
+__device__ __forceinline__ float neg_log_uniform(uint32_t n) {
+  if (n >= 0xff0000u) {
+    const float w = (static_cast<float>(0xffffffu - n) + 0.5f) * (1.0f / 16777216.0f);
+    return w * fmaf(w, fmaf(w, 1.0f / 3.0f, 0.5f), 1.0f);
+  }
+  return -__logf((static_cast<float>(n) + 0.5f) * (1.0f / 16777216.0f));
 }
 
 struct ArgMax {
@@ -553,8 +564,7 @@ sample_kernel(const __nv_bfloat16* __restrict__ logits, long long ld, int V, con
       score = z;
     } else {
       if (__expf(z) < thr) continue;
-      const float u = philox_uniform(seed, 0u, ctr, static_cast<uint32_t>(i));
-      score = z - __logf(-__logf(u));
+      score = z - __logf(neg_log_uniform(philox_uniform(seed, 0u, ctr, static_cast<uint32_t>(i))));
     }
     best = argmax_merge(best, ArgMax{score, i});
   }

@@ -187,3 +187,40 @@ def test_fused_rope_and_kv_write_matches_the_two_kernels():
     torch.cuda.synchronize()
     assert torch.equal(a, b) and torch.equal(kc1, kc2) and torch.equal(vc1, vc2)
     assert kc1.abs().sum() > 0 and vc1.abs().sum() > 0
+
+
+def test_sampler_kernel_at_the_top_of_the_uniform_numbers():
+    """Tokens whose uniform number is one of the three largest: their Gumbel numbers are finite, so a token of weight e^-60 is not
+    drawn, and they are exact enough that the drawn token changes where its exact score does.  Scores are z + g; fp32 leaves g off by
+    less than 2^-18 and z by 2^-18 (|z| <= 60), so 0.05 on either side of the border is far outside of that."""
+    import numpy as np
+
+    from open_instruct_b200.ops.lib import call, ptr, stream_ptr
+    from open_instruct_b200.rollout.sampler import philox_uniform
+
+    V, other = 128256, 5
+    top = [(227, 94317, 0), (495, 30102, 0), (520, 53449, 0), (51, 109084, 1), (63, 85396, 1), (194, 80566, 1), (23, 18365, 2), (295, 18239, 2)]
+    rows, want, ctr = [], [], []
+    for c, token, k in top:
+        u, v = philox_uniform(0, c, np.array([token, other], dtype=np.uint32))
+        assert u == (2.0 ** 24 - 0.5 - k) / 2.0 ** 24
+        border = -np.log(-np.log(v)) + np.log(-np.log(u))   # where z of the token makes it even with z = 0 of the other one
+        lower = upper = torch.tensor(border).bfloat16()
+        while float(lower) > border - 0.05:
+            lower = torch.nextafter(lower, torch.tensor(-1e9).bfloat16())
+        while float(upper) < border + 0.05:
+            upper = torch.nextafter(upper, torch.tensor(1e9).bfloat16())
+        for z, expect in ((torch.tensor(-60.0), other), (lower, other), (upper, token)):
+            rows.append((token, float(z)))
+            want.append(expect)
+            ctr.append(c)
+    B = len(rows)
+    logits = torch.full((B, V), -1e4, dtype=torch.bfloat16)
+    for i, (token, z) in enumerate(rows):
+        logits[i, token], logits[i, other] = z, 0.0
+    logits = logits.cuda()
+    temp, top_p = torch.ones(B, device="cuda"), torch.ones(B, device="cuda")
+    seeds, ctr = torch.zeros(B, dtype=torch.int64, device="cuda"), torch.tensor(ctr, dtype=torch.int32, device="cuda")
+    toks, lps = torch.empty(B, dtype=torch.int64, device="cuda"), torch.empty(B, device="cuda")
+    call("b200_sample", ptr(logits), logits.stride(0), B, V, ptr(temp), ptr(top_p), ptr(seeds), ptr(ctr), ptr(toks), ptr(lps), stream_ptr())
+    assert toks.tolist() == want
