@@ -34,10 +34,15 @@ class PromptLookup:
         self.seen = len(tokens)
 
     def continuations(self, tokens: list, length: int) -> list:
-        """What followed the last n-gram before, latest first: lists of at most ``length`` tokens."""
+        """What followed the last n-gram before, latest first: lists of at most ``length`` tokens, none the beginning of another."""
         self.update(tokens)
         at = self.behind.get(tuple(tokens[-self.ngram:])) if len(tokens) >= self.ngram and length > 0 else None
-        return [tokens[p:p + length] for p in at] if at else []
+        found = [tokens[p:p + length] for p in at] if at else []
+        if len(found) == 2:
+            short, long = sorted(found, key=len)
+            if long[:len(short)] == short:
+                return [long]
+        return found
 
 
 class Acceptance:
@@ -50,10 +55,13 @@ class Acceptance:
         self.hits = 0.9 * self.hits + hits
         self.trials = 0.9 * self.trials + trials
 
-    def expected(self, depth: int) -> float:
-        """Tokens that a draft of ``depth`` tokens in a row is expected to add."""
-        rate = (self.hits + 1.0) / (self.trials + 2.0)
-        return rate * (1.0 - rate ** depth) / (1.0 - rate)
+    def rate(self) -> float:
+        return (self.hits + 1.0) / (self.trials + 2.0)
+
+
+def expected_tokens(rate, depth):
+    """What drafts of ``depth`` tokens in a row are expected to add, each token being right with probability ``rate`` < 1."""
+    return rate * (1.0 - rate ** depth) / (1.0 - rate)
 
 
 DECODE_ROWS = 256  # rows up to which the projections run on the decode GEMMs
@@ -71,24 +79,40 @@ def step_ms(rows: int, layers: int, weights: int, eager: bool) -> float:
 
 
 def plan_drafts(ahead: list, chances: list, most: int, rows: int, plain: float, verified) -> int:
-    """How many nodes each sequence may draft in this step: as many as ``most`` and ``rows`` tokens in all allow, or so few that the
-    step stays within the decode GEMMs' rows, or 0 where an ordinary step emits more tokens a millisecond.  ``ahead``: the sequences'
-    continuations; ``chances``: their ``Acceptance``; ``plain``: the time of an ordinary step; ``verified(rows)``: of a verified one."""
+    """How many nodes each sequence may draft in this step, 0 where an ordinary step emits more tokens a millisecond.  Looked at are
+    as many as ``most`` and ``rows`` tokens in all allow, the halves of that, and as many as the decode GEMMs' rows allow.  ``ahead``:
+    the sequences' continuations; ``chances``: their ``Acceptance``; ``plain``: the time of an ordinary step; ``verified(rows)``: of a
+    verified one."""
     batch = len(ahead)
-    nodes = [min(most, sum(map(len, chains))) for chains in ahead]
-    drafting = [(chance, chains) for chance, chains in zip(chances, ahead) if chains]
-    best, rate = 0, batch / plain
-    for limit in (rows, min(rows, DECODE_ROWS)):
-        low, high = 0, most   # the largest share whose total fits
+    # drafts without end add rate / (1 - rate): most steps that do not pay are told by that alone
+    if batch + sum((c.hits + 1.0) / (c.trials - c.hits + 1.0) for c, chains in zip(chances, ahead) if chains) <= batch / plain * verified(batch + 1):
+        return 0
+    nodes = np.array([sum(map(len, chains)) for chains in ahead])
+    first = np.array([len(chains[0]) if chains else 0 for chains in ahead])
+    several = np.array([len(chains) > 1 for chains in ahead])
+    rate = np.array([chance.rate() for chance in chances])
+
+    def total(share):
+        return batch + int(np.minimum(nodes, share).sum())
+
+    def largest(limit):  # share whose total fits
+        low, high = 0, most
         while low < high:
             mid = (low + high + 1) // 2
-            low, high = (mid, high) if batch + sum(min(n, mid) for n in nodes) <= limit else (low, mid - 1)
-        if low == 0:
-            continue
-        expected = sum(chance.expected(min(len(chains[0]), _first_share(low, len(chains)))) for chance, chains in drafting)
-        got = (batch + expected) / verified(batch + sum(min(n, low) for n in nodes))
-        if got > rate:
-            best, rate = low, got
+            low, high = (mid, high) if total(mid) <= limit else (low, mid - 1)
+        return low
+
+    shares = {largest(min(rows, DECODE_ROWS))}
+    share = largest(rows)
+    while share:
+        shares.add(share)
+        share //= 2
+    best, speed = 0, batch / plain
+    for share in sorted(shares - {0}):
+        depth = np.minimum(first, np.where(several, _first_share(share, 2), share))
+        got = (batch + float(expected_tokens(rate, depth).sum())) / verified(total(share))
+        if got > speed:
+            best, speed = share, got
     return best
 
 

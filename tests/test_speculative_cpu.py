@@ -350,7 +350,7 @@ def test_long_context_inputs_show_every_border_key(ctx):
 
 def test_a_verified_step_has_to_pay():
     """Which steps draft: the expected tokens against the steps' modelled times."""
-    from open_instruct_b200.rollout.speculative import DECODE_ROWS, Acceptance, plan_drafts, step_ms
+    from open_instruct_b200.rollout.speculative import DECODE_ROWS, Acceptance, expected_tokens, plan_drafts, step_ms
 
     def chance(hits, trials):
         c = Acceptance()
@@ -358,10 +358,9 @@ def test_a_verified_step_has_to_pay():
             c.record(hits, trials)
         return c
 
-    c = Acceptance()
-    assert c.expected(1) == 0.5 and c.expected(3) == 0.875 and c.expected(0) == 0.0
+    assert Acceptance().rate() == 0.5 and [expected_tokens(0.5, d) for d in (0, 1, 3)] == [0.0, 0.5, 0.875]
     good, poor = chance(4, 4), chance(0, 1)
-    assert 3.5 < good.expected(4) < 4.0 and poor.expected(4) < 0.1
+    assert 0.95 < good.rate() < 1.0 and poor.rate() < 0.1
 
     def plan(ahead, chances, most=4, rows=1 << 20, graphs=True):
         model = lambda rows, eager: step_ms(rows, 32, 8_030_000_000, eager)
@@ -379,6 +378,8 @@ def test_a_verified_step_has_to_pay():
     assert plan([[[1, 2]]] * 120, [good] * 120, most=2, rows=240) == 1 and DECODE_ROWS == 256
     assert plan([draft] * 8, [good] * 8, rows=8) == 0                                  # no room for a single node
     assert plan([draft] * 8, [good] * 8, rows=16) == 1
+    # as many as the drafter offers are too many, fewer pay
+    assert 0 < plan([[list(range(32))]] * 256, [good] * 256, most=32) < 32
 
 
 def test_one_drafting_sequence_does_not_move_a_batch_off_its_ordinary_steps():
@@ -405,3 +406,12 @@ def test_one_drafting_sequence_does_not_move_a_batch_off_its_ordinary_steps():
         return eng.stats
 
     assert "drafted_tokens" not in run(1) and run(8)["accepted_tokens"] > 20
+
+
+def test_continuations_that_agree_are_one_draft():
+    from open_instruct_b200.rollout.speculative import PromptLookup
+
+    toks = [1, 2, 3, 4, 5, 9, 1, 2, 3, 4, 5, 8, 1, 2]
+    assert PromptLookup(2).continuations(toks, 3) == [[3, 4, 5]]
+    assert PromptLookup(2).continuations(toks, 4) == [[3, 4, 5, 8], [3, 4, 5, 9]]
+    assert PromptLookup(1).continuations([7, 7, 7], 4) == [[7, 7]]   # the latest one is cut by the end of the text
