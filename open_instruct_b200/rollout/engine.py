@@ -31,6 +31,7 @@ from ..ops import lib, ref
 from .speculative import Acceptance, PromptLookup, draft_tree, plan_drafts, step_ms, uniforms
 
 KV_BLOCK = 64
+DRAFT_ROWS = 4096   # nodes of all sequences in one verified step, at most
 
 
 class _Host:
@@ -214,7 +215,8 @@ class RolloutEngine:
                 raise NotImplementedError("speculative decoding is built for attention with head_dim 128 over the whole context, one GPU per engine "
                                           "(no gated-DeltaNet layers, no tensor parallelism, no sliding window shorter than max_model_len)")
         self.speculative_tokens = speculative_tokens
-        self.draft_rows = max_running * (1 + speculative_tokens)   # most rows of a verified step
+        # most rows of a verified step; no more than a few thousand, since the tensor cores have long been busy by then
+        self.draft_rows = min(max_running * (1 + speculative_tokens), DRAFT_ROWS) if speculative_tokens else 0
         dtype = torch.bfloat16 if self.device.type == "cuda" else torch.float32
         self.model = LlamaModel(spec, device=self.device, dtype=dtype, ops=ops, seed=seed, flat=flat)
         if ops == "ref":
@@ -227,6 +229,7 @@ class RolloutEngine:
         if num_blocks is None:
             if self.device.type == "cuda":
                 free, total = torch.cuda.mem_get_info(self.device)
+                free -= self.draft_bytes(spec, self.draft_rows)
                 num_blocks = max(16, int((free - (1 - gpu_memory_utilization) * total) // per_block))
             else:
                 num_blocks = 256
@@ -263,6 +266,17 @@ class RolloutEngine:
         self._gdn_runs: list = []   # (first row, end row, sequence continued or None, sequences that receive the new state) of the pass in flight
         self._stages: dict = {}  # pinned staging blobs of the decode step, by batch size
         self._last_sids = None
+
+    @staticmethod
+    def draft_bytes(spec: ModelSpec, rows: int) -> int:
+        """Device memory that a verified step over ``rows`` tokens takes (bf16): the qkv rows of all layers until the commit, the logits of
+        all nodes, one layer's activations (the MLP's two projections and their product, twelve rows of the hidden size), and the
+        workspaces of tree attention (39 MB at most) and verification (12 bytes for 2048 logits)."""
+        if not rows:
+            return 0
+        width = (spec.num_heads + 2 * spec.num_kv_heads) * spec.head_dim
+        per_row = 2 * (spec.num_layers * width + spec.vocab_size + 3 * spec.intermediate_size + 12 * spec.hidden_size) + spec.vocab_size // 100
+        return rows * per_row + (64 << 20)
 
     # ------------------------------------------------------------------ public API
     def kv_cache_max_concurrency(self, seq_len: int) -> int:

@@ -415,3 +415,24 @@ def test_continuations_that_agree_are_one_draft():
     assert PromptLookup(2).continuations(toks, 3) == [[3, 4, 5]]
     assert PromptLookup(2).continuations(toks, 4) == [[3, 4, 5, 8], [3, 4, 5, 9]]
     assert PromptLookup(1).continuations([7, 7, 7], 4) == [[7, 7]]   # the latest one is cut by the end of the text
+
+
+def test_a_verified_step_is_bounded_and_its_memory_is_set_aside(monkeypatch):
+    """No step has more nodes than ``draft_rows``, whatever the sequences offer, and an engine that sizes its own cache leaves room
+    for such a step."""
+    from open_instruct_b200.data_types import SamplingConfig
+    from open_instruct_b200.models import get_spec
+    from open_instruct_b200.rollout.engine import DRAFT_ROWS, RolloutEngine
+
+    eng = _engine(63, num_blocks=64, max_running=8)
+    assert eng.draft_rows == 8 * 64 and _engine(0, num_blocks=16).draft_rows == 0
+    eng.draft_rows, seen = 20, []
+    drafts = eng._decode_drafts
+    eng._decode_drafts = lambda seqs, trees: (seen.append(sum(len(t) for t, _, _ in trees)), drafts(seqs, trees))
+    cfg = SamplingConfig(temperature=0.0, max_tokens=70, n=2)
+    a, b = eng.generate(_prompts(), cfg), _engine(0, num_blocks=64).generate(_prompts(), cfg)
+    assert [r.responses for r in a] == [r.responses for r in b] and 6 < max(seen) <= 20
+    spec = get_spec("llama3.1-8b")
+    rows = min(256 * 64, DRAFT_ROWS)
+    assert RolloutEngine.draft_bytes(spec, 0) == 0
+    assert RolloutEngine.draft_bytes(spec, rows) > rows * 2 * (32 * 48 * 128 + spec.vocab_size)

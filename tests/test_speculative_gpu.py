@@ -529,3 +529,31 @@ def test_tree_attention_children_of_padding_are_roots(heads, kv_heads):
 def test_tree_attention_loses_no_key_of_a_long_context(ctx, nodes):
     """Every key at a page's border shows in the output (the CPU test of these inputs removes them one by one)."""
     _check_attn(make_borders(ctx, nodes, device="cuda")[0])
+
+
+def test_a_verified_step_takes_no_more_memory_than_is_set_aside():
+    from open_instruct_b200.data_types import SamplingConfig
+    from open_instruct_b200.models import get_spec
+    from open_instruct_b200.rollout.engine import RolloutEngine
+
+    spec = get_spec("llama3.2-1b").replace(head_dim=128, num_heads=16, num_kv_heads=4, num_layers=6, eos_token_id=None)
+    eng = RolloutEngine(spec, device="cuda", ops="fused", num_blocks=400, max_running=32, max_model_len=1024, seed=3, eos_token_ids=[], speculative_tokens=31)
+    assert eng.draft_rows == 1024
+    eng._step_ms = lambda rows, drafts: 1.0 if drafts else 100.0
+    peaks, drafts = [], eng._decode_drafts
+
+    def watched(seqs, trees):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        drafts(seqs, trees)
+        rows = sum(len(t) for t, _, _ in trees)
+        peaks.append((rows, torch.cuda.max_memory_allocated() - before))
+
+    eng._decode_drafts = watched
+    ahead = eng._ahead
+    eng._ahead = lambda q: (ahead(q), [[(q.tokens[-1] + i) % spec.vocab_size for i in range(1, 32)]] if len(q.tokens) < 60 else [])[1]
+    eng.generate([[5 + i, 6, 7] for i in range(32)], SamplingConfig(temperature=0.0, max_tokens=70, min_tokens=70, n=1))
+    assert max(peaks)[0] == 1024
+    for rows, peak in peaks:
+        assert peak <= eng.draft_bytes(spec, rows), (rows, peak, eng.draft_bytes(spec, rows))
