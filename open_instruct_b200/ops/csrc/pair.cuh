@@ -43,6 +43,9 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The one wait without a limit.  A pair that started on SMs the moment single CTAs with tensor memory of their own had left them
+// did not return from here, so a kernel of such CTAs and one of pairs must not overlap: nothing is launched early behind the join of
+// the tree attention, and callers keep the two kinds on one stream.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(ncols)
                : "memory");

@@ -521,10 +521,20 @@ def tree_attn(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     ``max_nodes`` <= 64 of them.  A node attends to the first ``ctx[b]`` (int32 [B]) cached tokens of its sequence, found
     through ``block_table`` (int32 [B, pages]) in the caches [blocks, n_kv, 64, head_dim], to its ancestors and to itself.
     ``parents`` (int32 [N]) gives a node's parent as a position inside its own sequence, smaller than the node's own; -1 is a
-    root, -2 padding (its row of the result is zero, its row of ``qkv`` may hold anything, a node that names it as its parent is a
-    root).  The nodes' keys and values are read from ``qkv``: the cache does not hold them and is not written.  Cache rows at or past ``ctx`` may hold anything; a page that is
-    not in the cache reads as zeros.  Values that are used have to be finite: a NaN or an infinity in a cached value or in a node's
-    reaches all nodes of its sequence, those that do not descend from that node too.  One node per sequence is an ordinary decode step.  With ``out`` the rows at and past ``cu_nodes[B]`` are left as they are.  head_dim 128, bf16 only."""
+    root, -2 padding (its row of the result is zero, its row of ``qkv`` may hold anything, a node that names it as its parent is
+    a root).  The nodes' keys and values are read from ``qkv``: the cache does not hold them and is not written.  Cache rows at
+    or past ``ctx`` may hold anything; a page that is not in the cache reads as zeros.  Values that are used have to be finite: a
+    NaN or an infinity in a cached value or in a node's reaches all nodes of its sequence, those that do not descend from that
+    node too.  One node per sequence is an ordinary decode step.  With ``out`` the rows at and past ``cu_nodes[B]`` are left as
+    they are.  head_dim 128, bf16 only.
+
+    Scores, maxima and sums are fp32; the softmax weights are rounded to bf16 before they meet the values, as the tensor cores
+    take them (the engine's one-token attention keeps them in fp32): the error against 64 bits is 1.4 times that of an fp32
+    softmax whose result is rounded to bf16.
+
+    Streams: the kernel holds tensor memory with single CTAs, the GEMMs of this package with pairs of CTAs (``gemm``, ``gemm_decode``).
+    Do not let a call and such a GEMM run at the same time on two streams of one device: a pair that starts on SMs which this
+    kernel has just left may wait for its tensor memory without limit.  On one stream they never overlap."""
     _need_cuda(qkv, "qkv")
     _check_tree_attn(qkv, k_cache, v_cache, block_table, ctx, cu_nodes, parents, n_q, n_kv, head_dim, scale, max_nodes, out, torch.bfloat16)
     dev, N, B = qkv.device, qkv.shape[0], ctx.shape[0]

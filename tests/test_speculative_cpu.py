@@ -436,3 +436,19 @@ def test_a_verified_step_is_bounded_and_its_memory_is_set_aside(monkeypatch):
     rows = min(256 * 64, DRAFT_ROWS)
     assert RolloutEngine.draft_bytes(spec, 0) == 0
     assert RolloutEngine.draft_bytes(spec, rows) > rows * 2 * (32 * 48 * 128 + spec.vocab_size)
+
+
+def test_nothing_is_launched_early_behind_the_join_of_the_tree_attention():
+    """The decode GEMMs' pairs of CTAs must not start on SMs that the attention is leaving (their allocation of tensor memory has no
+    limit on its wait): the join waits for the attention and lets nothing start before its own end."""
+    from pathlib import Path
+
+    import open_instruct_b200.ops as ops
+
+    src = (Path(ops.__file__).parent / "csrc" / "tree_attn.cu").read_text()
+    at = src.index("tree_join_kernel(const __grid_constant__ TreeArgs a) {")
+    body = src[at:src.index("\n}\n", at)]
+    assert "griddep_wait();" in body and "griddep_launch_dependents" not in body
+    launch = src[src.index('extern "C" int b200_tree_attn('):]
+    assert launch.index("ta_launch<true>") < launch.index("tree_join_kernel")   # and it is the last kernel of the call
+    assert "launch" not in launch[launch.index("tree_join_kernel"):].split("\n", 1)[1]
