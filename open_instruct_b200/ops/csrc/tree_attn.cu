@@ -27,9 +27,10 @@
 // keys are loaded once for both); a unit of one row tile gives each group its half of every key tile, merged at the end.  Each
 // group has its own product thread and two buffers for S, so the next scores are there when a step's softmax is through.  P
 // replaces S in tensor memory (bf16), O stays there for the whole unit and is rescaled only when the row maximum has grown by
-// more than 2^8.  Measured: 16 trees of 64 nodes, 8 heads a KV head, contexts of 8192 to 32768: 697 GFLOP in 815 to 900 us = 775
-// to 855 TFLOP/s; the GPU is at its 1000 W limit by then and holds the SM clock at 1.5 GHz, where steps of 128 keys with one
-// product thread (4 % behind), a later start of the second group, and scores fetched a step ahead (12 % behind) make no gain.
+// more than 2^8.  Measured: 16 trees of 64 nodes, 8 heads a KV head, contexts of 8192 to 32768: 697 GFLOP in 815 to 910 us = 765
+// to 855 TFLOP/s, 0.6 of what a plain GEMM gets from the same power (the GPU is at its 1000 W limit, the SM clock at 1.5 GHz): the
+// softmax bounds it, two warps a scheduler that wait for tensor memory in 900 of 2560 cycles a step.  Steps of 128 keys with one
+// product thread (4 % behind), a later start of the second group, and scores fetched a step ahead (12 % behind) made no gain.
 // 32 trees of 1 to 27 nodes, 7 heads a KV head: 88 to 97 us, 102 with shares in key tiles alone.
 //
 // Narrow kernel (at most 32 rows a unit: single tokens and short drafts).  As rows of a 128-row tile they would leave three
@@ -38,7 +39,7 @@
 // with the 128 keys (the 128 dimensions) as the tile's rows and 32 columns: a quarter of the tensor work, every thread of a
 // group has one key and 32 rows, and the result's rows are written by all of its warps.  The groups take alternate key tiles and
 // have two O each, so that a unit is written while the next one runs (298 -> 289 us at one head a group).  Measured: 32 sequences
-// of 4 nodes at 16384 tokens, 8 KV heads: 326 us, 6.6 TB/s; 128 trees of 8 nodes, 32 KV heads, contexts of 256 to 1024: 289 to 295 us,
+// of 4 nodes at 16384 tokens, 8 KV heads: 326 us, 6.6 TB/s; 128 trees of 8 nodes, 32 KV heads, contexts of 256 to 1024: 297 to 302 us,
 // 4.7 TB/s (6 key tiles a unit: a sixth of the tiles are the trees' own, and a unit's end costs about 4000 cycles).
 #include "common.cuh"
 

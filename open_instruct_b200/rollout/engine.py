@@ -183,7 +183,8 @@ class RolloutEngine:
         # ``speculative_tokens``: drafted tokens per sequence and decode step, at most (0: one token per step, as before).  Steps whose
         # sequences all sample without a nucleus (top_p = 1) and whose drafts are expected to pay are verified steps
         # (``speculative.plan_drafts``).  They run eagerly and over more rows: at 8B with 4 drafts each they take 1.3 times an ordinary
-        # step at 32 sequences, 2.0 at 64, 3.2 at 256, so a sequence has to gain 0.3, 1.0 and 2.2 tokens by them.
+        # step at 32 sequences, 2.0 at 64, 3.2 at 256, so a sequence has to gain 0.3, 1.0 and 2.2 tokens by them.  Verified steps draw
+        # otherwise than ordinary ones, so with drafts a seeded sequence's text depends on the batch it runs in (its distribution does not).
         # ``enable_prefix_caching``: full KV blocks outlive their request and serve later requests that start with the same
         # tokens (multi-turn conversations re-submit their history; the reference reaches this through vLLM's
         # ``enable_prefix_caching``, ``open_instruct/vllm_utils.py:1057-1070``).  Without it only the ``n`` samples of one
